@@ -122,6 +122,10 @@ hipError_t guarded_dev_alloc(void **p, size_t bytes, const char *file, int line,
 }
 
 hipError_t guarded_pin_alloc(void **p, size_t bytes, const char *file, int line, int mode) {
+    // Registering memory that exists is refused on some machines (containers without the right): said once, and from then on pinned blocks are the
+    // runtime's own there -- device memory stays fenced.
+    static std::atomic<bool> refused{false};
+    if (refused.load()) return hipHostMalloc(p, bytes, hipHostMallocDefault);
     const size_t page = (size_t)sysconf(_SC_PAGESIZE);
     Block b;
     b.host = true;
@@ -135,7 +139,12 @@ hipError_t guarded_pin_alloc(void **p, size_t bytes, const char *file, int line,
     if (mprotect(b.map, b.mapped, PROT_READ | PROT_WRITE) != 0) { munmap(va, b.reserved); return hipErrorOutOfMemory; }
     memset(b.map, 0xCB, b.mapped);
     hipError_t e = hipHostRegister(b.map, b.mapped, hipHostRegisterMapped);
-    if (e != hipSuccess) { munmap(va, b.reserved); return e; }
+    if (e != hipSuccess) {
+        (void)hipGetLastError();           // (or the next call's check would report it)
+        munmap(va, b.reserved);
+        if (!refused.exchange(true)) fprintf(stderr, "[shodh guard] hipHostRegister is refused here (%s): pinned host memory is plain hipHostMalloc, without fences\n", hipGetErrorString(e));
+        return hipHostMalloc(p, bytes, hipHostMallocDefault);
+    }
     void *dp = nullptr;
     e = hipHostGetDevicePointer(&dp, b.map, 0);
     if (e != hipSuccess || dp != (void *)b.map) {
