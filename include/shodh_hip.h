@@ -405,6 +405,56 @@ int shodh_int8_dense_quantized(int device, const float *x, const void *wq, uint3
                                uint32_t n_scale, const float *bias, uint32_t M, uint32_t N, uint32_t K, float *y, int32_t *acc_out,
                                float *a_scale, int32_t *a_zp);
 
+/* ---- layer operators of a text tower on device data ------------------------------------------------------------------------------------
+ * The pieces of a layer that newer towers have and the MiniLM encoder above does not: a host that runs such a tower next to the index builds
+ * its layers from these (and finishes the pooled vector with shodh_finalize_pooled). All of them take HIP device pointers, are asynchronous on
+ * `stream` (NULL = default stream of `device`), allocate nothing, keep no state between calls and can be captured into a graph; two calls at
+ * once are two calls. The calling thread's current device is left as it was. Strides count elements; 0 = packed. Rows and offsets are 64 bits. */
+enum { SHODH_DTYPE_FP16 = 3, SHODH_DTYPE_E4M3 = 4 };     /* for these operators; e4m3 = the OCP 8-bit float with largest value 448 */
+
+/* RMS norm with the residual's addition, and an output in 8 bits with scales:
+ *   h = x + residual;  sum = h;  y = h / sqrt(mean(h^2) + eps) * weight;  per group of a row: scale = max |y| / 127 (448), q = round(y / scale)
+ * h, the mean and y are f32 inside; every output is rounded once, to nearest even. x [rows][dim], residual and sum likewise (sum may be residual or x
+ * itself, y may be x: element for element in place). d_residual, d_sum, d_y and d_q + d_scale may be NULL, one output at least is asked for.
+ * q is of `q_dtype` int8 or e4m3, [rows][dim] bytes; d_scale f32 [rows][ceil(dim / q_group)], one a row with q_group 0. A group whose largest
+ * |y| is below 2^-100 is written as scale 0 and zeros; one that holds a NaN or an infinity as scale NaN and zeros: every value reads as NaN. */
+typedef struct {
+    uint64_t rows;
+    uint64_t x_stride, residual_stride, sum_stride, y_stride, q_stride;
+    uint32_t dim;            /* 1 .. 32768 */
+    uint32_t dtype;          /* of x, residual, sum, y: SHODH_DTYPE_FP32, _BF16, _FP16 */
+    uint32_t weight_dtype;   /* fp32, or dtype */
+    uint32_t q_dtype;        /* SHODH_DTYPE_INT8, _E4M3 (read where d_q is given) */
+    uint32_t q_group;        /* 0 = a whole row; 32, 64, 128, 256 */
+    float    eps;            /* 1e-30 or more */
+} shodh_rms_norm_cfg;
+void shodh_rms_norm_cfg_default(shodh_rms_norm_cfg *cfg);      /* bf16, int8 per row, eps 1e-6, packed, sizes 0 */
+int shodh_rms_norm_device(int device, const shodh_rms_norm_cfg *cfg, const void *d_x, const void *d_residual, const void *d_weight, void *d_sum,
+                          void *d_y, void *d_q, float *d_scale, void *stream);
+
+/* Dense layers for few rows on 4-bit weights with group scales (shodh_int8_dense's neighbour for one text or a handful of tokens):
+ *   y[m][n] = sum_k x[m][k] * (q[n][k] - z[n][k / group]) * s[n][k / group] * x_scale[m] + bias[n]
+ * A weight is laid out once; the handle is read-only afterwards (any number of calls at once). q: [N][ceil(K / 2)] bytes, two inputs a byte, the even one
+ * in the low bits; scale f32 [N][ceil(K / group)], kept in `scale_dtype` (fp16 or bf16: values that are numbers of that type already stay what they
+ * are); zero [N][ceil(K / group)] bytes 0 .. 15, NULL = 8 everywhere. group 32, 64 or 128; N and K any.
+ * _create takes host data, _create_device device data (both wait for the device: not for captured streams); _quantize rounds f32 weights itself:
+ * per group scale = max |w| / 7, or (max - min) / 15 with zero points. */
+typedef struct shodh_w4_weight shodh_w4_weight;
+int shodh_w4_weight_create(int device, const uint8_t *q, const float *scale, const uint8_t *zero, uint32_t N, uint32_t K, uint32_t group,
+                           uint32_t scale_dtype, shodh_w4_weight **out);
+int shodh_w4_weight_create_device(int device, const uint8_t *d_q, const float *d_scale, const uint8_t *d_zero, uint32_t N, uint32_t K, uint32_t group,
+                                  uint32_t scale_dtype, void *stream, shodh_w4_weight **out);
+int shodh_w4_weight_quantize(int device, const float *w /* host [N][K] */, uint32_t N, uint32_t K, uint32_t group, uint32_t zeros, uint32_t scale_dtype,
+                             shodh_w4_weight **out);
+void shodh_w4_weight_destroy(shodh_w4_weight *w);          /* no call may be in flight on it */
+int shodh_w4_weight_dequantize(const shodh_w4_weight *w, float *out /* host [N][K] */);
+int shodh_w4_weight_shape(const shodh_w4_weight *w, uint32_t *N, uint32_t *K, uint32_t *group, uint64_t *bytes);
+/* x [rows][K]: fp32 (exact: three bf16 parts), bf16, fp16, or int8 with one f32 scale a row (what shodh_rms_norm_device writes with q_group 0; sums exact in
+ * int32 per group); bias f32 [N] or NULL; y [rows][N] fp32, bf16 or fp16. Any number of rows (made for up to 64: beyond, the weights are read again
+ * for each 64). A row that holds a NaN or an infinity gives NaN in all its outputs; f32 and bf16 rows are taken up to a sum |x| * 31 in f32's range. */
+int shodh_w4_dense_device(const shodh_w4_weight *w, const void *d_x, uint32_t x_dtype, uint64_t x_stride, const float *d_x_scale, uint32_t rows,
+                          const float *d_bias, void *d_y, uint32_t y_dtype, uint64_t y_stride, void *stream);
+
 /* ---- host-side glue of the same path (string / uuid work: stays on the host by design) ------------------ */
 /* MiniLMEmbedder::new_simplified / generate_embedding_simplified (minilm.rs:777-831): SipHash-1-3
  * (DefaultHasher, zero keys) over whitespace words and char bigrams -> dim-d unit vector; zeros if

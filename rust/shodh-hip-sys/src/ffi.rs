@@ -35,6 +35,8 @@ pub const SHODH_WEIGHT_ABSENT: i32 = 0;
 pub const SHODH_WEIGHT_F32: i32 = 1;
 pub const SHODH_WEIGHT_EXPORT_Q8: i32 = 2;
 pub const SHODH_WEIGHT_SELF_Q8: i32 = 3;
+pub const SHODH_DTYPE_FP16: i32 = 3;
+pub const SHODH_DTYPE_E4M3: i32 = 4;
 pub const SHODH_REASON_COMBINED: i32 = 0;
 pub const SHODH_REASON_ENTITY_MATCH: i32 = 1;
 pub const SHODH_REASON_SEMANTIC_SIMILARITY: i32 = 2;
@@ -87,6 +89,21 @@ pub struct shodh_embed_cfg {
     pub weights_path: *const c_char,
 }
 impl Default for shodh_embed_cfg { fn default() -> Self { unsafe { std::mem::zeroed() } } }
+#[repr(C)] #[derive(Clone, Copy, Debug, Default)]
+pub struct shodh_rms_norm_cfg {
+    pub rows: u64,
+    pub x_stride: u64,
+    pub residual_stride: u64,
+    pub sum_stride: u64,
+    pub y_stride: u64,
+    pub q_stride: u64,
+    pub dim: u32,
+    pub dtype: u32,
+    pub weight_dtype: u32,
+    pub q_dtype: u32,
+    pub q_group: u32,
+    pub eps: f32,
+}
 #[repr(C)] #[derive(Clone, Copy, Debug, Default)]
 pub struct shodh_leg_fusion_cfg {
     pub fusion_v2: u8,
@@ -157,6 +174,7 @@ pub struct shodh_relevance_cfg {
 #[repr(C)] pub struct shodh_embedder { _private: [u8; 0] }
 #[repr(C)] pub struct shodh_sharded_index { _private: [u8; 0] }
 #[repr(C)] pub struct shodh_weight_file { _private: [u8; 0] }
+#[repr(C)] pub struct shodh_w4_weight { _private: [u8; 0] }
 
 #[link(name = "shodh_hip")]
 extern "C" {
@@ -256,6 +274,15 @@ extern "C" {
     pub fn shodh_embedder_stage_timings(e: *const shodh_embedder, us2: *mut f32) -> c_int;
     pub fn shodh_int8_dense(device: c_int, x: *const f32, w: *const f32, bias: *const f32, M: u32, N: u32, K: u32, y: *mut f32, acc_out: *mut i32, a_scale: *mut f32, a_zp: *mut i32, w_scale: *mut f32) -> c_int;
     pub fn shodh_int8_dense_quantized(device: c_int, x: *const f32, wq: *const c_void, is_signed: u32, w_scale: *const f32, w_zero_point: *const c_void, n_scale: u32, bias: *const f32, M: u32, N: u32, K: u32, y: *mut f32, acc_out: *mut i32, a_scale: *mut f32, a_zp: *mut i32) -> c_int;
+    pub fn shodh_rms_norm_cfg_default(cfg: *mut shodh_rms_norm_cfg);
+    pub fn shodh_rms_norm_device(device: c_int, cfg: *const shodh_rms_norm_cfg, d_x: *const c_void, d_residual: *const c_void, d_weight: *const c_void, d_sum: *mut c_void, d_y: *mut c_void, d_q: *mut c_void, d_scale: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn shodh_w4_weight_create(device: c_int, q: *const u8, scale: *const f32, zero: *const u8, N: u32, K: u32, group: u32, scale_dtype: u32, out: *mut *mut shodh_w4_weight) -> c_int;
+    pub fn shodh_w4_weight_create_device(device: c_int, d_q: *const u8, d_scale: *const f32, d_zero: *const u8, N: u32, K: u32, group: u32, scale_dtype: u32, stream: *mut c_void, out: *mut *mut shodh_w4_weight) -> c_int;
+    pub fn shodh_w4_weight_quantize(device: c_int, w: *const f32, N: u32, K: u32, group: u32, zeros: u32, scale_dtype: u32, out: *mut *mut shodh_w4_weight) -> c_int;
+    pub fn shodh_w4_weight_destroy(w: *mut shodh_w4_weight);
+    pub fn shodh_w4_weight_dequantize(w: *const shodh_w4_weight, out: *mut f32) -> c_int;
+    pub fn shodh_w4_weight_shape(w: *const shodh_w4_weight, N: *mut u32, K: *mut u32, group: *mut u32, bytes: *mut u64) -> c_int;
+    pub fn shodh_w4_dense_device(w: *const shodh_w4_weight, d_x: *const c_void, x_dtype: u32, x_stride: u64, d_x_scale: *const f32, rows: u32, d_bias: *const f32, d_y: *mut c_void, y_dtype: u32, y_stride: u64, stream: *mut c_void) -> c_int;
     pub fn shodh_hash_embed(utf8: *const c_char, len: usize, dim: u32, out: *mut f32) -> c_int;
     pub fn shodh_finalize_pooled(pooled: *const f32, n: usize, apply_prenorm: c_int, out_dim: usize, out: *mut f32) -> usize;
     pub fn shodh_search_ids_postprocess(vec_ids: *const u32, dists: *const f32, n_res: usize, vector_to_memory: *const u8, n_vectors: usize, limit: usize, out_uuid: *mut u8, out_sim: *mut f32) -> usize;

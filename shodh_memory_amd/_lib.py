@@ -26,6 +26,7 @@ ORDER_SCALAR4, ORDER_AVX2, ORDER_SEQ_1M = 0, 1, 2
 INDEX_FLAT, INDEX_IVFPQ = 0, 1
 SCAN_AUTO, SCAN_EXACT, SCAN_MFMA, SCAN_GRAPH = 0, 1, 2, 3
 DTYPE_FP32, DTYPE_BF16, DTYPE_INT8 = 0, 1, 2
+DTYPE_FP16, DTYPE_E4M3 = 3, 4                       # layer operators only
 QUANT_SCOPE_BATCH, QUANT_SCOPE_PER_TEXT = 0, 1      # shodh_embed_cfg.quant_scope
 WEIGHT_ABSENT, WEIGHT_F32, WEIGHT_EXPORT_Q8, WEIGHT_SELF_Q8 = 0, 1, 2, 3
 
@@ -48,6 +49,12 @@ class EmbedCfg(C.Structure):
                 ("hidden", C.c_uint32), ("layers", C.c_uint32), ("heads", C.c_uint32), ("intermediate", C.c_uint32),
                 ("max_pos", C.c_uint32), ("type_vocab", C.c_uint32), ("ln_eps", C.c_float), ("compute_padded", C.c_uint32),
                 ("quant_scope", C.c_uint32), ("weights_path", C.c_char_p)]
+
+
+class RmsNormCfg(C.Structure):
+    _fields_ = [("rows", C.c_uint64), ("x_stride", C.c_uint64), ("residual_stride", C.c_uint64), ("sum_stride", C.c_uint64), ("y_stride", C.c_uint64),
+                ("q_stride", C.c_uint64), ("dim", C.c_uint32), ("dtype", C.c_uint32), ("weight_dtype", C.c_uint32), ("q_dtype", C.c_uint32),
+                ("q_group", C.c_uint32), ("eps", C.c_float)]
 
 
 class Weights(C.Structure):
@@ -181,6 +188,15 @@ SYMBOLS = {
                                              C.POINTER(C.c_float), C.POINTER(C.c_int32)]),
     "shodh_embed_param_count": (C.c_uint64, [C.POINTER(EmbedCfg)]),
     "shodh_embedder_synthetic_weights": (C.c_int, [C.POINTER(EmbedCfg), C.c_uint64, _fp, C.c_uint64]),
+    "shodh_rms_norm_cfg_default": (None, [C.POINTER(RmsNormCfg)]),
+    "shodh_rms_norm_device": (C.c_int, [C.c_int, C.POINTER(RmsNormCfg), _vp, _vp, _vp, _vp, _vp, _vp, _fp, _vp]),
+    "shodh_w4_weight_create": (C.c_int, [C.c_int, _u8p, _fp, _u8p, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.POINTER(C.c_void_p)]),
+    "shodh_w4_weight_create_device": (C.c_int, [C.c_int, _u8p, _fp, _u8p, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, _vp, C.POINTER(C.c_void_p)]),
+    "shodh_w4_weight_quantize": (C.c_int, [C.c_int, _fp, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.POINTER(C.c_void_p)]),
+    "shodh_w4_weight_destroy": (None, [_vp]),
+    "shodh_w4_weight_dequantize": (C.c_int, [_vp, _fp]),
+    "shodh_w4_weight_shape": (C.c_int, [_vp, C.POINTER(C.c_uint32), C.POINTER(C.c_uint32), C.POINTER(C.c_uint32), C.POINTER(C.c_uint64)]),
+    "shodh_w4_dense_device": (C.c_int, [_vp, _vp, C.c_uint32, C.c_uint64, _fp, C.c_uint32, _fp, _vp, C.c_uint32, C.c_uint64, _vp]),
     "shodh_hash_embed": (C.c_int, [C.c_char_p, C.c_size_t, C.c_uint32, _fp]),
     "shodh_finalize_pooled": (C.c_size_t, [_fp, C.c_size_t, C.c_int, C.c_size_t, _fp]),
     "shodh_search_ids_postprocess": (C.c_size_t, [_u32p, _fp, C.c_size_t, _u8p, C.c_size_t, C.c_size_t, _u8p, _fp]),

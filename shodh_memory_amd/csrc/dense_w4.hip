@@ -1,0 +1,490 @@
+// dense_w4.hip -- dense layers for few rows on 4-bit weights with group scales (and zero points).
+//
+//   y[m][n] = (sum_k x[m][k] * (q[n][k] - z[n][g]) * s[n][g]) * x_scale[m] + bias[n],   g = k / group, q and z in 0 .. 15
+//
+// Bound: the weights' bytes (half a byte a weight) for up to 64 rows; a launch for small layers. Everything follows from that:
+//  * weights are laid out once, in records of 16 outputs x 128 inputs (1 KiB of 4-bit numbers, 16 B a lane, then the record's scales and zero
+//    points): a wave's load of a record is one contiguous KiB and lands where the matrix instruction wants it;
+//  * a 4-bit number becomes a matrix operand with a shift and an and-or per PAIR: or-ed into the mantissa of 16.0 it reads as 16 + q, in bf16 as in
+//    fp16, exactly. sum x (16 + q) - (16 + z) sum x is the group's sum; sum x comes from the same matrix instruction with ones for weights, in the same
+//    order. int8 rows multiply q as a byte: sums exact in int32, (q - z) likewise;
+//  * f32 rows are split into three bf16 parts (8 + 8 + 8 bits, by truncation, exact): three products, sums in f32;
+//  * scales multiply the f32 sum of a group, so no weight is rounded to 16 bits on the way.
+// A row of x that holds a NaN or an infinity gives NaN in all its outputs (16 x - 16 x).
+#include "layers.h"
+
+#include <new>
+#include <vector>
+
+#pragma clang fp contract(off)
+
+struct shodh_w4_weight {
+    int device = 0;
+    uint32_t N = 0, K = 0, group = 0, scale_dtype = 0, zeros = 0, tiles = 0, blocks = 0, record = 0;
+    uint8_t *data = nullptr;
+};
+
+namespace shodh {
+
+constexpr int W4_TN = 16, W4_TK = 128;        // outputs and inputs of a record
+
+static uint32_t record_bytes(uint32_t group, bool zeros) { return 1024u + (W4_TK / group) * (32u + (zeros ? 16u : 0u)); }
+
+// ---- laying out -----------------------------------------------------------------------------------------------------------------
+// Record: [lane 64][step 4] words; word (lane, step) holds inputs 32 step + 8 (lane >> 4) + e, e = 0 .. 7, of output lane & 15, element e in the 4 bits
+// number (e >> 1) + 4 (e & 1): a shift by 4 i and a mask leave elements 2 i and 2 i + 1 in the two halves of the word. Then [group][16 outputs] scales of
+// two bytes, then [group][16] bytes 16 + z.
+template <class S>
+__global__ __launch_bounds__(256) void w4_pack_kernel(const uint8_t *__restrict__ q, const float *__restrict__ scale, const uint8_t *__restrict__ zero, uint32_t N, uint32_t K,
+                                                      uint32_t group, uint32_t blocks, uint32_t record, uint8_t *__restrict__ out, uint32_t *__restrict__ bad) {
+    const uint32_t tile = blockIdx.y, block = blockIdx.x, t = threadIdx.x;
+    uint8_t *rec = out + ((size_t)tile * blocks + block) * record;
+    const uint32_t lane = t >> 2, step = t & 3, n = tile * W4_TN + (lane & 15), k0 = block * W4_TK + 32 * step + 8 * (lane >> 4);
+    const size_t pitch = (K + 1) / 2;
+    uint32_t word = 0;
+    for (uint32_t e = 0; e < 8; ++e) {
+        uint32_t v = 0;          // (behind the matrix: x reads as zero there, or the output is not written)
+        if (n < N && k0 + e < K) { const uint32_t b = q[n * pitch + ((k0 + e) >> 1)]; v = ((k0 + e) & 1) ? b >> 4 : b & 15u; }
+        word |= v << (4 * ((e >> 1) + 4 * (e & 1)));
+    }
+    reinterpret_cast<uint32_t *>(rec)[t] = word;
+    const uint32_t per = W4_TK / group, groups = (K + group - 1) / group;
+    if (t < per * 16) {
+        const uint32_t gl = t >> 4, g = block * per + gl, m = tile * W4_TN + (t & 15);
+        const bool in = m < N && g < groups;
+        const float s = in ? scale[(size_t)m * groups + g] : 0.0f;
+        const S r = (S)s;
+        if (!(__builtin_fabsf((float)r) < __builtin_inff())) atomicOr(bad, 1u);
+        reinterpret_cast<S *>(rec + 1024)[t] = r;
+        if (zero) {
+            const uint32_t z = in ? zero[(size_t)m * groups + g] : 8u;
+            if (z > 15u) atomicOr(bad, 2u);
+            rec[1024 + per * 32 + t] = (uint8_t)(16u + (z & 15u));
+        }
+    }
+}
+
+// a group's scale and zero point from its floats (one wave a group), then its 4-bit numbers
+template <class S>
+__global__ __launch_bounds__(64) void w4_quantize_kernel(const float *__restrict__ w, uint32_t N, uint32_t K, uint32_t group, uint32_t zeros, uint8_t *__restrict__ q /* one a byte */,
+                                                         float *__restrict__ scale, uint8_t *__restrict__ zero, uint32_t *__restrict__ bad) {
+    const uint32_t groups = (K + group - 1) / group, g = blockIdx.x, n = blockIdx.y + gridDim.y * blockIdx.z;
+    if (n >= N) return;
+    const uint32_t k0 = g * group, k1 = min(K, k0 + group);
+    float lo = 0.0f, hi = 0.0f;
+    bool odd = false;
+    for (uint32_t k = k0 + threadIdx.x; k < k1; k += 64) {
+        const float v = w[(size_t)n * K + k];
+        odd |= !(__builtin_fabsf(v) < __builtin_inff());
+        lo = fminf(lo, v); hi = fmaxf(hi, v);
+    }
+    for (int o = 32; o > 0; o >>= 1) { lo = fminf(lo, __shfl_xor(lo, o)); hi = fmaxf(hi, __shfl_xor(hi, o)); }
+    if (odd) atomicOr(bad, 4u);
+    const float s = (float)(S)(zeros ? (hi - lo) / 15.0f : fmaxf(-lo, hi) / 7.0f);
+    const bool none = !(s > 0.0f);
+    const float z = zeros ? (none ? 0.0f : fminf(fmaxf(__builtin_rintf(-lo / s), 0.0f), 15.0f)) : 8.0f;
+    for (uint32_t k = k0 + threadIdx.x; k < k1; k += 64) {
+        const float v = none ? z : __builtin_rintf(w[(size_t)n * K + k] / s) + z;
+        q[(size_t)n * K + k] = (uint8_t)(int)fminf(fmaxf(v, 0.0f), 15.0f);
+    }
+    if (threadIdx.x == 0) { scale[(size_t)n * groups + g] = s; if (zeros) zero[(size_t)n * groups + g] = (uint8_t)(int)z; }
+}
+__global__ __launch_bounds__(256) void w4_pairs_kernel(const uint8_t *__restrict__ q, uint32_t N, uint32_t K, uint8_t *__restrict__ out) {
+    const size_t pitch = (K + 1) / 2, total = (size_t)N * pitch;
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (size_t)gridDim.x * 256) {
+        const size_t n = i / pitch, k = (i - n * pitch) * 2;
+        const uint32_t lo = q[n * K + k], hi = k + 1 < K ? q[n * K + k + 1] : 0u;
+        out[i] = (uint8_t)(lo | (hi << 4));
+    }
+}
+template <class S>
+__global__ __launch_bounds__(256) void w4_unpack_kernel(const uint8_t *__restrict__ data, uint32_t N, uint32_t K, uint32_t group, uint32_t blocks, uint32_t record, uint32_t zeros,
+                                                        float *__restrict__ out) {
+    const uint32_t tile = blockIdx.y, block = blockIdx.x, t = threadIdx.x;
+    const uint8_t *rec = data + ((size_t)tile * blocks + block) * record;
+    const uint32_t lane = t >> 2, step = t & 3, n = tile * W4_TN + (lane & 15), kk = 32 * step + 8 * (lane >> 4), per = W4_TK / group;
+    const uint32_t word = reinterpret_cast<const uint32_t *>(rec)[t];
+    for (uint32_t e = 0; e < 8; ++e) {
+        const uint32_t k = block * W4_TK + kk + e, g = (kk + e) / group;
+        if (n >= N || k >= K) continue;
+        const float v = (float)((word >> (4 * ((e >> 1) + 4 * (e & 1)))) & 15u);
+        const float z = zeros ? (float)rec[1024 + per * 32 + g * 16 + (n & 15)] - 16.0f : 8.0f;
+        out[(size_t)n * K + k] = (v - z) * (float)reinterpret_cast<const S *>(rec + 1024)[g * 16 + (n & 15)];
+    }
+}
+
+// ---- the product ------------------------------------------------------------------------------------------------------------------
+struct W4Args {
+    const uint8_t *w;
+    const void *x;
+    const float *x_scale, *bias;
+    void *y;
+    uint64_t x_stride, y_stride;
+    uint32_t M, N, K, blocks, record, y_dtype, scale_f16, zeros;
+};
+
+enum { W4_BF16 = 0, W4_F16 = 1, W4_F32 = 2, W4_I8 = 3 };      // type of x
+
+// One lane's 8 neighbouring inputs of one row as matrix operands: one for 16-bit types and int8, three for f32.
+template <int X> struct XFrag;
+template <> struct XFrag<W4_BF16> { static constexpr int P = 1; using E = __bf16; u32x4 v[1]; };
+template <> struct XFrag<W4_F16> { static constexpr int P = 1; using E = _Float16; u32x4 v[1]; };
+template <> struct XFrag<W4_F32> { static constexpr int P = 3; using E = float; u32x4 v[3]; };
+template <> struct XFrag<W4_I8> { static constexpr int P = 1; using E = int8_t; u32x2 v[1]; };
+
+template <int X>
+__device__ __forceinline__ void x_convert(XFrag<X> &f, const typename XFrag<X>::E (&e)[8]) {
+    if constexpr (X == W4_BF16 || X == W4_F16) __builtin_memcpy(&f.v[0], e, 16);
+    else if constexpr (X == W4_F32) {
+        uint32_t u[3][8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t b0 = __float_as_uint(e[i]);
+            const float r1 = e[i] - __uint_as_float(b0 & 0xFFFF0000u);
+            const uint32_t b1 = __float_as_uint(r1);
+            const float r2 = r1 - __uint_as_float(b1 & 0xFFFF0000u);
+            u[0][i] = b0; u[1][i] = b1; u[2][i] = __float_as_uint(r2);
+        }
+#pragma unroll
+        for (int p = 0; p < 3; ++p)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f.v[p][i] = __builtin_amdgcn_perm(u[p][2 * i + 1], u[p][2 * i], 0x07060302u);     // the high halves of two words
+    } else {
+        // in the order in which a word of 4-bit numbers leaves its bytes: 0 4 1 5 | 2 6 3 7
+        uint32_t lo, hi;
+        __builtin_memcpy(&lo, e, 4);
+        __builtin_memcpy(&hi, e + 4, 4);
+        f.v[0][0] = __builtin_amdgcn_perm(hi, lo, 0x05010400u);
+        f.v[0][1] = __builtin_amdgcn_perm(hi, lo, 0x07030602u);
+    }
+}
+template <int X>
+__device__ __forceinline__ void x_load(XFrag<X> &f, const typename XFrag<X>::E *p, uint32_t n /* elements in the row from here on */) {
+    typename XFrag<X>::E e[8];
+    if (n >= 8) load_any(e, p);
+    else
+        for (int i = 0; i < 8; ++i) e[i] = (uint32_t)i < n ? p[i] : (typename XFrag<X>::E)0;
+    x_convert<X>(f, e);
+}
+
+template <int X> struct WFrag { u32x4 v; };
+template <> struct WFrag<W4_I8> { u32x2 v; };
+template <int X>
+__device__ __forceinline__ WFrag<X> w_expand(uint32_t w) {
+    WFrag<X> f;
+    if constexpr (X == W4_I8) { f.v[0] = w & 0x0F0F0F0Fu; f.v[1] = (w >> 4) & 0x0F0F0F0Fu; }
+    else if constexpr (X == W4_F16) {
+        f.v[0] = ((w << 6) & 0x03C003C0u) | 0x4C004C00u; f.v[1] = ((w << 2) & 0x03C003C0u) | 0x4C004C00u;
+        f.v[2] = ((w >> 2) & 0x03C003C0u) | 0x4C004C00u; f.v[3] = ((w >> 6) & 0x03C003C0u) | 0x4C004C00u;
+    } else {
+        f.v[0] = ((w << 3) & 0x00780078u) | 0x41804180u; f.v[1] = ((w >> 1) & 0x00780078u) | 0x41804180u;
+        f.v[2] = ((w >> 5) & 0x00780078u) | 0x41804180u; f.v[3] = ((w >> 9) & 0x00780078u) | 0x41804180u;
+    }
+    return f;
+}
+template <int X>
+__device__ __forceinline__ WFrag<X> w_ones() {
+    WFrag<X> f;
+    const uint32_t one = X == W4_I8 ? 0x01010101u : X == W4_F16 ? 0x3C003C00u : 0x3F803F80u;
+    for (int i = 0; i < (X == W4_I8 ? 2 : 4); ++i) f.v[i] = one;
+    return f;
+}
+template <int X> struct Acc { using V = f32x4; };
+template <> struct Acc<W4_I8> { using V = i32x4; };
+template <int X>
+__device__ __forceinline__ typename Acc<X>::V mma(const WFrag<X> &a, const XFrag<X> &b, typename Acc<X>::V c) {
+    if constexpr (X == W4_I8) return __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, a.v), __builtin_bit_cast(long, b.v[0]), c, 0, 0, 0);
+    else if constexpr (X == W4_F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a.v), __builtin_bit_cast(f16x8, b.v[0]), c, 0, 0, 0);
+    else {
+#pragma unroll
+        for (int p = XFrag<X>::P - 1; p >= 0; --p) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a.v), __builtin_bit_cast(bf16x8, b.v[p]), c, 0, 0, 0);
+        return c;
+    }
+}
+
+// A workgroup of `waves` waves: 16 outputs, MT x 16 rows; wave i takes the records i, i + waves, ... of its outputs, and the waves' sums are added in
+// their order. Matrix layouts: operand lane = output (weights) or row (x) lane & 15, inputs 8 (lane >> 4) ..; result lane = row lane & 15,
+// outputs 4 (lane >> 4) .. + 3.
+template <int X, int GROUP, int MT>
+__global__ __launch_bounds__(512) void w4_dense_kernel(const W4Args a) {
+    using F = XFrag<X>;
+    using E = typename F::E;
+    using V = typename Acc<X>::V;
+    extern __shared__ float sums[];              // [waves][MT][64][4]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, quad = lane >> 4;
+    const uint32_t m0 = blockIdx.y * 64u;
+    constexpr int PER = W4_TK / GROUP, STEPS = GROUP / 32;       // groups of a record; steps of 32 inputs of a group
+    const E *xr[MT];
+    bool in[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const uint32_t m = m0 + i * 16 + (lane & 15);
+        in[i] = m < a.M;
+        xr[i] = (const E *)a.x + (uint64_t)(in[i] ? m : 0) * a.x_stride + 8 * quad;
+    }
+    f32x4 acc[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[i] = f32x4{0, 0, 0, 0};
+    const WFrag<X> ones = w_ones<X>();
+    const uint8_t *rec = a.w + ((size_t)blockIdx.x * a.blocks + wave) * a.record;
+    for (uint32_t block = wave; block < a.blocks; block += waves, rec += (size_t)waves * a.record) {
+        const u32x4 w = *reinterpret_cast<const u32x4 *>(rec + lane * 16);
+        const uint32_t k0 = block * W4_TK + 8 * quad;
+#pragma unroll
+        for (int g = 0; g < PER; ++g) {
+            V d[MT], s[MT];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) { d[i] = V{0, 0, 0, 0}; s[i] = V{0, 0, 0, 0}; }
+#pragma unroll
+            for (int j = 0; j < STEPS; ++j) {
+                const int step = g * STEPS + j;
+                const uint32_t k = k0 + 32 * step;
+                const WFrag<X> wf = w_expand<X>(w[step]);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    F xf;
+                    x_load<X>(xf, xr[i] + block * W4_TK + 32 * step, in[i] && k < a.K ? a.K - k : 0);
+                    d[i] = mma<X>(wf, xf, d[i]);
+                    s[i] = mma<X>(ones, xf, s[i]);
+                }
+            }
+            float scale[4], zero[4];
+            {
+                const u32x2 raw = *reinterpret_cast<const u32x2 *>(rec + 1024 + g * 32 + quad * 8);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const uint16_t h = (uint16_t)(raw[r >> 1] >> (16 * (r & 1)));
+                    scale[r] = a.scale_f16 ? (float)__builtin_bit_cast(_Float16, h) : __uint_as_float((uint32_t)h << 16);
+                }
+                const uint32_t zb = a.zeros ? *reinterpret_cast<const uint32_t *>(rec + 1024 + PER * 32 + g * 16 + quad * 4) : 0x18181818u;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) zero[r] = (float)((zb >> (8 * r)) & 255u);
+            }
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float v;
+                    if constexpr (X == W4_I8) v = (float)(d[i][r] - ((int)zero[r] - 16) * s[i][r]);
+                    else v = __builtin_fmaf(-zero[r], s[i][r], d[i][r]);
+                    acc[i][r] = __builtin_fmaf(v, scale[r], acc[i][r]);
+                }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) *reinterpret_cast<f32x4 *>(sums + ((wave * MT + i) * 64 + lane) * 4) = acc[i];
+    __syncthreads();
+    for (int e = threadIdx.x; e < MT * 64; e += blockDim.x) {
+        f32x4 v = *reinterpret_cast<const f32x4 *>(sums + e * 4);
+        for (int w2 = 1; w2 < waves; ++w2) v += *reinterpret_cast<const f32x4 *>(sums + (w2 * MT * 64 + e) * 4);
+        const uint32_t m = m0 + (e >> 6) * 16 + (e & 15), n = blockIdx.x * W4_TN + ((e & 63) >> 4) * 4;
+        if (m >= a.M || n >= a.N) continue;
+        const float xs = X == W4_I8 ? a.x_scale[m] : 1.0f;
+        float o[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[r] = (X == W4_I8 ? v[r] * xs : v[r]) + (a.bias && n + r < a.N ? a.bias[n + r] : 0.0f);
+        const uint64_t at = (uint64_t)m * a.y_stride + n;
+        auto put = [&](auto *y) {
+            using Y = std::remove_reference_t<decltype(*y)>;
+            Y t[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) t[r] = (Y)o[r];
+            if (n + 4 <= a.N) store_any(y + at, t);
+            else
+                for (int r = 0; r < 4; ++r) if (n + r < a.N) y[at + r] = t[r];
+        };
+        if (a.y_dtype == SHODH_DTYPE_FP32) put((float *)a.y);
+        else if (a.y_dtype == SHODH_DTYPE_BF16) put((__bf16 *)a.y);
+        else put((_Float16 *)a.y);
+    }
+}
+
+template <int X, int GROUP>
+static int launch_w4(const W4Args &a, uint32_t tiles, hipStream_t st) {
+    const uint32_t waves = a.blocks >= 8 ? 8 : a.blocks >= 4 ? 4 : a.blocks >= 2 ? 2 : 1;
+    auto go = [&](auto kern, int mt) {
+        hipLaunchKernelGGL(kern, dim3(tiles, (a.M + 63) / 64), dim3(64 * waves), (size_t)waves * mt * 1024, st, a);
+    };
+    if (a.M <= 16) go(w4_dense_kernel<X, GROUP, 1>, 1);
+    else if (a.M <= 32) go(w4_dense_kernel<X, GROUP, 2>, 2);
+    else go(w4_dense_kernel<X, GROUP, 4>, 4);
+    SHODH_HIP_TRY(hipGetLastError());
+    return SHODH_OK;
+}
+template <int X>
+static int pick_w4(const W4Args &a, const shodh_w4_weight *w, hipStream_t st) {
+    return w->group == 32 ? launch_w4<X, 32>(a, w->tiles, st) : w->group == 64 ? launch_w4<X, 64>(a, w->tiles, st) : launch_w4<X, 128>(a, w->tiles, st);
+}
+
+static int check_w4(uint32_t N, uint32_t K, uint32_t group, uint32_t scale_dtype, shodh_w4_weight **out) {
+    if (!out) { set_error("null argument"); return SHODH_ERR_INVALID; }
+    *out = nullptr;
+    if (N == 0 || K == 0 || N > (1u << 20) - 16 || K > (1u << 24)) { set_error("w4: %u outputs, %u inputs out of range (1 .. 1048560, 1 .. 16777216)", N, K); return SHODH_ERR_INVALID; }
+    if (group != 32 && group != 64 && group != 128) { set_error("w4: group %u is none of 32, 64, 128", group); return SHODH_ERR_UNSUPPORTED; }
+    if (scale_dtype != SHODH_DTYPE_FP16 && scale_dtype != SHODH_DTYPE_BF16) { set_error("w4: scales are kept in fp16 or bf16 (got dtype %u)", scale_dtype); return SHODH_ERR_INVALID; }
+    return SHODH_OK;
+}
+
+// `q` packed two to a byte, `scale`, `zero`: device data. Waits for the stream: the handle is ready when the call returns.
+static int lay_out(int device, const uint8_t *q, const float *scale, const uint8_t *zero, uint32_t N, uint32_t K, uint32_t group, uint32_t scale_dtype, uint32_t *d_bad,
+                   hipStream_t st, shodh_w4_weight **out) {
+    shodh_w4_weight *w = new (std::nothrow) shodh_w4_weight();
+    if (!w) { set_error("out of memory"); return SHODH_ERR_OOM; }
+    w->device = device; w->N = N; w->K = K; w->group = group; w->scale_dtype = scale_dtype; w->zeros = zero != nullptr;
+    w->tiles = (N + W4_TN - 1) / W4_TN; w->blocks = (K + W4_TK - 1) / W4_TK; w->record = record_bytes(group, w->zeros);
+    if (dev_alloc(&w->data, (size_t)w->tiles * w->blocks * w->record) != hipSuccess) { (void)hipGetLastError(); delete w; set_error("out of HBM for 4-bit weights"); return SHODH_ERR_OOM; }
+    const dim3 grid(w->blocks, w->tiles);
+    if (scale_dtype == SHODH_DTYPE_FP16) hipLaunchKernelGGL((w4_pack_kernel<_Float16>), grid, dim3(256), 0, st, q, scale, zero, N, K, group, w->blocks, w->record, w->data, d_bad);
+    else hipLaunchKernelGGL((w4_pack_kernel<__bf16>), grid, dim3(256), 0, st, q, scale, zero, N, K, group, w->blocks, w->record, w->data, d_bad);
+    uint32_t bad = 0;
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess) e = hipMemcpyAsync(&bad, d_bad, 4, hipMemcpyDeviceToHost, st);
+    if (e == hipSuccess) e = hipStreamSynchronize(st);
+    if (e != hipSuccess || bad) {
+        (void)dev_free(w->data); delete w;
+        if (e != hipSuccess) { set_error("w4: laying out failed: %s", hipGetErrorString(e)); return SHODH_ERR_DEVICE; }
+        if (bad & 2u) { set_error("w4: a zero point is over 15"); return SHODH_ERR_INVALID; }
+        set_error(bad & 4u ? "w4: a weight is a NaN or an infinity" : "w4: a scale is no finite number of its 16-bit type"); return SHODH_ERR_NONFINITE;
+    }
+    *out = w;
+    return SHODH_OK;
+}
+
+struct Buffers {           // device scratch of one create call
+    std::vector<void *> held;
+    template <class T> T *take(size_t n) {
+        void *p = nullptr;
+        if (dev_alloc(&p, n * sizeof(T)) != hipSuccess) { (void)hipGetLastError(); return nullptr; }
+        held.push_back(p);
+        return (T *)p;
+    }
+    ~Buffers() { for (void *p : held) (void)dev_free(p); }
+};
+
+}  // namespace shodh
+
+using namespace shodh;
+
+extern "C" {
+
+int shodh_w4_weight_create_device(int device, const uint8_t *d_q, const float *d_scale, const uint8_t *d_zero, uint32_t N, uint32_t K, uint32_t group, uint32_t scale_dtype,
+                                  void *stream, shodh_w4_weight **out) {
+    SHODH_TRY(check_w4(N, K, group, scale_dtype, out));
+    if (!d_q || !d_scale) { set_error("null argument"); return SHODH_ERR_INVALID; }
+    DeviceScope scope;
+    SHODH_TRY(scope.enter(device));
+    try {
+        Buffers b;
+        uint32_t *bad = b.take<uint32_t>(1);
+        if (!bad) { set_error("out of HBM"); return SHODH_ERR_OOM; }
+        SHODH_HIP_TRY(hipMemsetAsync(bad, 0, 4, (hipStream_t)stream));
+        return lay_out(device, d_q, d_scale, d_zero, N, K, group, scale_dtype, bad, (hipStream_t)stream, out);
+    } catch (const std::exception &ex) { set_error("w4: %s", ex.what()); return SHODH_ERR_OOM; }
+}
+
+int shodh_w4_weight_create(int device, const uint8_t *q, const float *scale, const uint8_t *zero, uint32_t N, uint32_t K, uint32_t group, uint32_t scale_dtype, shodh_w4_weight **out) {
+    SHODH_TRY(check_w4(N, K, group, scale_dtype, out));
+    if (!q || !scale) { set_error("null argument"); return SHODH_ERR_INVALID; }
+    DeviceScope scope;
+    SHODH_TRY(scope.enter(device));
+    try {
+        Buffers b;
+        const size_t nq = (size_t)N * ((K + 1) / 2), ng = (size_t)N * ((K + group - 1) / group);
+        uint8_t *dq = b.take<uint8_t>(nq), *dz = zero ? b.take<uint8_t>(ng) : nullptr;
+        float *ds = b.take<float>(ng);
+        if (!dq || !ds || (zero && !dz)) { set_error("out of HBM"); return SHODH_ERR_OOM; }
+        SHODH_HIP_TRY(hipMemcpy(dq, q, nq, hipMemcpyHostToDevice));
+        SHODH_HIP_TRY(hipMemcpy(ds, scale, ng * 4, hipMemcpyHostToDevice));
+        if (zero) SHODH_HIP_TRY(hipMemcpy(dz, zero, ng, hipMemcpyHostToDevice));
+        return shodh_w4_weight_create_device(device, dq, ds, dz, N, K, group, scale_dtype, nullptr, out);
+    } catch (const std::exception &ex) { set_error("w4: %s", ex.what()); return SHODH_ERR_OOM; }
+}
+
+int shodh_w4_weight_quantize(int device, const float *w, uint32_t N, uint32_t K, uint32_t group, uint32_t zeros, uint32_t scale_dtype, shodh_w4_weight **out) {
+    SHODH_TRY(check_w4(N, K, group, scale_dtype, out));
+    if (!w) { set_error("null argument"); return SHODH_ERR_INVALID; }
+    DeviceScope scope;
+    SHODH_TRY(scope.enter(device));
+    try {
+        Buffers b;
+        const size_t n = (size_t)N * K, ng = (size_t)N * ((K + group - 1) / group), pairs = (size_t)N * ((K + 1) / 2);
+        float *dw = b.take<float>(n), *ds = b.take<float>(ng);
+        uint8_t *d1 = b.take<uint8_t>(n), *dq = b.take<uint8_t>(pairs), *dz = zeros ? b.take<uint8_t>(ng) : nullptr;
+        uint32_t *bad = b.take<uint32_t>(1);
+        if (!dw || !ds || !d1 || !dq || (zeros && !dz) || !bad) { set_error("out of HBM"); return SHODH_ERR_OOM; }
+        SHODH_HIP_TRY(hipMemcpy(dw, w, n * 4, hipMemcpyHostToDevice));
+        SHODH_HIP_TRY(hipMemset(bad, 0, 4));
+        const uint32_t ny = N < 32768 ? N : 32768;
+        const dim3 grid((K + group - 1) / group, ny, (N + ny - 1) / ny);
+        if (scale_dtype == SHODH_DTYPE_FP16) hipLaunchKernelGGL((w4_quantize_kernel<_Float16>), grid, dim3(64), 0, nullptr, dw, N, K, group, zeros, d1, ds, dz, bad);
+        else hipLaunchKernelGGL((w4_quantize_kernel<__bf16>), grid, dim3(64), 0, nullptr, dw, N, K, group, zeros, d1, ds, dz, bad);
+        hipLaunchKernelGGL(w4_pairs_kernel, dim3((uint32_t)(ceil_div(pairs, 256) < 8192 ? ceil_div(pairs, 256) : 8192)), dim3(256), 0, nullptr, d1, N, K, dq);
+        SHODH_HIP_TRY(hipGetLastError());
+        return lay_out(device, dq, ds, dz, N, K, group, scale_dtype, bad, nullptr, out);
+    } catch (const std::exception &ex) { set_error("w4: %s", ex.what()); return SHODH_ERR_OOM; }
+}
+
+void shodh_w4_weight_destroy(shodh_w4_weight *w) {
+    if (!w) return;
+    DeviceScope scope;
+    if (scope.enter(w->device) == SHODH_OK) (void)dev_free(w->data);
+    delete w;
+}
+
+int shodh_w4_weight_dequantize(const shodh_w4_weight *w, float *out) {
+    if (!w || !out) { set_error("null argument"); return SHODH_ERR_INVALID; }
+    DeviceScope scope;
+    SHODH_TRY(scope.enter(w->device));
+    try {
+        Buffers b;
+        const size_t n = (size_t)w->N * w->K;
+        float *d = b.take<float>(n);
+        if (!d) { set_error("out of HBM"); return SHODH_ERR_OOM; }
+        const dim3 grid(w->blocks, w->tiles);
+        if (w->scale_dtype == SHODH_DTYPE_FP16) hipLaunchKernelGGL((w4_unpack_kernel<_Float16>), grid, dim3(256), 0, nullptr, w->data, w->N, w->K, w->group, w->blocks, w->record, w->zeros, d);
+        else hipLaunchKernelGGL((w4_unpack_kernel<__bf16>), grid, dim3(256), 0, nullptr, w->data, w->N, w->K, w->group, w->blocks, w->record, w->zeros, d);
+        SHODH_HIP_TRY(hipGetLastError());
+        SHODH_HIP_TRY(hipMemcpy(out, d, n * 4, hipMemcpyDeviceToHost));
+        return SHODH_OK;
+    } catch (const std::exception &ex) { set_error("w4: %s", ex.what()); return SHODH_ERR_OOM; }
+}
+
+int shodh_w4_weight_shape(const shodh_w4_weight *w, uint32_t *N, uint32_t *K, uint32_t *group, uint64_t *bytes) {
+    if (!w) { set_error("null argument"); return SHODH_ERR_INVALID; }
+    if (N) *N = w->N;
+    if (K) *K = w->K;
+    if (group) *group = w->group;
+    if (bytes) *bytes = (uint64_t)w->tiles * w->blocks * w->record;
+    return SHODH_OK;
+}
+
+int shodh_w4_dense_device(const shodh_w4_weight *w, const void *d_x, uint32_t x_dtype, uint64_t x_stride, const float *d_x_scale, uint32_t rows, const float *d_bias, void *d_y,
+                          uint32_t y_dtype, uint64_t y_stride, void *stream) {
+    if (!w) { set_error("null argument"); return SHODH_ERR_INVALID; }
+    if (!is_float_dtype(x_dtype) && x_dtype != SHODH_DTYPE_INT8) { set_error("w4: x of dtype %u: fp32, bf16, fp16 or int8 are taken", x_dtype); return SHODH_ERR_INVALID; }
+    if (!is_float_dtype(y_dtype)) { set_error("w4: y of dtype %u: fp32, bf16 or fp16", y_dtype); return SHODH_ERR_INVALID; }
+    if (rows == 0) return SHODH_OK;
+    if (!d_x || !d_y) { set_error("null argument"); return SHODH_ERR_INVALID; }
+    if ((x_dtype == SHODH_DTYPE_INT8) != (d_x_scale != nullptr)) { set_error("w4: int8 rows come with a scale each, others with none"); return SHODH_ERR_INVALID; }
+    const uint64_t xs = x_stride ? x_stride : w->K, ys = y_stride ? y_stride : w->N;
+    if (rows > 1 && ys < w->N) { set_error("w4: y's rows overlap (stride %llu below %u)", (unsigned long long)ys, w->N); return SHODH_ERR_DIM; }
+    if (rows > 64u * 65535u) { set_error("w4: %u rows: at most 4194240", rows); return SHODH_ERR_UNSUPPORTED; }
+    if (!aligned_to(d_x, dtype_bytes(x_dtype)) || !aligned_to(d_y, dtype_bytes(y_dtype)) || !aligned_to(d_x_scale, 4) || !aligned_to(d_bias, 4)) {
+        set_error("w4: a pointer is not a multiple of its element's size"); return SHODH_ERR_INVALID;
+    }
+    DeviceScope scope;
+    SHODH_TRY(scope.enter(w->device));
+    W4Args a;
+    a.w = w->data; a.x = d_x; a.x_scale = d_x_scale; a.bias = d_bias; a.y = d_y; a.x_stride = xs; a.y_stride = ys;
+    a.M = rows; a.N = w->N; a.K = w->K; a.blocks = w->blocks; a.record = w->record; a.y_dtype = y_dtype;
+    a.scale_f16 = w->scale_dtype == SHODH_DTYPE_FP16; a.zeros = w->zeros;
+    hipStream_t st = (hipStream_t)stream;
+    switch (x_dtype) {
+        case SHODH_DTYPE_BF16: return pick_w4<W4_BF16>(a, w, st);
+        case SHODH_DTYPE_FP16: return pick_w4<W4_F16>(a, w, st);
+        case SHODH_DTYPE_FP32: return pick_w4<W4_F32>(a, w, st);
+        default: return pick_w4<W4_I8>(a, w, st);
+    }
+}
+
+}  // extern "C"

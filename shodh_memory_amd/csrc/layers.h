@@ -1,0 +1,46 @@
+// layers.h -- what the layer operators on device data share (rms_norm.hip, dense_w4.hip, window_attention.hip): element types, loads of any
+// alignment, and the two checks every entry point makes.
+#pragma once
+#include "common.h"
+
+namespace shodh {
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// A vector of N elements at an address that is a multiple of one element only (odd row lengths, views into wider rows): global memory takes
+// 16-byte accesses at any such address, so these compile to the same wide instructions as aligned ones.
+template <class T, int N>
+__device__ __forceinline__ void load_any(T (&dst)[N], const T *src) { __builtin_memcpy(dst, __builtin_assume_aligned(src, sizeof(T)), sizeof(T) * N); }
+template <class T, int N>
+__device__ __forceinline__ void store_any(T *dst, const T (&src)[N]) { __builtin_memcpy(__builtin_assume_aligned(dst, sizeof(T)), src, sizeof(T) * N); }
+
+inline size_t dtype_bytes(uint32_t t) { return t == SHODH_DTYPE_FP32 ? 4 : t == SHODH_DTYPE_INT8 || t == SHODH_DTYPE_E4M3 ? 1 : 2; }
+inline bool is_float_dtype(uint32_t t) { return t == SHODH_DTYPE_FP32 || t == SHODH_DTYPE_BF16 || t == SHODH_DTYPE_FP16; }
+inline bool aligned_to(const void *p, size_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
+
+// The calling thread's current device is the caller's (torch keeps its own idea of it): it is switched for the call and put back.
+struct DeviceScope {
+    int before = -1;
+    bool changed = false;
+    int enter(int device) {
+        if (hipGetDevice(&before) != hipSuccess) { set_error("no HIP device: libshodh_hip has no CPU fallback"); return SHODH_ERR_DEVICE; }
+        if (before == device) return SHODH_OK;
+        if (hipSetDevice(device) != hipSuccess) { (void)hipGetLastError(); set_error("device %d not present", device); return SHODH_ERR_DEVICE; }
+        changed = true;
+        return SHODH_OK;
+    }
+    ~DeviceScope() { if (changed) (void)hipSetDevice(before); }
+};
+
+int compute_units(int device);      // of an existing device; asked once per device
+
+}  // namespace shodh

@@ -1,0 +1,213 @@
+"""Layer operators of a text tower on torch device tensors, over the C ABI (include/shodh_hip.h, "layer operators"): RMS norm with residual and 8-bit
+output, dense layers on 4-bit weights, attention with a sliding window and always-visible first tokens. They run on the tensors' device, on its
+current stream unless `stream` names another (a raw hipStream_t), and can be captured into a graph. Nothing here computes on the host."""
+import collections
+import ctypes as C
+
+import torch
+
+from . import _lib as L
+
+_DTYPES = {torch.float32: L.DTYPE_FP32, torch.bfloat16: L.DTYPE_BF16, torch.float16: L.DTYPE_FP16}
+_QUANT = {"int8": (L.DTYPE_INT8, torch.int8), "e4m3": (L.DTYPE_E4M3, torch.float8_e4m3fn)}
+
+RmsNorm = collections.namedtuple("RmsNorm", "y q scale sum")
+
+
+def _refuse(msg, code=L.ERR_INVALID):
+    raise L.ShodhError(code, msg)
+
+
+def _dtype(t, name):
+    d = _DTYPES.get(t.dtype)
+    if d is None:
+        _refuse("%s is %s: fp32, bf16 or fp16 is taken" % (name, t.dtype))
+    return d
+
+
+def _on(t, device, name):
+    if t.device != device:
+        _refuse("%s is on %s, not on %s" % (name, t.device, device))
+
+
+def _stream(device, stream):
+    return torch.cuda.current_stream(device).cuda_stream if stream is None else stream
+
+
+def _matrix(t, name):
+    """(rows, columns, row stride) of [..., columns] with neighbouring elements next to each other: a view of rows at one distance."""
+    if t.dim() == 2:
+        rows, cols = t.shape
+        if cols > 1 and t.stride(1) != 1:
+            _refuse("%s: the last dimension has to be contiguous" % name)
+        if rows > 1 and t.stride(0) == 0:
+            _refuse("%s: rows at distance 0 (an expanded tensor)" % name)
+        return rows, cols, t.stride(0) if rows > 1 else cols
+    if t.dim() == 0:
+        _refuse("%s has no dimension" % name)
+    cols = t.shape[-1]
+    rows = t.numel() // cols if cols else 0
+    if not t.is_contiguous():
+        _refuse("%s: more than two dimensions have to be contiguous" % name)
+    return rows, cols, cols
+
+
+def rms_norm(x, weight, eps=1e-6, residual=None, want_y=True, quant=None, group=0, sum_out=None, stream=None):
+    """h = x + residual; y = h / sqrt(mean(h^2) + eps) * weight over the last dimension (shodh_rms_norm_device).
+    quant "int8" / "e4m3": the row in 8 bits, with a scale per `group` values (0: per row; 32, 64, 128, 256): y ~ q * scale.
+    -> RmsNorm(y, q, scale, sum): what was not asked for is None; sum (with a residual) = h in x's type, written to `sum_out` (it may be
+    `residual` itself: in place) or a new tensor; scale f32 [rows, groups]."""
+    device = x.device
+    if device.type != "cuda":
+        _refuse("x is on %s: there is no CPU fallback" % device, L.ERR_DEVICE)
+    dt = _dtype(x, "x")
+    rows, dim, xs = _matrix(x, "x")
+    if weight.dim() != 1 or weight.shape[0] != dim or (dim > 1 and weight.stride(0) != 1):
+        _refuse("weight has to be contiguous [%d]" % dim, L.ERR_DIM)
+    _on(weight, device, "weight")
+    wd = _dtype(weight, "weight")
+    rs = ss = 0
+    total = None
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            _refuse("residual has to be of x's shape and type", L.ERR_DIM)
+        _on(residual, device, "residual")
+        rs = _matrix(residual, "residual")[2]
+        total = torch.empty(x.shape, dtype=x.dtype, device=device) if sum_out is None else sum_out
+        if sum_out is not None:
+            if total.shape != x.shape or total.dtype != x.dtype:
+                _refuse("sum_out has to be of x's shape and type", L.ERR_DIM)
+            _on(total, device, "sum_out")
+        ss = _matrix(total, "sum_out")[2]
+    elif sum_out is not None:
+        _refuse("sum_out without a residual")
+    y = torch.empty(x.shape, dtype=x.dtype, device=device) if want_y else None
+    q = scale = None
+    qd = L.DTYPE_INT8
+    if quant is not None:
+        if quant not in _QUANT:
+            _refuse("quant %r is neither 'int8' nor 'e4m3'" % (quant,))
+        qd, qt = _QUANT[quant]
+        q = torch.empty(x.shape, dtype=qt, device=device)
+        scale = torch.empty((rows, -(-dim // group) if group else 1), dtype=torch.float32, device=device)
+    if rows == 0:
+        return RmsNorm(y, q, scale, total)
+    cfg = L.RmsNormCfg(rows, xs, rs, ss, 0, 0, dim, dt, wd, qd, group, eps)
+    L.check(L.lib().shodh_rms_norm_device(device.index, C.byref(cfg), x.data_ptr(), residual.data_ptr() if residual is not None else None, weight.data_ptr(),
+                                          total.data_ptr() if total is not None else None, y.data_ptr() if want_y else None,
+                                          q.data_ptr() if q is not None else None, scale.data_ptr() if q is not None else None, _stream(device, stream)))
+    return RmsNorm(y, q, scale, total)
+
+
+class W4Weight:
+    """A dense layer's weights in 4 bits with group scales, laid out on the device once (shodh_w4_weight). The handle is read-only: any number of
+    threads and streams may use it."""
+
+    def __init__(self, handle, device):
+        self._h, self.device = handle, device
+        n, k, g, b = C.c_uint32(), C.c_uint32(), C.c_uint32(), C.c_uint64()
+        L.check(L.lib().shodh_w4_weight_shape(handle, C.byref(n), C.byref(k), C.byref(g), C.byref(b)))
+        self.n, self.k, self.group, self.nbytes = n.value, k.value, g.value, b.value
+
+    @staticmethod
+    def _scale_dtype(scale_dtype):
+        d = {torch.float16: L.DTYPE_FP16, torch.bfloat16: L.DTYPE_BF16}.get(scale_dtype)
+        if d is None:
+            _refuse("scales are kept in fp16 or bf16")
+        return d
+
+    @classmethod
+    def quantize(cls, w, group=128, zeros=False, scale_dtype=torch.float16, device=0):
+        """f32 weights [N, K] (host) rounded to 4 bits by the library."""
+        w = torch.as_tensor(w, dtype=torch.float32, device="cpu").contiguous()
+        if w.dim() != 2:
+            _refuse("the weight has to be [N, K]", L.ERR_DIM)
+        h = C.c_void_p()
+        L.check(L.lib().shodh_w4_weight_quantize(int(device), w.data_ptr(), w.shape[0], w.shape[1], group, int(bool(zeros)), cls._scale_dtype(scale_dtype), C.byref(h)))
+        return cls(h, torch.device("cuda", int(device)))
+
+    @classmethod
+    def from_quantized(cls, q, scale, zeros=None, k=None, group=128, scale_dtype=torch.float16, device=0):
+        """q uint8 [N, ceil(K / 2)] (two inputs a byte, the even one in the low bits), scale [N, ceil(K / group)], zeros uint8 of scale's shape or None (8):
+        device tensors (their device is used) or host tensors / arrays (`device`)."""
+        q, scale = torch.as_tensor(q), torch.as_tensor(scale)
+        zeros = None if zeros is None else torch.as_tensor(zeros)
+        if q.dim() != 2 or q.dtype != torch.uint8:
+            _refuse("q has to be uint8 [N, ceil(K / 2)]")
+        n = q.shape[0]
+        k = 2 * q.shape[1] if k is None else int(k)
+        if q.shape[1] != (k + 1) // 2:
+            _refuse("q has %d bytes a row, %d inputs need %d" % (q.shape[1], k, (k + 1) // 2), L.ERR_DIM)
+        if group not in (32, 64, 128):
+            _refuse("group %r is none of 32, 64, 128" % (group,), L.ERR_UNSUPPORTED)
+        shape = (n, -(-k // group))
+        if tuple(scale.shape) != shape or (zeros is not None and (tuple(zeros.shape) != shape or zeros.dtype != torch.uint8)):
+            _refuse("scale (and uint8 zeros) have to be %s" % (shape,), L.ERR_DIM)
+        sd = cls._scale_dtype(scale_dtype)
+        for t, name in ((scale, "scale"), (zeros, "zeros")):
+            if t is not None:
+                _on(t, q.device, name)
+        q, scale = q.contiguous(), scale.float().contiguous()
+        zeros = None if zeros is None else zeros.contiguous()
+        h, zp = C.c_void_p(), zeros.data_ptr() if zeros is not None else None
+        if q.device.type == "cuda":
+            L.check(L.lib().shodh_w4_weight_create_device(q.device.index, q.data_ptr(), scale.data_ptr(), zp, n, k, group, sd, _stream(q.device, None), C.byref(h)))
+            return cls(h, q.device)
+        L.check(L.lib().shodh_w4_weight_create(int(device), q.data_ptr(), scale.data_ptr(), zp, n, k, group, sd, C.byref(h)))
+        return cls(h, torch.device("cuda", int(device)))
+
+    def dequantize(self):
+        """the weights as the products see them: f32 [N, K] (host)"""
+        out = torch.empty((self.n, self.k), dtype=torch.float32)
+        L.check(L.lib().shodh_w4_weight_dequantize(self._h, out.data_ptr()))
+        return out
+
+    def dense(self, x, x_scale=None, bias=None, out_dtype=None, out=None, stream=None):
+        """x [..., K] -> [..., N]: x @ W^T (* x_scale per row) + bias. x fp32, bf16, fp16, or int8 with x_scale f32 [rows] (or [rows, 1]);
+        the result is of x's type (bf16 for int8 rows) unless out_dtype or `out` says otherwise."""
+        if self._h is None:
+            _refuse("the weight is closed", L.ERR_STATE)
+        rows, k, xs = _matrix(x, "x")
+        if k != self.k:
+            _refuse("x has %d columns, the weight %d inputs" % (k, self.k), L.ERR_DIM)
+        _on(x, self.device, "x")
+        sp = bp = None
+        if x.dtype == torch.int8:
+            xd = L.DTYPE_INT8
+            if x_scale is None or x_scale.dtype != torch.float32 or x_scale.numel() != rows or not x_scale.is_contiguous():
+                _refuse("int8 rows come with x_scale, contiguous f32 [%d]" % rows)
+            _on(x_scale, self.device, "x_scale")
+            sp = x_scale.data_ptr()
+        else:
+            xd = _dtype(x, "x")
+            if x_scale is not None:
+                _refuse("x_scale belongs to int8 rows")
+        if bias is not None:
+            if bias.dtype != torch.float32 or bias.shape != (self.n,) or not bias.is_contiguous():
+                _refuse("bias has to be contiguous f32 [%d]" % self.n, L.ERR_DIM)
+            _on(bias, self.device, "bias")
+            bp = bias.data_ptr()
+        shape = x.shape[:-1] + (self.n,)
+        if out is None:
+            out = torch.empty(shape, dtype=out_dtype or (torch.bfloat16 if xd == L.DTYPE_INT8 else x.dtype), device=self.device)
+        else:
+            if out.shape != shape or (out_dtype is not None and out.dtype != out_dtype):
+                _refuse("out has to be %s" % (tuple(shape),), L.ERR_DIM)
+            _on(out, self.device, "out")
+        if rows == 0:
+            return out
+        L.check(L.lib().shodh_w4_dense_device(self._h, x.data_ptr(), xd, xs, sp, rows, bp, out.data_ptr(), _dtype(out, "out"), _matrix(out, "out")[2],
+                                              _stream(self.device, stream)))
+        return out
+
+    def close(self):
+        """Frees the device copy (the runtime waits for what was started on it; not while a graph is being captured)."""
+        if self._h is not None:
+            h, self._h = self._h, None
+            L.lib().shodh_w4_weight_destroy(h)
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass

@@ -1,0 +1,214 @@
+"""Dense layers on 4-bit weights against their definition in 64 bits (GPU).
+
+Tolerance. A group's sum is formed as sum x (16 + q) - (16 + z) sum x. With u = 2^-23 (one unit in the last place per addition: the matrix unit's own order and
+rounding of its sums is not specified), a sum of G products of bf16 / fp16 / split f32 numbers is off by at most G u sum |x| (16 + q), sum |x|
+likewise, and the steps behind it (the difference, the scale, the sum over K / G groups, at most 8 waves, bias) by one u each of what has been added up:
+    |y - exact| <= (G + K / G + 16) u T + eps(type) / 2 |exact|,   T = sum_k |x| (32 + q + z) s  (+ |bias|)
+f32 rows: three parts of x, three sums each: 3 G. int8 rows: the groups' sums are exact, T = sum |x| |q - z| s and no G."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -23
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+@pytest.fixture(scope="module")
+def layers():
+    from shodh_memory_amd import layers
+    return layers
+
+
+def make(n, k, group, zeros, seed, device="cuda"):
+    g = torch.Generator().manual_seed(seed)
+    q = torch.randint(0, 16, (n, k), generator=g, dtype=torch.uint8)
+    ng = -(-k // group)
+    scale = (0.01 + 0.02 * torch.rand(n, ng, generator=g)).half().float()
+    z = torch.randint(0, 16, (n, ng), generator=g, dtype=torch.uint8) if zeros else None
+    p = torch.nn.functional.pad(q, (0, k % 2))
+    return q, (p[:, 0::2] | (p[:, 1::2] << 4)).contiguous().to(device), scale.to(device), z.to(device) if zeros else None
+
+
+def exact(x, xs, q, scale, z, bias, group):
+    """(values, T) in 64 bits on the host"""
+    k = q.shape[1]
+    at = torch.arange(k) // group
+    s = scale.cpu().double()[:, at]
+    zz = z.cpu().double()[:, at] if z is not None else torch.full_like(s, 8.0)
+    x = x.cpu().double()
+    y = x @ ((q.double() - zz) * s).t()
+    t = x.abs() @ (((q.double() - zz).abs() if xs is not None else 32 + q.double() + zz) * s).t()
+    if xs is not None:
+        y, t = y * xs.cpu().double()[:, None], t * xs.cpu().double()[:, None]
+    if bias is not None:
+        y, t = y + bias.cpu().double(), t + bias.cpu().double().abs()
+    return y, t
+
+
+def check(got, y, t, x_dtype, k, group):
+    adds = {torch.int8: 0, torch.float32: 3 * group}.get(x_dtype, group) + -(-k // group) + 16
+    tol = adds * U * t + torch.finfo(got.dtype).eps / 2 * y.abs() * (1 + 1e-6) + (2.0 ** -25 if got.dtype == torch.float16 else 0)
+    off = (got.cpu().double() - y).abs()
+    assert (off <= tol).all(), float((off / tol).max())
+
+
+def rows_of(kind, m, k, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(m, k, generator=g, device="cuda")
+    if kind == "int8":
+        xs = x.abs().amax(1).clamp(min=1e-6) / 127
+        return torch.round(x / xs[:, None]).to(torch.int8), xs
+    return x.to(TYPES[kind]), None
+
+
+SHAPES = [(1, 1, 1), (1, 16, 32), (1, 384, 384), (1, 17, 129), (2, 33, 31), (3, 100, 255), (5, 1001, 1234), (16, 64, 256), (17, 48, 1000), (31, 130, 513), (32, 31, 128), (33, 20, 2048),
+          (64, 96, 640), (65, 40, 300), (130, 35, 1025)]
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16", "f32", "int8"])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_against_the_definition(layers, kind, group):
+    for i, (m, n, k) in enumerate(SHAPES):
+        for zeros in (False, True):
+            q, packed, scale, z = make(n, k, group, zeros, 7 * i + group)
+            w = layers.W4Weight.from_quantized(packed, scale, z, k=k, group=group)
+            x, xs = rows_of(kind, m, k, i)
+            bias = torch.randn(n, device="cuda") if i % 2 else None
+            out = w.dense(x, x_scale=xs, bias=bias)
+            assert out.dtype == (torch.bfloat16 if kind == "int8" else x.dtype) and out.shape == (m, n)
+            y, t = exact(x, xs, q, scale, z, bias, group)
+            check(out, y, t, x.dtype, k, group)
+            check(w.dense(x, x_scale=xs, bias=bias, out_dtype=torch.float32), y, t, x.dtype, k, group)
+            w.close()
+
+
+def test_host_data_and_dequantize(layers):
+    q, packed, scale, z = make(37, 200, 64, True, 3, device="cpu")
+    want = (q.double() - z.double()[:, torch.arange(200) // 64]) * scale.double()[:, torch.arange(200) // 64]
+    for zeros in (z, None):
+        host = layers.W4Weight.from_quantized(packed, scale, zeros, k=200, group=64)
+        dev = layers.W4Weight.from_quantized(packed.cuda(), scale.cuda(), zeros.cuda() if zeros is not None else None, k=200, group=64)
+        ref = want if zeros is not None else (q.double() - 8) * scale.double()[:, torch.arange(200) // 64]
+        assert torch.equal(host.dequantize(), ref.float()) and torch.equal(dev.dequantize(), ref.float())
+        x = torch.randn(4, 200, device="cuda").half()
+        assert torch.equal(host.dense(x), dev.dense(x))
+    assert (host.n, host.k, host.group) == (37, 200, 64)
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("scale_dtype", [torch.float16, torch.bfloat16])
+def test_quantize(layers, zeros, scale_dtype):
+    """half a step of the group's scale (its rounding to 16 bits moves the largest values by a little more), zeros stay zeros"""
+    g = torch.Generator().manual_seed(1)
+    w = 0.02 * torch.randn(50, 333, generator=g)
+    w[7, 32:64] = 0
+    h = layers.W4Weight.quantize(w, group=32, zeros=zeros, scale_dtype=scale_dtype)
+    p = torch.nn.functional.pad(w, (0, 352 - 333)).view(50, 11, 32)
+    step = ((p.amax(2).clamp(min=0) - p.amin(2).clamp(max=0)) / 15 if zeros else p.abs().amax(2) / 7).repeat_interleave(32, 1)[:, :333]
+    rounding = torch.finfo(scale_dtype).eps / 2
+    # rounded to half a step, and the scale's own rounding times the number in front of it; with zero points the two ends can lie half a step outside
+    tol = step * (1 + rounding) * (0.5 + (0.5 if zeros else 0)) + 15 * rounding * step + 1e-6
+    assert ((h.dequantize() - w).abs() <= tol).all()
+    assert (h.dequantize()[7, 32:64] == 0).all()
+
+
+def test_views_columns_and_out(layers):
+    q, packed, scale, z = make(70, 391, 128, True, 9)
+    w = layers.W4Weight.from_quantized(packed, scale, z, k=391, group=128)
+    wide = torch.randn(6, 1000, device="cuda").bfloat16()
+    x = wide[:, 5:396]
+    want = w.dense(x.contiguous())
+    assert torch.equal(w.dense(x), want)
+    out = torch.full((6, 200), 3.0, device="cuda").bfloat16()
+    w.dense(x, out=out[:, 11:81])
+    assert torch.equal(out[:, 11:81], want) and (out[:, :11] == 3).all() and (out[:, 81:] == 3).all()
+    assert torch.equal(w.dense(x.contiguous().view(2, 3, 391)).view(6, 70), want)
+    for m in range(6):          # a row does not depend on its neighbours
+        assert torch.equal(w.dense(x[m:m + 1]), want[m:m + 1])
+    assert w.dense(x[:0]).shape == (0, 70)
+
+
+def test_nan_and_infinity_stay_in_their_row(layers):
+    q, packed, scale, z = make(40, 256, 64, False, 2)
+    w = layers.W4Weight.from_quantized(packed, scale, z, group=64)
+    for t in (torch.float32, torch.bfloat16, torch.float16):
+        x = torch.randn(5, 256, device="cuda").to(t)
+        clean = w.dense(x)
+        x[1, 100], x[3, 0] = float("nan"), float("inf")
+        out = w.dense(x)
+        assert torch.isnan(out[1]).all() and torch.isnan(out[3]).all()
+        assert torch.equal(out[[0, 2, 4]], clean[[0, 2, 4]])
+
+
+def test_f32_rows_keep_their_24_bits(layers):
+    """weights of one (q - z = 1, scale 1) at single places: the products are x itself, bit for bit"""
+    n = k = 64
+    q = torch.full((n, k), 8, dtype=torch.uint8)
+    q[torch.arange(n), torch.arange(n)] = 9
+    w = layers.W4Weight.from_quantized((q[:, 0::2] | (q[:, 1::2] << 4)).cuda(), torch.ones(n, 2, device="cuda"), group=32)
+    x = torch.zeros(64, k, device="cuda")
+    v = torch.randn(64, device="cuda")
+    x[torch.arange(64), torch.arange(64)] = v
+    got = w.dense(x)
+    # one value a row: 17 x - 16 ... : sums of 25 x's parts in f32, off by at most the 25 |x| u of the two sums
+    assert ((got.diagonal().double() - v.double()).abs() <= 50 * U * v.double().abs()).all()
+    assert (got - torch.diag(got.diagonal())).abs().max() <= 48 * U * v.abs().max()
+
+
+def test_streams_threads_and_graph(layers):
+    import threading
+    q, packed, scale, z = make(300, 1024, 128, True, 4)
+    w = layers.W4Weight.from_quantized(packed, scale, z, group=128)
+    xs = [torch.randn(3, 1024, device="cuda").half() for _ in range(4)]
+    want = [w.dense(x) for x in xs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def caller(i):
+        st = torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            for _ in range(20):
+                if not torch.equal(w.dense(xs[i]), want[i]):
+                    wrong.append(i)
+        st.synchronize()
+    th = [threading.Thread(target=caller, args=(i,)) for i in range(4)]
+    [t.start() for t in th]
+    [t.join() for t in th]
+    assert not wrong
+    x = xs[0].clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = w.dense(x)
+    for k in range(4):
+        x.copy_(xs[k])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(held, want[k]), k
+
+
+def test_refusals(layers):
+    from shodh_memory_amd import ShodhError
+    q, packed, scale, z = make(32, 128, 64, True, 1)
+    W = layers.W4Weight
+    w = W.from_quantized(packed, scale, z, group=64)
+    x = torch.randn(2, 128, device="cuda")
+    bad_scale = scale.clone()
+    bad_scale[3, 1] = float("inf")
+    big = scale.clone()
+    big[0, 0] = 1e6                                # no number of fp16
+    for call in [lambda: W.from_quantized(packed, scale, z, group=48), lambda: W.from_quantized(packed, scale[:, :1], z, group=64), lambda: W.from_quantized(packed, scale, z, k=200, group=64),
+                 lambda: W.from_quantized(packed, scale, z + 16, group=64), lambda: W.from_quantized(packed, bad_scale, z, group=64), lambda: W.from_quantized(packed, big, z, group=64),
+                 lambda: W.from_quantized(packed, scale, z.cpu(), group=64), lambda: W.from_quantized(packed, scale, z, group=64, scale_dtype=torch.float32),
+                 lambda: W.quantize(torch.full((4, 32), float("nan")), group=32), lambda: w.dense(x[:, :100]), lambda: w.dense(x.cpu()), lambda: w.dense(x.double()),
+                 lambda: w.dense(x, x_scale=torch.ones(2, device="cuda")), lambda: w.dense(x.to(torch.int8)), lambda: w.dense(x.to(torch.int8), x_scale=torch.ones(3, device="cuda")),
+                 lambda: w.dense(x, bias=torch.zeros(31, device="cuda")), lambda: w.dense(x, out=torch.empty(2, 31, device="cuda")), lambda: w.dense(x.t()),
+                 lambda: w.dense(x, out_dtype=torch.float64), lambda: w.dense(x[:1].expand(2, 128))]:
+        with pytest.raises(ShodhError):
+            call()
+    W.from_quantized(packed, big, z, group=64, scale_dtype=torch.bfloat16).close()
+    w.close()
+    with pytest.raises(ShodhError):
+        w.dense(x)
+    torch.cuda.synchronize()
