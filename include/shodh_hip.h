@@ -455,6 +455,33 @@ int shodh_w4_weight_shape(const shodh_w4_weight *w, uint32_t *N, uint32_t *K, ui
 int shodh_w4_dense_device(const shodh_w4_weight *w, const void *d_x, uint32_t x_dtype, uint64_t x_stride, const float *d_x_scale, uint32_t rows,
                           const float *d_bias, void *d_y, uint32_t y_dtype, uint64_t y_stride, void *stream);
 
+/* Attention with a sliding window and a few first tokens that stay visible (sinks), over ragged batches, with grouped heads, for whole texts as for
+ * single tokens at the end of a cache. Sequence b has the query tokens cu[b] .. cu[b + 1) (cu int32 [seqs + 1], device data, rising) and the
+ * keys kv_start[b] .. + kv_len[b) of k and v (int64 and int32 [seqs], device data; both NULL: the keys are the queries' own tokens). Query i of Lq stands
+ * at p = i + Lk - Lq (the last query at the last key) and sees key j iff
+ *     j <= p + right  and  (j >= p - left or j < sinks)          left, right < 0: no bound on that side; causal = right 0
+ * out = softmax(scale q k) v over the visible keys, lse = log sum exp (natural, f32 [q_tokens][heads], or NULL); a query that sees no key gets zeros and
+ * -inf. What masked keys hold (NaN, infinities) does not matter. Rows of out and lse behind the last sequence are left as they were; a sequence whose
+ * kv range does not lie in [0, kv_tokens) has no keys; what is written for one whose cu is out of order or range is undefined, within out and lse.
+ * q [q_tokens][heads][head_dim], k and v [kv_tokens][kv_heads][head_dim], out like q: any token and head strides. Query head h reads key head
+ * h * kv_heads / heads. Statistics and sums are f32; probabilities are multiplied in the inputs' 16-bit type.
+ * The workspace (shodh_window_attention_workspace bytes, may be 0; a multiple of 16) belongs to one call until that call's work is done. */
+typedef struct {
+    uint64_t q_tokens, kv_tokens;                /* rows of q and of k and v, all sequences */
+    uint64_t q_stride, q_head_stride, k_stride, k_head_stride, v_stride, v_head_stride, out_stride, out_head_stride;
+    uint32_t dtype;                              /* SHODH_DTYPE_BF16, _FP16 */
+    uint32_t heads, kv_heads, head_dim;          /* heads a multiple of kv_heads; head_dim a multiple of 8 up to 128 */
+    uint32_t seqs, sinks;
+    int32_t  left, right;
+    float    scale;                              /* 0 = 1 / sqrt(head_dim) */
+    uint32_t reserved;
+} shodh_attention_cfg;
+void shodh_attention_cfg_default(shodh_attention_cfg *cfg);        /* bf16, no bounds, no sinks, packed, sizes 0 */
+int shodh_window_attention_workspace(int device, const shodh_attention_cfg *cfg, uint64_t *bytes);
+int shodh_window_attention_device(int device, const shodh_attention_cfg *cfg, const void *d_q, const void *d_k, const void *d_v, const int32_t *d_cu,
+                                  const int64_t *d_kv_start, const int32_t *d_kv_len, void *d_out, float *d_lse, void *d_workspace,
+                                  uint64_t workspace_bytes, void *stream);
+
 /* ---- host-side glue of the same path (string / uuid work: stays on the host by design) ------------------ */
 /* MiniLMEmbedder::new_simplified / generate_embedding_simplified (minilm.rs:777-831): SipHash-1-3
  * (DefaultHasher, zero keys) over whitespace words and char bigrams -> dim-d unit vector; zeros if

@@ -105,6 +105,29 @@ pub struct shodh_rms_norm_cfg {
     pub eps: f32,
 }
 #[repr(C)] #[derive(Clone, Copy, Debug, Default)]
+pub struct shodh_attention_cfg {
+    pub q_tokens: u64,
+    pub kv_tokens: u64,
+    pub q_stride: u64,
+    pub q_head_stride: u64,
+    pub k_stride: u64,
+    pub k_head_stride: u64,
+    pub v_stride: u64,
+    pub v_head_stride: u64,
+    pub out_stride: u64,
+    pub out_head_stride: u64,
+    pub dtype: u32,
+    pub heads: u32,
+    pub kv_heads: u32,
+    pub head_dim: u32,
+    pub seqs: u32,
+    pub sinks: u32,
+    pub left: i32,
+    pub right: i32,
+    pub scale: f32,
+    pub reserved: u32,
+}
+#[repr(C)] #[derive(Clone, Copy, Debug, Default)]
 pub struct shodh_leg_fusion_cfg {
     pub fusion_v2: u8,
     pub fusion_flat: u8,
@@ -283,6 +306,9 @@ extern "C" {
     pub fn shodh_w4_weight_dequantize(w: *const shodh_w4_weight, out: *mut f32) -> c_int;
     pub fn shodh_w4_weight_shape(w: *const shodh_w4_weight, N: *mut u32, K: *mut u32, group: *mut u32, bytes: *mut u64) -> c_int;
     pub fn shodh_w4_dense_device(w: *const shodh_w4_weight, d_x: *const c_void, x_dtype: u32, x_stride: u64, d_x_scale: *const f32, rows: u32, d_bias: *const f32, d_y: *mut c_void, y_dtype: u32, y_stride: u64, stream: *mut c_void) -> c_int;
+    pub fn shodh_attention_cfg_default(cfg: *mut shodh_attention_cfg);
+    pub fn shodh_window_attention_workspace(device: c_int, cfg: *const shodh_attention_cfg, bytes: *mut u64) -> c_int;
+    pub fn shodh_window_attention_device(device: c_int, cfg: *const shodh_attention_cfg, d_q: *const c_void, d_k: *const c_void, d_v: *const c_void, d_cu: *const i32, d_kv_start: *const i64, d_kv_len: *const i32, d_out: *mut c_void, d_lse: *mut f32, d_workspace: *mut c_void, workspace_bytes: u64, stream: *mut c_void) -> c_int;
     pub fn shodh_hash_embed(utf8: *const c_char, len: usize, dim: u32, out: *mut f32) -> c_int;
     pub fn shodh_finalize_pooled(pooled: *const f32, n: usize, apply_prenorm: c_int, out_dim: usize, out: *mut f32) -> usize;
     pub fn shodh_search_ids_postprocess(vec_ids: *const u32, dists: *const f32, n_res: usize, vector_to_memory: *const u8, n_vectors: usize, limit: usize, out_uuid: *mut u8, out_sim: *mut f32) -> usize;

@@ -57,6 +57,13 @@ class RmsNormCfg(C.Structure):
                 ("q_group", C.c_uint32), ("eps", C.c_float)]
 
 
+class AttentionCfg(C.Structure):
+    _fields_ = [("q_tokens", C.c_uint64), ("kv_tokens", C.c_uint64), ("q_stride", C.c_uint64), ("q_head_stride", C.c_uint64), ("k_stride", C.c_uint64),
+                ("k_head_stride", C.c_uint64), ("v_stride", C.c_uint64), ("v_head_stride", C.c_uint64), ("out_stride", C.c_uint64), ("out_head_stride", C.c_uint64),
+                ("dtype", C.c_uint32), ("heads", C.c_uint32), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("seqs", C.c_uint32), ("sinks", C.c_uint32),
+                ("left", C.c_int32), ("right", C.c_int32), ("scale", C.c_float), ("reserved", C.c_uint32)]
+
+
 class Weights(C.Structure):
     _fields_ = [("semantic", C.c_float), ("entity", C.c_float), ("tag", C.c_float), ("importance", C.c_float),
                 ("momentum", C.c_float), ("access_count", C.c_float), ("graph_strength", C.c_float),
@@ -197,6 +204,9 @@ SYMBOLS = {
     "shodh_w4_weight_dequantize": (C.c_int, [_vp, _fp]),
     "shodh_w4_weight_shape": (C.c_int, [_vp, C.POINTER(C.c_uint32), C.POINTER(C.c_uint32), C.POINTER(C.c_uint32), C.POINTER(C.c_uint64)]),
     "shodh_w4_dense_device": (C.c_int, [_vp, _vp, C.c_uint32, C.c_uint64, _fp, C.c_uint32, _fp, _vp, C.c_uint32, C.c_uint64, _vp]),
+    "shodh_attention_cfg_default": (None, [C.POINTER(AttentionCfg)]),
+    "shodh_window_attention_workspace": (C.c_int, [C.c_int, C.POINTER(AttentionCfg), C.POINTER(C.c_uint64)]),
+    "shodh_window_attention_device": (C.c_int, [C.c_int, C.POINTER(AttentionCfg), _vp, _vp, _vp, _i32p, _vp, _i32p, _vp, _fp, _vp, C.c_uint64, _vp]),
     "shodh_hash_embed": (C.c_int, [C.c_char_p, C.c_size_t, C.c_uint32, _fp]),
     "shodh_finalize_pooled": (C.c_size_t, [_fp, C.c_size_t, C.c_int, C.c_size_t, _fp]),
     "shodh_search_ids_postprocess": (C.c_size_t, [_u32p, _fp, C.c_size_t, _u8p, C.c_size_t, C.c_size_t, _u8p, _fp]),

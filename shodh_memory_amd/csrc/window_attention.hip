@@ -1,0 +1,647 @@
+// window_attention.hip -- attention with a sliding window and a few first tokens that stay visible (sinks), over ragged batches, with grouped heads,
+// for whole texts as for single tokens at the end of a cache.
+//
+//   query i of a sequence (Lq new tokens, Lk keys) stands at p = i + Lk - Lq and sees key j iff  j <= p + right  and  (j >= p - left or j < sinks)
+//   out = sum_j softmax_j(scale q k_j) v_j over the visible keys;  lse = log sum_j exp(scale q k_j);  no visible key: zeros and -inf
+//
+// Everything is computed transposed, so that a lane owns one query: S^T = K Q^T (matrix instruction 32 x 32 x 16: rows = keys, columns = queries), softmax
+// down the lane's own registers, O^T = V^T P^T with P straight from those registers. The order in which the first product hands keys to a lane
+// (register r of half h holds key (r & 3) + 8 (r >> 2) + 4 h of 32) is taken as the order of the second product's inner index; V^T in that order is what
+// the transposing LDS read returns for four neighbouring keys. One pass over the keys, with a running maximum and sum in f32. The reference maximum is
+// only raised when a tile's maximum is more than 8 (in powers of two) above it: until then exp2 stays below 256, so nothing is lost and the accumulator
+// is not scaled again. P is rounded to the inputs' 16-bit type, because that is what the matrix instruction multiplies; the sum is of unrounded values.
+//
+// A row of work is one (query token, head of a group): the heads that share a key head read the same tile. Two forms:
+//  * tiles (texts, prompts): 4 waves x 32 rows, K and V tiles of 64 keys through LDS, next tile in registers meanwhile. Bound: MFMA and exp2 side by side.
+//  * split (few rows): one tile of 32 rows, the 4 waves take different blocks of 32 keys through LDS of their own, and further workgroups other parts of
+//    the key range; parts are added in a fixed order. Bound: HBM (the visible keys are read once).
+// Masked places may hold anything: scores there are replaced, and where a tile is partly masked and its V holds a NaN or an infinity (looked for while
+// staging), those values are multiplied only into the rows that see them.
+#include "layers.h"
+
+#pragma clang fp contract(off)
+
+namespace shodh {
+
+struct AttnArgs {
+    const void *q, *k, *v;
+    void *out;
+    float *lse;
+    const int32_t *cu;
+    const int64_t *kv_start;
+    const int32_t *kv_len;
+    float *part;               // split form: [splits][rows of out][DP] sums, then [splits][rows][2] maxima and sums
+    uint64_t q_stride, q_head, k_stride, k_head, v_stride, v_head, o_stride, o_head;
+    int64_t q_tokens, kv_tokens;
+    uint32_t heads, kv_heads, group, dim, seqs, slots, splits, sinks;
+    int32_t left, right;       // negative: no bound
+    float scale2;              // scale * log2(e)
+};
+
+constexpr float NEG_INF = -__builtin_inff();
+
+__device__ __forceinline__ float half_max(float x) {        // over a lane and its partner in the other half of the wave
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+__device__ __forceinline__ float half_sum(float x) {
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+
+template <class T> struct Vec8;
+template <> struct Vec8<__bf16> { using V = bf16x8; static constexpr uint32_t EXP = 0x7F807F80u, ONE = 0x00800080u; };
+template <> struct Vec8<_Float16> { using V = f16x8; static constexpr uint32_t EXP = 0x7C007C00u, ONE = 0x04000400u; };
+__device__ __forceinline__ f32x16 mma32(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mma32(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+template <class T>
+__device__ __forceinline__ bool any_nonfinite(u32x4 w) {     // an exponent of all ones in any of 8 values (a carry into the sign's place)
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m |= (w[i] & Vec8<T>::EXP) + Vec8<T>::ONE;
+    return (m & 0x80008000u) != 0;
+}
+
+// 16-byte places of a row of DP values, exchanged so that neither reading 8 rows' same place (K) nor 4 rows' same two places (V) meets on LDS banks
+template <int DP> __device__ __forceinline__ int k_place(int row, int c) { return DP == 32 ? c ^ ((row >> 1) & 3) : c ^ (row & 7); }
+template <int DP> __device__ __forceinline__ int v_place(int row, int c) { return DP == 32 ? c ^ (((row >> 1) & 1) << 1) : c ^ ((row & 3) << 1); }
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// Sequence of a tile slot: the largest b with cu[b] * group / BM + b <= slot (those starts rise strictly). 64 probes at a time.
+__device__ __forceinline__ int find_seq(const AttnArgs &a, int64_t slot, int bm) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = (int)a.seqs;            // the answer is in [lo, lo + n)
+    while (n > 1) {
+        const int step = (n + 63) / 64, b = lo + lane * step;
+        bool le = false;
+        if (lane * step < n) {
+            int64_t c = a.cu[b];
+            c = c < 0 ? 0 : c > a.q_tokens ? a.q_tokens : c;
+            le = c * a.group / bm + b <= slot;
+        }
+        const int got = __popcll(__ballot(le));       // (lane 0's start is never above the slot)
+        const int at = got > 0 ? got - 1 : 0;
+        lo += at * step;
+        n = min(step, n - at * step);
+    }
+    return lo;
+}
+
+struct Seq {
+    int64_t q0, k0;
+    int nq, nk;
+};
+__device__ __forceinline__ Seq seq_of(const AttnArgs &a, int b) {
+    Seq s;
+    int64_t t0 = a.cu[b], t1 = a.cu[b + 1];
+    if (t0 < 0 || t1 < t0 || t1 > a.q_tokens) t0 = t1 = 0;            // no such rows: nothing is done for them
+    s.q0 = t0; s.nq = (int)(t1 - t0);
+    if (a.kv_start) {
+        s.k0 = a.kv_start[b]; s.nk = a.kv_len[b];
+        if (s.k0 < 0 || s.nk < 0 || s.k0 > a.kv_tokens || s.nk > a.kv_tokens - s.k0) { s.k0 = 0; s.nk = 0; }      // no such keys: none is seen
+    } else { s.k0 = t0; s.nk = s.nq; }
+    return s;
+}
+
+// One wave's 32 rows: positions, running statistics, accumulators.
+template <class T, int DP>
+struct Rows {
+    using V8 = typename Vec8<T>::V;
+    V8 q[DP / 16];
+    f32x16 o[DP / 32];
+    float m, l;                // reference maximum (powers of two) and this half's part of the sum
+    int lo, hi;                // the lane's query sees [lo, hi) and the sinks below hi
+    bool live;
+    uint32_t token, head;      // of the lane's row (token within the sequence)
+
+    __device__ __forceinline__ void init(const AttnArgs &a, const Seq &s, uint32_t kvh, int64_t row) {
+        const int lane = threadIdx.x & 63, half = lane >> 5;
+        const int64_t r = row + (lane & 31);
+        live = r < (int64_t)s.nq * a.group;
+        token = live ? (uint32_t)(r / a.group) : 0;
+        head = kvh * a.group + (live ? (uint32_t)(r % a.group) : 0);
+        const int64_t p = (int64_t)token + s.nk - s.nq;
+        const int64_t h = a.right < 0 ? s.nk : p + a.right + 1, w = a.left < 0 ? 0 : p - a.left;
+        hi = live ? (int)(h < 0 ? 0 : h > s.nk ? s.nk : h) : 0;
+        lo = (int)(w < 0 ? 0 : w > s.nk ? s.nk : w);
+        const T *src = (const T *)a.q + (uint64_t)(s.q0 + token) * a.q_stride + (uint64_t)head * a.q_head;
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+            const uint32_t d = i * 16 + half * 8;
+            T e[8];
+            if (live && d < a.dim) load_any(e, src + d);
+            else
+                for (int x = 0; x < 8; ++x) e[x] = (T)0.0f;
+            __builtin_memcpy(&q[i], e, 16);
+        }
+#pragma unroll
+        for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+            for (int r2 = 0; r2 < 16; ++r2) o[t][r2] = 0.0f;
+        m = NEG_INF; l = 0.0f;
+    }
+
+    // NB blocks of 32 keys from `key` on, at Ks / Vs; keys from `limit` on belong to no one here. masked: some row does not see some key of them.
+    template <int NB>
+    __device__ __forceinline__ void tile(const AttnArgs &a, const unsigned char *Ks, const unsigned char *Vs, int key, int limit, bool masked, bool dirty) {
+        const int lane = threadIdx.x & 63, half = lane >> 5, l31 = lane & 31;
+        f32x16 s[NB];
+        float top = NEG_INF;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[b][r] = 0.0f;
+            const int row = b * 32 + l31;
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i) {
+                const V8 k = *reinterpret_cast<const V8 *>(Ks + row * (DP * 2) + k_place<DP>(row, 2 * i + half) * 16);
+                s[b] = mma32(k, q[i], s[b]);
+            }
+        }
+        const int end = min(hi, limit);
+        if (masked) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int j = key + b * 32 + (r & 3) + 8 * (r >> 2) + 4 * half;
+                    s[b][r] = j < end && (j >= lo || j < (int)a.sinks) ? s[b][r] * a.scale2 : NEG_INF;
+                    top = fmaxf(top, s[b][r]);
+                }
+        } else {
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) { s[b][r] *= a.scale2; top = fmaxf(top, s[b][r]); }
+        }
+        top = half_max(top);
+        const bool raise = top > m + 8.0f;      // (m = -inf: any finite score); a row's own affair: its neighbours change nothing in it
+        if (__any(raise)) {
+            const float next = raise ? top : m, c = raise ? __builtin_amdgcn_exp2f(m - next) : 1.0f;
+            m = next;
+            l *= c;
+#pragma unroll
+            for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[t][r] *= c;
+        }
+        const float base = m == NEG_INF ? 0.0f : m;
+        V8 p[NB][2];
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float v = __builtin_amdgcn_exp2f(s[b][r] - base);
+                l += v;
+                p[b][r >> 3][r & 7] = (T)v;
+            }
+        if (__builtin_expect(!(masked && dirty), 1)) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int t = 0; t < DP / 32; ++t) o[t] = mma32(v_frag(Vs, b, u, t), p[b][u], o[t]);
+        } else {
+#pragma unroll
+            for (int b = 0; b < NB; ++b) dirty_block(a, Vs, key, b, end, p[b]);
+        }
+    }
+
+    // V^T of 16 keys (inner order as above) and 32 features
+    __device__ __forceinline__ V8 v_frag(const unsigned char *Vs, int b, int u, int t) {
+        const int lane = threadIdx.x & 63, half = lane >> 5, sub = lane & 15, c = t * 4 + ((lane >> 4) & 1) * 2 + ((sub & 3) >> 1);
+        s16x4 v[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const int row = b * 32 + u * 16 + x * 8 + half * 4 + (sub >> 2);
+            const unsigned char *at = Vs + row * (DP * 2) + v_place<DP>(row, c) * 16 + (sub & 1) * 8;
+            v[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)at);
+        }
+        V8 f;
+        __builtin_memcpy(&f, v, 16);
+        return f;
+    }
+
+    // The same for a block that some rows see in part and whose V holds a NaN or an infinity: those values are left out of the matrix product and
+    // multiplied one by one into the rows that see their key.
+    __device__ __forceinline__ void dirty_block(const AttnArgs &a, const unsigned char *Vs, int key, int b, int end, const V8 (&p)[2]) {
+        const int lane = threadIdx.x & 63, half = lane >> 5;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int t = 0; t < DP / 32; ++t) {
+                V8 f = v_frag(Vs, b, u, t);
+                u32x4 w;
+                __builtin_memcpy(&w, &f, 16);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t bad = ((w[i] & Vec8<T>::EXP) + Vec8<T>::ONE) & 0x80008000u;
+                    w[i] &= (bad & 0x8000u ? 0u : 0x0000FFFFu) | (bad & 0x80000000u ? 0u : 0xFFFF0000u);
+                }
+                __builtin_memcpy(&f, &w, 16);
+                o[t] = mma32(f, p[u], o[t]);
+            }
+#pragma clang loop unroll(disable)
+        for (int kk = 0; kk < 32; ++kk) {
+            const int h = (kk >> 2) & 1, r0 = (kk & 3) + 4 * (kk >> 3), j = key + b * 32 + kk, row = b * 32 + kk;
+            float mine = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mine = r == r0 ? (float)p[r >> 3][r & 7] : mine;
+            const float pv = __shfl(mine, (lane & 31) + 32 * h);
+            const bool sees = j < end && (j >= lo || j < (int)a.sinks);
+#pragma unroll
+            for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+                for (int x = 0; x < 16; ++x) {
+                    const int d = t * 32 + (x & 3) + 8 * (x >> 2) + 4 * half;
+                    const float f = (float)*reinterpret_cast<const T *>(Vs + row * (DP * 2) + v_place<DP>(row, d >> 3) * 16 + (d & 7) * 2);
+                    if (sees && !(__builtin_fabsf(f) < __builtin_inff())) o[t][x] += pv * f;
+                }
+        }
+    }
+
+    __device__ __forceinline__ void store(const AttnArgs &a, const Seq &s, float total) {
+        const int half = (threadIdx.x & 63) >> 5;
+        if (!live) return;
+        const float inv = total > 0.0f || total != total ? 1.0f / total : 0.0f;
+        T *dst = (T *)a.out + (uint64_t)(s.q0 + token) * a.o_stride + (uint64_t)head * a.o_head;
+#pragma unroll
+        for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const uint32_t d = t * 32 + g * 8 + half * 4;
+                T e[4];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) e[x] = (T)(total == 0.0f ? 0.0f : o[t][4 * g + x] * inv);
+                if (d < a.dim) store_any(dst + d, e);
+            }
+        if (a.lse && half == 0)
+            a.lse[(uint64_t)(s.q0 + token) * a.heads + head] = total == 0.0f ? NEG_INF : (m + __builtin_amdgcn_logf(total)) * 0.69314718055994530942f;
+    }
+};
+
+// Range of keys that the rows [r0, r1) of a sequence see: sinks [0, first) and [begin, end); a multiple of 32 begins the second.
+struct Range {
+    int first, begin, end;
+};
+__device__ __forceinline__ Range range_of(const AttnArgs &a, const Seq &s, int64_t r0, int64_t r1) {
+    const int64_t rows = (int64_t)s.nq * a.group;
+    r1 = r1 < rows ? r1 : rows;
+    const int64_t p0 = r0 / a.group + s.nk - s.nq, p1 = (r1 - 1) / a.group + s.nk - s.nq;
+    int64_t end = a.right < 0 ? s.nk : p1 + a.right + 1, begin = a.left < 0 ? 0 : p0 - a.left;
+    end = end < 0 ? 0 : end > s.nk ? s.nk : end;
+    begin = begin < 0 ? 0 : begin > end ? end : begin;
+    Range g;
+    g.end = (int)end;
+    g.begin = (int)begin & ~31;
+    g.first = (int)a.sinks < g.begin ? (int)a.sinks : g.begin;
+    return g;
+}
+
+// 16-byte pieces of KEYS rows of K or V that a thread of NT carries: loaded to registers, written to LDS a tile later
+template <class T, int DP, int KEYS, int NT>
+struct Piece {
+    static constexpr int N = KEYS * DP / 8 / NT;
+    u32x4 v[N];
+    __device__ __forceinline__ void load(const T *base, uint64_t stride, int keys /* valid */, uint32_t dim, int t) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int e = i * NT + t, row = e / (DP / 8), c = e % (DP / 8);
+            T x[8];
+            if (row < keys && (uint32_t)(c * 8) < dim) load_any(x, base + (uint64_t)row * stride + c * 8);
+            else
+                for (int y = 0; y < 8; ++y) x[y] = (T)0.0f;
+            __builtin_memcpy(&v[i], x, 16);
+        }
+    }
+    __device__ __forceinline__ void store_k(unsigned char *lds, int t) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int e = i * NT + t, row = e / (DP / 8), c = e % (DP / 8);
+            *reinterpret_cast<u32x4 *>(lds + row * (DP * 2) + k_place<DP>(row, c) * 16) = v[i];
+        }
+    }
+    __device__ __forceinline__ bool store_v(unsigned char *lds, int t) const {       // -> a value that is no number among them
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int e = i * NT + t, row = e / (DP / 8), c = e % (DP / 8);
+            *reinterpret_cast<u32x4 *>(lds + row * (DP * 2) + v_place<DP>(row, c) * 16) = v[i];
+            bad |= any_nonfinite<T>(v[i]);
+        }
+        return bad;
+    }
+};
+
+// ---- tiles: 128 rows, tiles of 64 keys --------------------------------------------------------------------------------------------------
+template <class T, int DP>
+__global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs a) {
+    constexpr int BM = 128, KT = 64, TILE = KT * DP * 2;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];      // [2][K | V]
+    __shared__ int dirty[2];
+    const uint32_t items = gridDim.x;
+    // neighbouring items (tiles of one key head) on one XCD: it takes every eighth workgroup
+    const uint32_t per = items / 8, xcd = blockIdx.x & 7, item = blockIdx.x < per * 8 ? xcd * per + (blockIdx.x >> 3) : blockIdx.x;
+    const uint32_t kvh = item / a.slots, slot = item % a.slots;
+    const int b = find_seq(a, slot, BM);
+    const Seq s = seq_of(a, b);
+    const int64_t row0 = ((int64_t)slot - (s.q0 * a.group / BM + b)) * BM;
+    if (row0 < 0 || row0 >= (int64_t)s.nq * a.group) return;
+    const int t = threadIdx.x, wave = t >> 6;
+    Rows<T, DP> rows;
+    rows.init(a, s, kvh, row0 + wave * 32);
+    const Range g = range_of(a, s, row0, row0 + BM);
+    const int n_first = (g.first + KT - 1) / KT, n = n_first + (g.end - g.begin + KT - 1) / KT;
+    // what all of the wave's rows see, and what any of them does
+    int lo_max = rows.live ? rows.lo : 0, hi_min = rows.live ? rows.hi : 0x7FFFFFFF, lo_min = rows.live ? rows.lo : 0x7FFFFFFF, hi_max = rows.hi;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        lo_max = max(lo_max, __shfl_xor(lo_max, o)); hi_min = min(hi_min, __shfl_xor(hi_min, o));
+        lo_min = min(lo_min, __shfl_xor(lo_min, o)); hi_max = max(hi_max, __shfl_xor(hi_max, o));
+    }
+    const T *kb = (const T *)a.k + (uint64_t)s.k0 * a.k_stride + (uint64_t)kvh * a.k_head, *vb = (const T *)a.v + (uint64_t)s.k0 * a.v_stride + (uint64_t)kvh * a.v_head;
+    Piece<T, DP, KT, 256> pk, pv;
+    auto start_of = [&](int i) { return i < n_first ? i * KT : g.begin + (i - n_first) * KT; };
+    auto limit_of = [&](int i) { return i < n_first ? g.first : g.end; };
+    auto fetch = [&](int i) {
+        const int j = start_of(i), valid = min(KT, limit_of(i) - j);
+        pk.load(kb + (uint64_t)j * a.k_stride, a.k_stride, valid, a.dim, t);
+        pv.load(vb + (uint64_t)j * a.v_stride, a.v_stride, valid, a.dim, t);
+    };
+    if (t < 2) dirty[t] = 0;
+    if (n > 0) fetch(0);
+    __syncthreads();
+    for (int i = 0; i < n; ++i) {
+        unsigned char *Ks = smem + (i & 1) * 2 * TILE, *Vs = Ks + TILE;
+        pk.store_k(Ks, t);
+        if (pv.store_v(Vs, t)) dirty[i & 1] = 1;
+        __syncthreads();
+        const bool bad = dirty[i & 1] != 0;
+        if (i + 1 < n) fetch(i + 1);
+        const int j = start_of(i), limit = limit_of(i);
+        if (j < hi_max && (j + KT > lo_min || j < (int)a.sinks)) {
+            const bool masked = !(j + KT <= min(hi_min, limit) && (j >= lo_max || j + KT <= (int)a.sinks));
+            rows.template tile<KT / 32>(a, Ks, Vs, j, limit, masked, bad);
+        }
+        if (bad) {                   // (rare) cleared behind everybody's reading of it
+            __syncthreads();
+            if (t == 0) dirty[i & 1] = 0;
+            __syncthreads();
+        }
+    }
+    rows.store(a, s, half_sum(rows.l));
+}
+
+// ---- split: 32 rows, every wave its own blocks of 32 keys, every workgroup its own part of them ------------------------------------------------
+__device__ __forceinline__ void wave_fence() {      // LDS serves a wave's accesses in order: only the compiler has to be held
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+template <class T, int DP>
+__global__ __launch_bounds__(256, 2) void attn_split_kernel(const AttnArgs a) {
+    constexpr int BM = 32, KT = 32, TILE = KT * DP * 2;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];      // [4 waves][K | V]; then the waves' sums
+    const uint32_t kvh = blockIdx.y, slot = blockIdx.x, split = blockIdx.z;
+    const int b = find_seq(a, slot, BM);
+    const Seq s = seq_of(a, b);
+    const int64_t row0 = ((int64_t)slot - (s.q0 * a.group / BM + b)) * BM;
+    if (row0 < 0 || row0 >= (int64_t)s.nq * a.group) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    Rows<T, DP> rows;
+    rows.init(a, s, kvh, row0);
+    const Range g = range_of(a, s, row0, row0 + BM);
+    const int n_first = (g.first + KT - 1) / KT, n = n_first + (g.end - g.begin + KT - 1) / KT;
+    const int i0 = (int)((int64_t)n * split / a.splits), i1 = (int)((int64_t)n * (split + 1) / a.splits);
+    int lo_max = rows.live ? rows.lo : 0, hi_min = rows.live ? rows.hi : 0x7FFFFFFF;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) { lo_max = max(lo_max, __shfl_xor(lo_max, o)); hi_min = min(hi_min, __shfl_xor(hi_min, o)); }
+    const T *kb = (const T *)a.k + (uint64_t)s.k0 * a.k_stride + (uint64_t)kvh * a.k_head, *vb = (const T *)a.v + (uint64_t)s.k0 * a.v_stride + (uint64_t)kvh * a.v_head;
+    unsigned char *Ks = smem + wave * 2 * TILE, *Vs = Ks + TILE;
+    Piece<T, DP, KT, 64> pk, pv;
+    auto start_of = [&](int i) { return i < n_first ? i * KT : g.begin + (i - n_first) * KT; };
+    auto limit_of = [&](int i) { return i < n_first ? g.first : g.end; };
+    auto fetch = [&](int i) {
+        const int j = start_of(i), valid = min(KT, limit_of(i) - j);
+        pk.load(kb + (uint64_t)j * a.k_stride, a.k_stride, valid, a.dim, lane);
+        pv.load(vb + (uint64_t)j * a.v_stride, a.v_stride, valid, a.dim, lane);
+    };
+    if (i0 + wave < i1) fetch(i0 + wave);
+    for (int i = i0 + wave; i < i1; i += 4) {
+        wave_fence();
+        pk.store_k(Ks, lane);
+        const bool bad = __any(pv.store_v(Vs, lane));
+        wave_fence();
+        if (i + 4 < i1) fetch(i + 4);
+        const int j = start_of(i), limit = limit_of(i);
+        const bool masked = !(j + KT <= min(hi_min, limit) && (j >= lo_max || j + KT <= (int)a.sinks));
+        rows.template tile<1>(a, Ks, Vs, j, limit, masked, bad);
+    }
+    // the four waves' parts, in their order: statistics first, then the sums, 32 features at a time
+    float *stat = reinterpret_cast<float *>(smem + 8 * TILE);       // [4][32][2]
+    const float part = half_sum(rows.l);
+    if (lane < 32) { stat[(wave * 32 + lane) * 2] = rows.m; stat[(wave * 32 + lane) * 2 + 1] = part; }
+    __syncthreads();
+    float top = NEG_INF, total = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) top = fmaxf(top, stat[(w * 32 + (lane & 31)) * 2]);
+    const float base = top == NEG_INF ? 0.0f : top;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) total += stat[(w * 32 + (lane & 31)) * 2 + 1] * __builtin_amdgcn_exp2f(stat[(w * 32 + (lane & 31)) * 2] - base);
+    const float mine = __builtin_amdgcn_exp2f(rows.m - base);
+    float *sums = reinterpret_cast<float *>(smem);                  // [4 waves][16][64]
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t) {
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sums[(wave * 16 + r) * 64 + lane] = rows.o[t][r] * mine;
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            float v = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) v += sums[(w * 16 + r) * 64 + lane];
+            rows.o[t][r] = v;
+        }
+    }
+    rows.m = top;
+    if (a.splits == 1) {
+        if (wave == 0) rows.store(a, s, total);
+        return;
+    }
+    if (!rows.live || wave >= DP / 32) return;
+    const uint64_t all = (uint64_t)a.q_tokens * a.heads, at = (uint64_t)(s.q0 + rows.token) * a.heads + rows.head;
+    float *stats = a.part + (uint64_t)a.splits * all * DP;
+    if (wave == 0 && lane < 32) { stats[(split * all + at) * 2] = top; stats[(split * all + at) * 2 + 1] = total; }
+    float *dst = a.part + (split * all + at) * DP;
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t)
+        if (t == wave)
+#pragma unroll
+            for (int gq = 0; gq < 4; ++gq) {
+                f32x4 e;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) e[x] = rows.o[t][4 * gq + x];
+                *reinterpret_cast<f32x4 *>(dst + t * 32 + gq * 8 + (lane >> 5) * 4) = e;
+            }
+}
+
+// the parts of a row, in their order: one wave a row
+template <class T, int DP>
+__global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
+    const uint64_t all = (uint64_t)a.q_tokens * a.heads, at = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    int64_t last = a.cu[a.seqs];
+    if (at >= all || (int64_t)(at / a.heads) < (int64_t)a.cu[0] || (int64_t)(at / a.heads) >= last) return;       // rows behind the last sequence stay as they were
+    const float *stats = a.part + (uint64_t)a.splits * all * DP;
+    float m = NEG_INF, l = 0.0f;
+    if ((uint32_t)lane < a.splits) { m = stats[(lane * all + at) * 2]; l = stats[(lane * all + at) * 2 + 1]; }
+    float top = m;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    const float base = top == NEG_INF ? 0.0f : top, w = __builtin_amdgcn_exp2f(m - base);
+    float total = l * w;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o);
+    constexpr int PER = DP >= 64 ? DP / 64 : 1;
+    float v[PER] = {};
+    const int d = lane * PER;
+    for (uint32_t i = 0; i < a.splits; ++i) {
+        const float c = __shfl(w, (int)i);
+        if (d < DP)
+#pragma unroll
+            for (int x = 0; x < PER; ++x) v[x] += c * a.part[(i * all + at) * DP + d + x];
+    }
+    T *dst = (T *)a.out + (at / a.heads) * a.o_stride + (at % a.heads) * a.o_head;
+#pragma unroll
+    for (int x = 0; x < PER; ++x)
+        if ((uint32_t)(d + x) < a.dim) dst[d + x] = (T)(total == 0.0f ? 0.0f : v[x] / total);
+    if (a.lse && lane == 0) a.lse[at] = total == 0.0f ? NEG_INF : (top + __builtin_amdgcn_logf(total)) * 0.69314718055994530942f;
+}
+
+static int padded_dim(uint32_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
+
+struct AttnPlan {
+    bool split;
+    uint32_t slots, splits;
+    uint64_t workspace;
+};
+// Which form, and into how many parts the keys are cut.
+static AttnPlan plan_attention(const shodh_attention_cfg *c, int cus) {
+    AttnPlan p;
+    const uint64_t group = c->heads / c->kv_heads, rows = c->q_tokens * group;
+    const uint64_t tiles = (rows / 128 + c->seqs) * c->kv_heads;
+    p.split = rows <= 32ull * c->seqs || tiles < (uint64_t)cus;
+    p.slots = (uint32_t)(rows / (p.split ? 32 : 128) + c->seqs);
+    p.splits = 1;
+    p.workspace = 0;
+    if (p.split) {
+        uint64_t seen = c->kv_tokens;
+        if (c->left >= 0 && c->right >= 0) {
+            const uint64_t w = (uint64_t)c->left + (uint64_t)c->right + 1 + c->sinks + 32;
+            if (w < seen) seen = w;
+        }
+        const uint64_t groups = (uint64_t)p.slots * c->kv_heads, want = ceil_div(4ull * cus, groups ? groups : 1), most = ceil_div(seen, 256);
+        uint64_t n = want < most ? want : most;
+        p.splits = (uint32_t)(n < 1 ? 1 : n > 64 ? 64 : n);
+        if (p.splits > 1) p.workspace = p.splits * c->q_tokens * c->heads * (uint64_t)(padded_dim(c->head_dim) + 2) * 4;
+    }
+    return p;
+}
+
+static int check_attention(const shodh_attention_cfg *c) {
+    if (!c) { set_error("null argument"); return SHODH_ERR_INVALID; }
+    if (c->dtype != SHODH_DTYPE_BF16 && c->dtype != SHODH_DTYPE_FP16) { set_error("attention: dtype %u is neither bf16 nor fp16", c->dtype); return SHODH_ERR_UNSUPPORTED; }
+    if (c->heads == 0 || c->kv_heads == 0 || c->heads % c->kv_heads != 0) { set_error("attention: %u heads over %u key heads", c->heads, c->kv_heads); return SHODH_ERR_INVALID; }
+    if (c->head_dim == 0 || c->head_dim % 8 != 0 || c->head_dim > 128) { set_error("attention: head_dim %u is no multiple of 8 up to 128", c->head_dim); return SHODH_ERR_UNSUPPORTED; }
+    if (!(c->scale == c->scale) || c->scale > 3.0e38f || c->scale < -3.0e38f) { set_error("attention: scale is no number"); return SHODH_ERR_INVALID; }
+    if (c->q_tokens > 0x7FFFFFFFull || c->kv_tokens > (1ull << 40) || c->heads > 65535u || c->seqs > 0x3FFFFFFFu || c->sinks > 0x7FFFFFFFu) { set_error("attention: a size is out of range"); return SHODH_ERR_UNSUPPORTED; }
+    if (c->q_tokens * (c->heads / c->kv_heads) / 32 + c->seqs > 0x7FFFFFFFull / c->kv_heads) { set_error("attention: too many rows for one launch"); return SHODH_ERR_UNSUPPORTED; }
+    return SHODH_OK;
+}
+
+template <class T, int DP>
+static int launch_attention(const AttnArgs &a, const AttnPlan &p, hipStream_t st) {
+    if (!p.split) {
+        constexpr size_t lds = 4 * 64 * DP * 2;
+        SHODH_TRY(ensure_dynamic_lds((const void *)attn_tile_kernel<T, DP>, lds));
+        hipLaunchKernelGGL((attn_tile_kernel<T, DP>), dim3(p.slots * a.kv_heads), dim3(256), lds, st, a);
+        SHODH_HIP_TRY(hipGetLastError());
+        return SHODH_OK;
+    }
+    constexpr size_t tiles = 8 * 32 * DP * 2, lds = (tiles < 16384 ? 16384 : tiles) + 1024;
+    SHODH_TRY(ensure_dynamic_lds((const void *)attn_split_kernel<T, DP>, lds));
+    hipLaunchKernelGGL((attn_split_kernel<T, DP>), dim3(p.slots, a.kv_heads, p.splits), dim3(256), lds, st, a);
+    SHODH_HIP_TRY(hipGetLastError());
+    if (p.splits > 1) {
+        hipLaunchKernelGGL((attn_join_kernel<T, DP>), dim3((uint32_t)ceil_div((uint64_t)a.q_tokens * a.heads, 4)), dim3(256), 0, st, a);
+        SHODH_HIP_TRY(hipGetLastError());
+    }
+    return SHODH_OK;
+}
+
+}  // namespace shodh
+
+using namespace shodh;
+
+extern "C" {
+
+void shodh_attention_cfg_default(shodh_attention_cfg *cfg) {
+    if (!cfg) return;
+    memset(cfg, 0, sizeof *cfg);
+    cfg->dtype = SHODH_DTYPE_BF16;
+    cfg->left = cfg->right = -1;
+}
+
+int shodh_window_attention_workspace(int device, const shodh_attention_cfg *cfg, uint64_t *bytes) {
+    if (!bytes) { set_error("null argument"); return SHODH_ERR_INVALID; }
+    *bytes = 0;
+    SHODH_TRY(check_attention(cfg));
+    if (cfg->seqs == 0 || cfg->q_tokens == 0) return SHODH_OK;
+    *bytes = plan_attention(cfg, compute_units(device)).workspace;
+    return SHODH_OK;
+}
+
+int shodh_window_attention_device(int device, const shodh_attention_cfg *cfg, const void *d_q, const void *d_k, const void *d_v, const int32_t *d_cu, const int64_t *d_kv_start,
+                                  const int32_t *d_kv_len, void *d_out, float *d_lse, void *d_workspace, uint64_t workspace_bytes, void *stream) {
+    SHODH_TRY(check_attention(cfg));
+    if (cfg->seqs == 0 || cfg->q_tokens == 0) return SHODH_OK;
+    if (!d_q || !d_cu || !d_out || (cfg->kv_tokens && (!d_k || !d_v))) { set_error("null argument"); return SHODH_ERR_INVALID; }
+    if ((d_kv_start == nullptr) != (d_kv_len == nullptr)) { set_error("attention: kv_start and kv_len come together"); return SHODH_ERR_INVALID; }
+    if (!d_kv_start && cfg->kv_tokens != cfg->q_tokens) { set_error("attention: without kv_start and kv_len the keys are those of the queries' tokens (%llu tokens, %llu keys)",
+                                                                    (unsigned long long)cfg->q_tokens, (unsigned long long)cfg->kv_tokens); return SHODH_ERR_DIM; }
+    const uint64_t d = cfg->head_dim, H = cfg->heads;
+    AttnArgs a;
+    a.q_head = cfg->q_head_stride ? cfg->q_head_stride : d; a.q_stride = cfg->q_stride ? cfg->q_stride : H * d;
+    a.k_head = cfg->k_head_stride ? cfg->k_head_stride : d; a.k_stride = cfg->k_stride ? cfg->k_stride : cfg->kv_heads * d;
+    a.v_head = cfg->v_head_stride ? cfg->v_head_stride : d; a.v_stride = cfg->v_stride ? cfg->v_stride : cfg->kv_heads * d;
+    a.o_head = cfg->out_head_stride ? cfg->out_head_stride : d; a.o_stride = cfg->out_stride ? cfg->out_stride : H * d;
+    // rows of the output that lie over one another: neither [token][head] nor [head][token] with room for each
+    if (a.o_head < d || a.o_stride < d || (H > 1 && cfg->q_tokens > 1 && a.o_stride < (H - 1) * a.o_head + d && a.o_head < (cfg->q_tokens - 1) * a.o_stride + d)) {
+        set_error("attention: the output's rows overlap"); return SHODH_ERR_DIM;
+    }
+    if (!aligned_to(d_q, 2) || !aligned_to(d_k, 2) || !aligned_to(d_v, 2) || !aligned_to(d_out, 2) || !aligned_to(d_lse, 4) || !aligned_to(d_cu, 4) || !aligned_to(d_kv_start, 8) ||
+        !aligned_to(d_kv_len, 4) || !aligned_to(d_workspace, 16)) {
+        set_error("attention: a pointer is not a multiple of its element's size (the workspace: of 16)"); return SHODH_ERR_INVALID;
+    }
+    DeviceScope scope;
+    SHODH_TRY(scope.enter(device));
+    const AttnPlan p = plan_attention(cfg, compute_units(device));
+    if (p.workspace && (!d_workspace || workspace_bytes < p.workspace)) {
+        set_error("attention: a workspace of %llu bytes is needed (%llu given)", (unsigned long long)p.workspace, (unsigned long long)(d_workspace ? workspace_bytes : 0)); return SHODH_ERR_INVALID;
+    }
+    a.q = d_q; a.k = d_k; a.v = d_v; a.out = d_out; a.lse = d_lse; a.cu = d_cu; a.kv_start = d_kv_start; a.kv_len = d_kv_len; a.part = (float *)d_workspace;
+    a.q_tokens = (int64_t)cfg->q_tokens; a.kv_tokens = (int64_t)cfg->kv_tokens;
+    a.heads = cfg->heads; a.kv_heads = cfg->kv_heads; a.group = cfg->heads / cfg->kv_heads; a.dim = cfg->head_dim; a.seqs = cfg->seqs;
+    a.slots = p.slots; a.splits = p.splits; a.sinks = cfg->sinks; a.left = cfg->left; a.right = cfg->right;
+    const float scale = cfg->scale == 0.0f ? 1.0f / __builtin_sqrtf((float)d) : cfg->scale;
+    a.scale2 = scale * 1.44269504088896340736f;
+    hipStream_t st = (hipStream_t)stream;
+    const int dp = padded_dim(cfg->head_dim);
+    if (cfg->dtype == SHODH_DTYPE_BF16) return dp == 32 ? launch_attention<__bf16, 32>(a, p, st) : dp == 64 ? launch_attention<__bf16, 64>(a, p, st) : launch_attention<__bf16, 128>(a, p, st);
+    return dp == 32 ? launch_attention<_Float16, 32>(a, p, st) : dp == 64 ? launch_attention<_Float16, 64>(a, p, st) : launch_attention<_Float16, 128>(a, p, st);
+}
+
+}  // extern "C"

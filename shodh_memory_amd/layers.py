@@ -211,3 +211,70 @@ class W4Weight:
             self.close()
         except Exception:
             pass
+
+
+def _heads(t, name, device, dtype):
+    """(token stride, head stride) of [tokens, heads, head_dim] with neighbouring features next to each other"""
+    if t.dim() != 3 or t.dtype != dtype or t.device != device:
+        _refuse("%s has to be [tokens, heads, head_dim], %s, on %s (got %s, %s, %s)" % (name, dtype, device, tuple(t.shape), t.dtype, t.device))
+    n, h, d = t.shape
+    s, hs, one = t.stride()
+    if (d > 1 and one != 1) or (n > 1 and s == 0) or (h > 1 and hs == 0):
+        _refuse("%s: the last dimension has to be contiguous, no dimension expanded" % name)
+    return s if n > 1 else max(s, h * d), hs if h > 1 else d
+
+
+def _descriptor(t, name, device, dtype, n):
+    if t.dtype != dtype or t.device != device or tuple(t.shape) != (n,) or not t.is_contiguous():
+        _refuse("%s has to be contiguous %s [%d] on %s" % (name, dtype, n, device))
+    return t.data_ptr()
+
+
+def window_attention(q, k, v, cu, left=-1, right=-1, sinks=0, kv_start=None, kv_len=None, scale=None, return_lse=False, out=None, stream=None):
+    """Attention over a sliding window plus the first `sinks` tokens of each sequence (shodh_window_attention_device).
+    q [tokens, heads, head_dim] of all sequences one after another, sequence b = cu[b] .. cu[b + 1] (int32, device). k, v [kv_tokens, kv_heads, head_dim]:
+    the same tokens, or with kv_start (int64) and kv_len (int32) a cache in which sequence b has the keys kv_start[b] .. + kv_len[b], its queries
+    being the last ones. Query i of Lq stands at p = i + Lk - Lq and sees key j iff j <= p + right and (j >= p - left or j < sinks); a negative
+    bound is none; causal: right=0. bf16 or fp16, head_dim a multiple of 8 up to 128, any strides of tokens and heads.
+    -> out like q (and with return_lse the log of the sum of exponentials, f32 [tokens, heads]); tokens behind cu[-1] are left as they were."""
+    device = q.device
+    if device.type != "cuda":
+        _refuse("q is on %s: there is no CPU fallback" % device, L.ERR_DEVICE)
+    dt = _dtype(q, "q")
+    qs, qh = _heads(q, "q", device, q.dtype)
+    ks, kh = _heads(k, "k", device, q.dtype)
+    vs, vh = _heads(v, "v", device, q.dtype)
+    n, heads, dim = q.shape
+    kn, kv_heads, kd = k.shape
+    if v.shape != k.shape or kd != dim:
+        _refuse("k %s and v %s have to be [kv_tokens, kv_heads, %d] alike" % (tuple(k.shape), tuple(v.shape), dim), L.ERR_DIM)
+    if cu.dim() != 1 or cu.shape[0] < 1:
+        _refuse("cu has to be int32 [sequences + 1]")
+    seqs = cu.shape[0] - 1
+    cup = _descriptor(cu, "cu", device, torch.int32, seqs + 1)
+    if (kv_start is None) != (kv_len is None):
+        _refuse("kv_start and kv_len come together")
+    sp = lp = None
+    if kv_start is not None:
+        sp, lp = _descriptor(kv_start, "kv_start", device, torch.int64, seqs), _descriptor(kv_len, "kv_len", device, torch.int32, seqs)
+    if out is None:
+        out = torch.empty((n, heads, dim), dtype=q.dtype, device=device)
+    elif out.shape != q.shape:
+        _refuse("out has to be of q's shape", L.ERR_DIM)
+    os_, oh = _heads(out, "out", device, q.dtype)
+    if sinks < 0 or not -2 ** 31 <= left < 2 ** 31 or not -2 ** 31 <= right < 2 ** 31:
+        _refuse("left, right and sinks are 32-bit numbers, sinks 0 or more")
+    if scale is not None and not scale != 0:
+        _refuse("scale 0 (or no number)")
+    lse = torch.empty((n, heads), dtype=torch.float32, device=device) if return_lse else None
+    if n and seqs:
+        cfg = L.AttentionCfg(n, kn, qs, qh, ks, kh, vs, vh, os_, oh, dt, heads, kv_heads, dim, seqs, sinks, left, right, scale or 0.0, 0)
+        need = C.c_uint64()
+        L.check(L.lib().shodh_window_attention_workspace(device.index, C.byref(cfg), C.byref(need)))
+        work = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
+        st = _stream(device, stream)
+        if work is not None and stream is not None:
+            work.record_stream(torch.cuda.ExternalStream(stream, device=device))
+        L.check(L.lib().shodh_window_attention_device(device.index, C.byref(cfg), q.data_ptr(), k.data_ptr(), v.data_ptr(), cup, sp, lp, out.data_ptr(),
+                                                      lse.data_ptr() if return_lse else None, work.data_ptr() if work is not None else None, need.value, st))
+    return (out, lse) if return_lse else out

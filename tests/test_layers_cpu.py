@@ -79,3 +79,36 @@ def test_python_functions_take_device_tensors_only(L):
         with pytest.raises(ShodhError) as e:
             layers.W4Weight.from_quantized(torch.zeros(4, 16, dtype=torch.uint8), torch.ones(4, 1), group=32)
         assert e.value.code == L.ERR_DEVICE and "no CPU fallback" in str(e.value)
+
+
+def attn(L, q=P, k=P, v=P, cu=P, start=None, length=None, out=P, lse=None, work=None, nwork=0, **kw):
+    cfg = L.AttentionCfg()
+    L.lib().shodh_attention_cfg_default(C.byref(cfg))
+    cfg.q_tokens = cfg.kv_tokens = 8
+    cfg.heads, cfg.kv_heads, cfg.head_dim, cfg.seqs = 4, 2, 64, 1
+    for name, value in kw.items():
+        setattr(cfg, name, value)
+    return L.lib().shodh_window_attention_device(0, C.byref(cfg), q, k, v, cu, start, length, out, lse, work, nwork, None)
+
+
+def test_attention_defaults(L):
+    cfg = L.AttentionCfg()
+    L.lib().shodh_attention_cfg_default(C.byref(cfg))
+    assert (cfg.dtype, cfg.left, cfg.right, cfg.sinks, cfg.scale, cfg.heads) == (L.DTYPE_BF16, -1, -1, 0, 0.0, 0) and C.sizeof(cfg) == 120
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(dtype=0), -8), (dict(dtype=2), -8), (dict(heads=0), -1), (dict(kv_heads=0), -1), (dict(heads=5), -1), (dict(head_dim=0), -8), (dict(head_dim=60), -8), (dict(head_dim=136), -8),
+    (dict(scale=float("nan")), -1), (dict(scale=float("inf")), -1), (dict(q_tokens=1 << 31), -8), (dict(kv_tokens=(1 << 40) + 1), -8), (dict(sinks=1 << 31), -8), (dict(seqs=1 << 30), -8),
+    (dict(heads=65536), -8), (dict(q=None), -1), (dict(k=None), -1), (dict(v=None), -1), (dict(cu=None), -1), (dict(out=None), -1), (dict(start=P), -1), (dict(length=P), -1),
+    (dict(kv_tokens=9), -2), (dict(out_stride=63), -2), (dict(out_head_stride=8), -2), (dict(out_stride=64), -2), (dict(q=P + 1), -1), (dict(out=P + 1), -1), (dict(cu=P + 2), -1),
+    (dict(lse=P + 2), -1), (dict(work=P + 8), -1), (dict(start=P + 4, length=P), -1)])
+def test_attention_refuses(L, kw, code):
+    assert attn(L, **kw) == code and L.last_error()
+
+
+def test_attention_of_nothing_needs_no_device(L):
+    assert attn(L, seqs=0, cu=None) == 0 and attn(L, q_tokens=0, kv_tokens=0, q=None, k=None, v=None, out=None) == 0
+    n = C.c_uint64(7)
+    assert L.lib().shodh_window_attention_workspace(0, None, C.byref(n)) == -1 and n.value == 0
+    assert L.lib().shodh_window_attention_workspace(0, C.byref(L.AttentionCfg()), None) == -1
