@@ -15,8 +15,9 @@
 //  * tiles (texts, prompts): 4 waves x 32 rows, K and V tiles of 64 keys through LDS, next tile in registers meanwhile. Bound: MFMA and exp2 side by side.
 //  * split (few rows): one tile of 32 rows, the 4 waves take different blocks of 32 keys through LDS of their own, and further workgroups other parts of
 //    the key range; parts are added in a fixed order. Bound: HBM (the visible keys are read once).
-// Masked places may hold anything: scores there are replaced, and where a tile is partly masked and its V holds a NaN or an infinity (looked for while
-// staging), those values are multiplied only into the rows that see them.
+// Masked places may hold anything: scores there are replaced, and where a tile is partly masked its V is looked through for a NaN or an infinity: such
+// values are multiplied only into the rows that see them.
+#include "glds.h"
 #include "layers.h"
 
 #pragma clang fp contract(off)
@@ -35,7 +36,8 @@ struct AttnArgs {
     int64_t q_tokens, kv_tokens;
     uint32_t heads, kv_heads, group, dim, seqs, slots, splits, sinks;
     int32_t left, right;       // negative: no bound
-    float scale2;              // scale * log2(e)
+    float scale2;              // |scale| * log2(e)
+    uint32_t sign;             // 0, or the sign bits of two 16-bit numbers
 };
 
 constexpr float NEG_INF = -__builtin_inff();
@@ -115,6 +117,8 @@ struct Rows {
     int lo, hi;                // the lane's query sees [lo, hi) and the sinks below hi
     bool live;
     uint32_t token, head;      // of the lane's row (token within the sequence)
+    // LDS offsets of the lane's fragments: the exchanges of places touch two bits of a fragment's number only, the rest are constant distances
+    uint32_t at_k[DP == 32 ? 2 : 4], at_v[DP == 32 ? 1 : 2];
 
     __device__ __forceinline__ void init(const AttnArgs &a, const Seq &s, uint32_t kvh, int64_t row) {
         const int lane = threadIdx.x & 63, half = lane >> 5;
@@ -134,49 +138,63 @@ struct Rows {
             if (live && d < a.dim) load_any(e, src + d);
             else
                 for (int x = 0; x < 8; ++x) e[x] = (T)0.0f;
-            __builtin_memcpy(&q[i], e, 16);
+            u32x4 w;
+            __builtin_memcpy(&w, e, 16);
+            w ^= a.sign;                // a negative scale: its sign goes to q (exact), so that the largest score has the largest product
+            __builtin_memcpy(&q[i], &w, 16);
         }
 #pragma unroll
         for (int t = 0; t < DP / 32; ++t)
 #pragma unroll
             for (int r2 = 0; r2 < 16; ++r2) o[t][r2] = 0.0f;
         m = NEG_INF; l = 0.0f;
+        const int l31 = lane & 31, sub = lane & 15;
+#pragma unroll
+        for (int i = 0; i < (DP == 32 ? 2 : 4); ++i) {
+            at_k[i] = l31 * (DP * 2) + k_place<DP>(l31, 2 * i + half) * 16;
+            asm volatile("" : "+v"(at_k[i]));
+        }
+#pragma unroll
+        for (int t = 0; t < (DP == 32 ? 1 : 2); ++t) {
+            const int row = half * 4 + (sub >> 2);
+            at_v[t] = row * (DP * 2) + v_place<DP>(row, t * 4 + ((lane >> 4) & 1) * 2 + ((sub & 3) >> 1)) * 16 + (sub & 1) * 8;
+            asm volatile("" : "+v"(at_v[t]));
+        }
     }
 
-    // NB blocks of 32 keys from `key` on, at Ks / Vs; keys from `limit` on belong to no one here. masked: some row does not see some key of them.
+    // Scores of NB blocks of 32 keys in LDS at Ks.
     template <int NB>
-    __device__ __forceinline__ void tile(const AttnArgs &a, const unsigned char *Ks, const unsigned char *Vs, int key, int limit, bool masked, bool dirty) {
-        const int lane = threadIdx.x & 63, half = lane >> 5, l31 = lane & 31;
-        f32x16 s[NB];
-        float top = NEG_INF;
+    __device__ __forceinline__ void scores(const unsigned char *Ks, f32x16 (&s)[NB]) const {
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[b][r] = 0.0f;
-            const int row = b * 32 + l31;
 #pragma unroll
             for (int i = 0; i < DP / 16; ++i) {
-                const V8 k = *reinterpret_cast<const V8 *>(Ks + row * (DP * 2) + k_place<DP>(row, 2 * i + half) * 16);
+                const V8 k = *reinterpret_cast<const V8 *>(Ks + at_k[i & 3] + b * (32 * DP * 2) + (i >> 2) * 128);
                 s[b] = mma32(k, q[i], s[b]);
             }
         }
-        const int end = min(hi, limit);
+    }
+    // Scores to probabilities. Keys from `limit` on belong to no one here; masked: some row does not see some key of these.
+    template <int NB>
+    __device__ __forceinline__ void softmax(const AttnArgs &a, f32x16 (&s)[NB], V8 (&p)[NB][2], int key, int limit, bool masked) {
+        const int half = (threadIdx.x & 63) >> 5, end = min(hi, limit);
         if (masked) {
 #pragma unroll
             for (int b = 0; b < NB; ++b)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const int j = key + b * 32 + (r & 3) + 8 * (r >> 2) + 4 * half;
-                    s[b][r] = j < end && (j >= lo || j < (int)a.sinks) ? s[b][r] * a.scale2 : NEG_INF;
-                    top = fmaxf(top, s[b][r]);
+                    s[b][r] = j < end && (j >= lo || j < (int)a.sinks) ? s[b][r] : NEG_INF;
                 }
-        } else {
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) { s[b][r] *= a.scale2; top = fmaxf(top, s[b][r]); }
         }
-        top = half_max(top);
+        float tops[4] = {NEG_INF, NEG_INF, NEG_INF, NEG_INF};
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) tops[r & 3] = fmaxf(tops[r & 3], s[b][r]);
+        const float top = half_max(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]))) * a.scale2;
         const bool raise = top > m + 8.0f;      // (m = -inf: any finite score); a row's own affair: its neighbours change nothing in it
         if (__any(raise)) {
             const float next = raise ? top : m, c = raise ? __builtin_amdgcn_exp2f(m - next) : 1.0f;
@@ -188,38 +206,48 @@ struct Rows {
                 for (int r = 0; r < 16; ++r) o[t][r] *= c;
         }
         const float base = m == NEG_INF ? 0.0f : m;
-        V8 p[NB][2];
+        float ls[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const float v = __builtin_amdgcn_exp2f(s[b][r] - base);
-                l += v;
+                const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], a.scale2, -base));
+                ls[r & 3] += v;
                 p[b][r >> 3][r & 7] = (T)v;
             }
-        if (__builtin_expect(!(masked && dirty), 1)) {
+        l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+    }
+    // Probabilities times values in LDS at Vs.
+    template <int NB>
+    __device__ __forceinline__ void values(const AttnArgs &a, const unsigned char *Vs, const V8 (&p)[NB][2], int key, int limit, bool masked) {
+        if (masked) {
+            bool bad = false;
+            for (int e = threadIdx.x & 63; e < NB * 32 * DP / 8; e += 64) bad |= any_nonfinite<T>(*reinterpret_cast<const u32x4 *>(Vs + e * 16));
+            if (__builtin_expect(__any(bad), 0)) {
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
+                for (int b = 0; b < NB; ++b) spoiled_block(a, Vs, key, b, min(hi, limit), p[b]);
+                return;
+            }
+        }
+        V8 f[2][DP / 32];           // the fragments of 16 keys are on their way while those of the 16 before them are multiplied
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+        for (int t = 0; t < DP / 32; ++t) f[0][t] = v_frag(Vs, 0, 0, t);
 #pragma unroll
-                    for (int t = 0; t < DP / 32; ++t) o[t] = mma32(v_frag(Vs, b, u, t), p[b][u], o[t]);
-        } else {
+        for (int x = 0; x < 2 * NB; ++x) {
+            if (x + 1 < 2 * NB)
 #pragma unroll
-            for (int b = 0; b < NB; ++b) dirty_block(a, Vs, key, b, end, p[b]);
+                for (int t = 0; t < DP / 32; ++t) f[(x + 1) & 1][t] = v_frag(Vs, (x + 1) >> 1, (x + 1) & 1, t);
+#pragma unroll
+            for (int t = 0; t < DP / 32; ++t) o[t] = mma32(f[x & 1][t], p[x >> 1][x & 1], o[t]);
         }
     }
 
     // V^T of 16 keys (inner order as above) and 32 features
-    __device__ __forceinline__ V8 v_frag(const unsigned char *Vs, int b, int u, int t) {
-        const int lane = threadIdx.x & 63, half = lane >> 5, sub = lane & 15, c = t * 4 + ((lane >> 4) & 1) * 2 + ((sub & 3) >> 1);
+    __device__ __forceinline__ V8 v_frag(const unsigned char *Vs, int b, int u, int t) const {
         s16x4 v[2];
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            const int row = b * 32 + u * 16 + x * 8 + half * 4 + (sub >> 2);
-            const unsigned char *at = Vs + row * (DP * 2) + v_place<DP>(row, c) * 16 + (sub & 1) * 8;
-            v[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)at);
-        }
+        for (int x = 0; x < 2; ++x)
+            v[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(Vs + at_v[t & 1] + (b * 32 + u * 16 + x * 8) * (DP * 2) + (t >> 1) * 128));
         V8 f;
         __builtin_memcpy(&f, v, 16);
         return f;
@@ -227,7 +255,7 @@ struct Rows {
 
     // The same for a block that some rows see in part and whose V holds a NaN or an infinity: those values are left out of the matrix product and
     // multiplied one by one into the rows that see their key.
-    __device__ __forceinline__ void dirty_block(const AttnArgs &a, const unsigned char *Vs, int key, int b, int end, const V8 (&p)[2]) {
+    __device__ __forceinline__ void spoiled_block(const AttnArgs &a, const unsigned char *Vs, int key, int b, int end, const V8 (&p)[2]) {
         const int lane = threadIdx.x & 63, half = lane >> 5;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
@@ -243,6 +271,7 @@ struct Rows {
                 }
                 __builtin_memcpy(&f, &w, 16);
                 o[t] = mma32(f, p[u], o[t]);
+                asm volatile("" ::: "memory");
             }
 #pragma clang loop unroll(disable)
         for (int kk = 0; kk < 32; ++kk) {
@@ -259,6 +288,7 @@ struct Rows {
                     const int d = t * 32 + (x & 3) + 8 * (x >> 2) + 4 * half;
                     const float f = (float)*reinterpret_cast<const T *>(Vs + row * (DP * 2) + v_place<DP>(row, d >> 3) * 16 + (d & 7) * 2);
                     if (sees && !(__builtin_fabsf(f) < __builtin_inff())) o[t][x] += pv * f;
+                    asm volatile("" ::: "memory");       // (one value at a time: this path must not cost the other one registers)
                 }
         }
     }
@@ -301,47 +331,51 @@ __device__ __forceinline__ Range range_of(const AttnArgs &a, const Seq &s, int64
     return g;
 }
 
-// 16-byte pieces of KEYS rows of K or V that a thread of NT carries: loaded to registers, written to LDS a tile later
-template <class T, int DP, int KEYS, int NT>
-struct Piece {
-    static constexpr int N = KEYS * DP / 8 / NT;
-    u32x4 v[N];
-    __device__ __forceinline__ void load(const T *base, uint64_t stride, int keys /* valid */, uint32_t dim, int t) {
+// KEYS rows of K or V to LDS by NT threads (t of them is this one). DMA: straight from memory, 16 bytes a lane, in flight when the call returns; every
+// place of LDS fetches what belongs there, places behind the head's features are left alone (they were cleared once). Rows and heads that do not
+// begin at multiples of 16 bytes go through registers instead, and are there when the call returns. Rows behind the last valid one repeat it: their
+// scores are replaced, and what V holds there counts as any masked place does.
+template <class T, int DP, int KEYS, int NT, bool DMA, class Place>
+__device__ __forceinline__ void stage(unsigned char *lds, const T *base, uint64_t stride, int last, uint32_t dim, int t, Place place) {
+    constexpr int N = KEYS * DP / 8 / NT, STEP = NT / (DP / 8);          // 16-byte places of a thread, rows between them
+    auto to = [&](int i) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)(lds + (size_t)(i * NT + (t & ~63)) * 16)); };
+    if constexpr (DMA && STEP % 8 == 0) {
+        // (places are exchanged by the row's last three bits: the same ones in every step)
+        if (last == KEYS - 1) {
+            const int row = t / (DP / 8), c = place(row, t % (DP / 8));
+            if ((uint32_t)(c * 8) < dim)
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int e = i * NT + t, row = e / (DP / 8), c = e % (DP / 8);
-            T x[8];
-            if (row < keys && (uint32_t)(c * 8) < dim) load_any(x, base + (uint64_t)row * stride + c * 8);
-            else
-                for (int y = 0; y < 8; ++y) x[y] = (T)0.0f;
-            __builtin_memcpy(&v[i], x, 16);
+                for (int i = 0; i < N; ++i) glds16(uniform_ptr((const unsigned char *)(base + (uint64_t)(i * STEP) * stride)), ((uint32_t)row * (uint32_t)stride + c * 8) * 2, to(i));
+            return;
         }
     }
-    __device__ __forceinline__ void store_k(unsigned char *lds, int t) const {
+    int t2 = t;
+    asm volatile("" : "+v"(t2));           // (addresses are formed here, not kept in registers through the loop around)
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int e = i * NT + t, row = e / (DP / 8), c = e % (DP / 8);
-            *reinterpret_cast<u32x4 *>(lds + row * (DP * 2) + k_place<DP>(row, c) * 16) = v[i];
+    for (int i = 0; i < N; ++i) {
+        const int e = i * NT + t2, row = e / (DP / 8), x = e % (DP / 8), c = place(row, x);      // (an exchange is its own inverse)
+        const uint32_t from = (uint32_t)min(row, last);
+        const bool in = (uint32_t)(c * 8) < dim;
+        if constexpr (DMA) {
+            if (in) glds16(uniform_ptr((const unsigned char *)base), (from * (uint32_t)stride + c * 8) * 2, to(i));
+        } else {
+            T v[8];
+            load_any(v, base + (uint64_t)from * stride + (in ? c * 8 : 0));
+            u32x4 w;
+            __builtin_memcpy(&w, v, 16);
+            if (!in) w = u32x4{0, 0, 0, 0};
+            *reinterpret_cast<u32x4 *>(lds + e * 16) = w;
         }
     }
-    __device__ __forceinline__ bool store_v(unsigned char *lds, int t) const {       // -> a value that is no number among them
-        bool bad = false;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int e = i * NT + t, row = e / (DP / 8), c = e % (DP / 8);
-            *reinterpret_cast<u32x4 *>(lds + row * (DP * 2) + v_place<DP>(row, c) * 16) = v[i];
-            bad |= any_nonfinite<T>(v[i]);
-        }
-        return bad;
-    }
-};
+}
+template <int DP> struct KPlace { __device__ __forceinline__ int operator()(int row, int c) const { return k_place<DP>(row, c); } };
+template <int DP> struct VPlace { __device__ __forceinline__ int operator()(int row, int c) const { return v_place<DP>(row, c); } };
 
 // ---- tiles: 128 rows, tiles of 64 keys --------------------------------------------------------------------------------------------------
-template <class T, int DP>
+template <class T, int DP, bool DMA>
 __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs a) {
     constexpr int BM = 128, KT = 64, TILE = KT * DP * 2;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];      // [2][K | V]
-    __shared__ int dirty[2];
     const uint32_t items = gridDim.x;
     // neighbouring items (tiles of one key head) on one XCD: it takes every eighth workgroup
     const uint32_t per = items / 8, xcd = blockIdx.x & 7, item = blockIdx.x < per * 8 ? xcd * per + (blockIdx.x >> 3) : blockIdx.x;
@@ -363,44 +397,39 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs a) {
         lo_min = min(lo_min, __shfl_xor(lo_min, o)); hi_max = max(hi_max, __shfl_xor(hi_max, o));
     }
     const T *kb = (const T *)a.k + (uint64_t)s.k0 * a.k_stride + (uint64_t)kvh * a.k_head, *vb = (const T *)a.v + (uint64_t)s.k0 * a.v_stride + (uint64_t)kvh * a.v_head;
-    Piece<T, DP, KT, 256> pk, pv;
     auto start_of = [&](int i) { return i < n_first ? i * KT : g.begin + (i - n_first) * KT; };
     auto limit_of = [&](int i) { return i < n_first ? g.first : g.end; };
     auto fetch = [&](int i) {
-        const int j = start_of(i), valid = min(KT, limit_of(i) - j);
-        pk.load(kb + (uint64_t)j * a.k_stride, a.k_stride, valid, a.dim, t);
-        pv.load(vb + (uint64_t)j * a.v_stride, a.v_stride, valid, a.dim, t);
+        const int j = start_of(i), last = min(KT, limit_of(i) - j) - 1;
+        unsigned char *Ks = smem + (i & 1) * 2 * TILE;
+        stage<T, DP, KT, 256, DMA>(Ks, kb + (uint64_t)j * a.k_stride, a.k_stride, last, a.dim, t, KPlace<DP>());
+        stage<T, DP, KT, 256, DMA>(Ks + TILE, vb + (uint64_t)j * a.v_stride, a.v_stride, last, a.dim, t, VPlace<DP>());
     };
-    if (t < 2) dirty[t] = 0;
-    if (n > 0) fetch(0);
-    __syncthreads();
-    for (int i = 0; i < n; ++i) {
-        unsigned char *Ks = smem + (i & 1) * 2 * TILE, *Vs = Ks + TILE;
-        pk.store_k(Ks, t);
-        if (pv.store_v(Vs, t)) dirty[i & 1] = 1;
+    if (DMA && a.dim < DP) {
+        for (int e = t; e < 4 * TILE / 16; e += 256) *reinterpret_cast<u32x4 *>(smem + e * 16) = u32x4{0, 0, 0, 0};
         __syncthreads();
-        const bool bad = dirty[i & 1] != 0;
+    }
+    if (n > 0) fetch(0);
+    for (int i = 0; i < n; ++i) {
+        // this tile has arrived, for every wave; nobody reads the other buffer any more
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         if (i + 1 < n) fetch(i + 1);
+        const unsigned char *Ks = smem + (i & 1) * 2 * TILE;
         const int j = start_of(i), limit = limit_of(i);
         if (j < hi_max && (j + KT > lo_min || j < (int)a.sinks)) {
             const bool masked = !(j + KT <= min(hi_min, limit) && (j >= lo_max || j + KT <= (int)a.sinks));
-            rows.template tile<KT / 32>(a, Ks, Vs, j, limit, masked, bad);
-        }
-        if (bad) {                   // (rare) cleared behind everybody's reading of it
-            __syncthreads();
-            if (t == 0) dirty[i & 1] = 0;
-            __syncthreads();
+            f32x16 sc[KT / 32];
+            typename Rows<T, DP>::V8 p[KT / 32][2];
+            rows.scores(Ks, sc);
+            rows.softmax(a, sc, p, j, limit, masked);
+            rows.values(a, Ks + TILE, p, j, limit, masked);
         }
     }
     rows.store(a, s, half_sum(rows.l));
 }
 
 // ---- split: 32 rows, every wave its own blocks of 32 keys, every workgroup its own part of them ------------------------------------------------
-__device__ __forceinline__ void wave_fence() {      // LDS serves a wave's accesses in order: only the compiler has to be held
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
-template <class T, int DP>
+template <class T, int DP, bool DMA>
 __global__ __launch_bounds__(256, 2) void attn_split_kernel(const AttnArgs a) {
     constexpr int BM = 32, KT = 32, TILE = KT * DP * 2;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];      // [4 waves][K | V]; then the waves' sums
@@ -420,24 +449,43 @@ __global__ __launch_bounds__(256, 2) void attn_split_kernel(const AttnArgs a) {
     for (int o = 16; o > 0; o >>= 1) { lo_max = max(lo_max, __shfl_xor(lo_max, o)); hi_min = min(hi_min, __shfl_xor(hi_min, o)); }
     const T *kb = (const T *)a.k + (uint64_t)s.k0 * a.k_stride + (uint64_t)kvh * a.k_head, *vb = (const T *)a.v + (uint64_t)s.k0 * a.v_stride + (uint64_t)kvh * a.v_head;
     unsigned char *Ks = smem + wave * 2 * TILE, *Vs = Ks + TILE;
-    Piece<T, DP, KT, 64> pk, pv;
     auto start_of = [&](int i) { return i < n_first ? i * KT : g.begin + (i - n_first) * KT; };
     auto limit_of = [&](int i) { return i < n_first ? g.first : g.end; };
-    auto fetch = [&](int i) {
-        const int j = start_of(i), valid = min(KT, limit_of(i) - j);
-        pk.load(kb + (uint64_t)j * a.k_stride, a.k_stride, valid, a.dim, lane);
-        pv.load(vb + (uint64_t)j * a.v_stride, a.v_stride, valid, a.dim, lane);
+    auto fetch_k = [&](int i) {
+        const int j = start_of(i);
+        stage<T, DP, KT, 64, DMA>(Ks, kb + (uint64_t)j * a.k_stride, a.k_stride, min(KT, limit_of(i) - j) - 1, a.dim, lane, KPlace<DP>());
     };
-    if (i0 + wave < i1) fetch(i0 + wave);
+    auto fetch_v = [&](int i) {
+        const int j = start_of(i);
+        stage<T, DP, KT, 64, DMA>(Vs, vb + (uint64_t)j * a.v_stride, a.v_stride, min(KT, limit_of(i) - j) - 1, a.dim, lane, VPlace<DP>());
+    };
+    if (DMA && a.dim < DP) {
+        for (int e = lane; e < 2 * TILE / 16; e += 64) *reinterpret_cast<u32x4 *>(Ks + e * 16) = u32x4{0, 0, 0, 0};
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    // K's next block is fetched while this one's values are multiplied, V's next while the next scores are: each wait leaves the other's loads (one
+    // per 64 lanes x 16 bytes: DP / 16 of them) in flight. (With a head smaller than DP some are left out: there all are waited for.)
+    const bool whole = a.dim == DP;
+    auto arrived = [&](bool all) {
+        if (DMA && whole && !all) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(DP / 16) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
+    };
+    if (i0 + wave < i1) { fetch_k(i0 + wave); fetch_v(i0 + wave); }
     for (int i = i0 + wave; i < i1; i += 4) {
-        wave_fence();
-        pk.store_k(Ks, lane);
-        const bool bad = __any(pv.store_v(Vs, lane));
-        wave_fence();
-        if (i + 4 < i1) fetch(i + 4);
         const int j = start_of(i), limit = limit_of(i);
-        const bool masked = !(j + KT <= min(hi_min, limit) && (j >= lo_max || j + KT <= (int)a.sinks));
-        rows.template tile<1>(a, Ks, Vs, j, limit, masked, bad);
+        const bool masked = !(j + KT <= min(hi_min, limit) && (j >= lo_max || j + KT <= (int)a.sinks)), more = i + 4 < i1;
+        f32x16 sc[1];
+        typename Rows<T, DP>::V8 p[1][2];
+        arrived(false);                       // K
+        rows.scores(Ks, sc);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (more) fetch_k(i + 4);
+        rows.softmax(a, sc, p, j, limit, masked);
+        arrived(!more);                       // V
+        rows.values(a, Vs, p, j, limit, masked);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (more) fetch_v(i + 4);
     }
     // the four waves' parts, in their order: statistics first, then the sums, 32 features at a time
     float *stat = reinterpret_cast<float *>(smem + 8 * TILE);       // [4][32][2]
@@ -562,24 +610,34 @@ static int check_attention(const shodh_attention_cfg *c) {
     return SHODH_OK;
 }
 
-template <class T, int DP>
+template <class T, int DP, bool DMA>
 static int launch_attention(const AttnArgs &a, const AttnPlan &p, hipStream_t st) {
     if (!p.split) {
         constexpr size_t lds = 4 * 64 * DP * 2;
-        SHODH_TRY(ensure_dynamic_lds((const void *)attn_tile_kernel<T, DP>, lds));
-        hipLaunchKernelGGL((attn_tile_kernel<T, DP>), dim3(p.slots * a.kv_heads), dim3(256), lds, st, a);
+        SHODH_TRY(ensure_dynamic_lds((const void *)attn_tile_kernel<T, DP, DMA>, lds));
+        hipLaunchKernelGGL((attn_tile_kernel<T, DP, DMA>), dim3(p.slots * a.kv_heads), dim3(256), lds, st, a);
         SHODH_HIP_TRY(hipGetLastError());
         return SHODH_OK;
     }
     constexpr size_t tiles = 8 * 32 * DP * 2, lds = (tiles < 16384 ? 16384 : tiles) + 1024;
-    SHODH_TRY(ensure_dynamic_lds((const void *)attn_split_kernel<T, DP>, lds));
-    hipLaunchKernelGGL((attn_split_kernel<T, DP>), dim3(p.slots, a.kv_heads, p.splits), dim3(256), lds, st, a);
+    SHODH_TRY(ensure_dynamic_lds((const void *)attn_split_kernel<T, DP, DMA>, lds));
+    hipLaunchKernelGGL((attn_split_kernel<T, DP, DMA>), dim3(p.slots, a.kv_heads, p.splits), dim3(256), lds, st, a);
     SHODH_HIP_TRY(hipGetLastError());
     if (p.splits > 1) {
         hipLaunchKernelGGL((attn_join_kernel<T, DP>), dim3((uint32_t)ceil_div((uint64_t)a.q_tokens * a.heads, 4)), dim3(256), 0, st, a);
         SHODH_HIP_TRY(hipGetLastError());
     }
     return SHODH_OK;
+}
+template <class T, bool DMA>
+static int pick_dim(const AttnArgs &a, const AttnPlan &p, hipStream_t st) {
+    return a.dim <= 32 ? launch_attention<T, 32, DMA>(a, p, st) : a.dim <= 64 ? launch_attention<T, 64, DMA>(a, p, st) : launch_attention<T, 128, DMA>(a, p, st);
+}
+template <class T>
+static int pick_attention(const AttnArgs &a, const AttnPlan &p, hipStream_t st) {
+    // 16-byte pieces straight to LDS: every row and head at a multiple of 16 bytes, a tile's rows within a 32-bit offset
+    const bool dma = aligned_to(a.k, 16) && aligned_to(a.v, 16) && ((a.k_stride | a.v_stride | a.k_head | a.v_head) & 7) == 0 && a.k_stride < (1u << 24) && a.v_stride < (1u << 24);
+    return dma ? pick_dim<T, true>(a, p, st) : pick_dim<T, false>(a, p, st);
 }
 
 }  // namespace shodh
@@ -637,11 +695,10 @@ int shodh_window_attention_device(int device, const shodh_attention_cfg *cfg, co
     a.heads = cfg->heads; a.kv_heads = cfg->kv_heads; a.group = cfg->heads / cfg->kv_heads; a.dim = cfg->head_dim; a.seqs = cfg->seqs;
     a.slots = p.slots; a.splits = p.splits; a.sinks = cfg->sinks; a.left = cfg->left; a.right = cfg->right;
     const float scale = cfg->scale == 0.0f ? 1.0f / __builtin_sqrtf((float)d) : cfg->scale;
-    a.scale2 = scale * 1.44269504088896340736f;
+    a.scale2 = __builtin_fabsf(scale) * 1.44269504088896340736f;
+    a.sign = scale < 0.0f ? 0x80008000u : 0u;
     hipStream_t st = (hipStream_t)stream;
-    const int dp = padded_dim(cfg->head_dim);
-    if (cfg->dtype == SHODH_DTYPE_BF16) return dp == 32 ? launch_attention<__bf16, 32>(a, p, st) : dp == 64 ? launch_attention<__bf16, 64>(a, p, st) : launch_attention<__bf16, 128>(a, p, st);
-    return dp == 32 ? launch_attention<_Float16, 32>(a, p, st) : dp == 64 ? launch_attention<_Float16, 64>(a, p, st) : launch_attention<_Float16, 128>(a, p, st);
+    return cfg->dtype == SHODH_DTYPE_BF16 ? pick_attention<__bf16>(a, p, st) : pick_attention<_Float16>(a, p, st);
 }
 
 }  // extern "C"
