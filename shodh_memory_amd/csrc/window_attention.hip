@@ -16,7 +16,7 @@
 //  * split (few rows): one tile of 32 rows, the 4 waves take different blocks of 32 keys through LDS of their own, and further workgroups other parts of
 //    the key range; parts are added in a fixed order. Bound: HBM (the visible keys are read once).
 // Masked places may hold anything: scores there are replaced, and where a tile is partly masked its V is looked through for a NaN or an infinity: such
-// values are multiplied only into the rows that see them.
+// values are taken out of the tile, and put into the rows that see them at the end.
 #include "glds.h"
 #include "layers.h"
 
@@ -52,8 +52,8 @@ __device__ __forceinline__ float half_sum(float x) {
 }
 
 template <class T> struct Vec8;
-template <> struct Vec8<__bf16> { using V = bf16x8; static constexpr uint32_t EXP = 0x7F807F80u, ONE = 0x00800080u; };
-template <> struct Vec8<_Float16> { using V = f16x8; static constexpr uint32_t EXP = 0x7C007C00u, ONE = 0x04000400u; };
+template <> struct Vec8<__bf16> { using V = bf16x8; using V2 = bf16x2; static constexpr uint32_t EXP = 0x7F807F80u, ONE = 0x00800080u; };
+template <> struct Vec8<_Float16> { using V = f16x8; using V2 = f16x2; static constexpr uint32_t EXP = 0x7C007C00u, ONE = 0x04000400u; };
 __device__ __forceinline__ f32x16 mma32(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16 mma32(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
@@ -65,9 +65,28 @@ __device__ __forceinline__ bool any_nonfinite(u32x4 w) {     // an exponent of a
     return (m & 0x80008000u) != 0;
 }
 
-// 16-byte places of a row of DP values, exchanged so that neither reading 8 rows' same place (K) nor 4 rows' same two places (V) meets on LDS banks
-template <int DP> __device__ __forceinline__ int k_place(int row, int c) { return DP == 32 ? c ^ ((row >> 1) & 3) : c ^ (row & 7); }
-template <int DP> __device__ __forceinline__ int v_place(int row, int c) { return DP == 32 ? c ^ (((row >> 1) & 1) << 1) : c ^ ((row & 3) << 1); }
+// Takes the values that are no numbers out of `bytes` of V in LDS, by NT threads; true for a thread that found one.
+template <class T, int NT>
+__device__ __forceinline__ bool clear_values(unsigned char *Vs, int bytes, int t) {
+    bool found = false;
+    for (int e = t * 16; e < bytes; e += NT * 16) {
+        u32x4 w = *reinterpret_cast<const u32x4 *>(Vs + e);
+        if (!any_nonfinite<T>(w)) continue;
+        found = true;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t bad = ((w[i] & Vec8<T>::EXP) + Vec8<T>::ONE) & 0x80008000u;
+            w[i] &= (bad & 0x8000u ? 0u : 0x0000FFFFu) | (bad & 0x80000000u ? 0u : 0xFFFF0000u);
+        }
+        *reinterpret_cast<u32x4 *>(Vs + e) = w;
+    }
+    return found;
+}
+
+// 16-byte places of a row of DP values, exchanged so that neither 16 rows' same place (a fragment of K) nor 4 rows' same four places (of V, read across)
+// meet on LDS banks, which repeat every 256 bytes: 1, 2 or 4 rows
+template <int DP> __device__ __forceinline__ int k_place(int row, int c) { return DP == 32 ? c ^ ((row >> 2) & 3) : DP == 64 ? c ^ ((row >> 1) & 7) : c ^ (row & 15); }
+template <int DP> __device__ __forceinline__ int v_place(int row, int c) { return DP == 32 ? c : DP == 64 ? c ^ ((row & 2) << 1) : c ^ ((row & 3) << 2); }
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
@@ -91,6 +110,9 @@ __device__ __forceinline__ int find_seq(const AttnArgs &a, int64_t slot, int bm)
     return lo;
 }
 
+__device__ __forceinline__ int64_t uniform64(int64_t x) {       // a number that all lanes hold alike, in scalar registers
+    return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)x));
+}
 struct Seq {
     int64_t q0, k0;
     int nq, nk;
@@ -104,6 +126,8 @@ __device__ __forceinline__ Seq seq_of(const AttnArgs &a, int b) {
         s.k0 = a.kv_start[b]; s.nk = a.kv_len[b];
         if (s.k0 < 0 || s.nk < 0 || s.k0 > a.kv_tokens || s.nk > a.kv_tokens - s.k0) { s.k0 = 0; s.nk = 0; }      // no such keys: none is seen
     } else { s.k0 = t0; s.nk = s.nq; }
+    s.q0 = uniform64(s.q0); s.k0 = uniform64(s.k0);
+    s.nq = __builtin_amdgcn_readfirstlane(s.nq); s.nk = __builtin_amdgcn_readfirstlane(s.nk);
     return s;
 }
 
@@ -117,8 +141,7 @@ struct Rows {
     int lo, hi;                // the lane's query sees [lo, hi) and the sinks below hi
     bool live;
     uint32_t token, head;      // of the lane's row (token within the sequence)
-    // LDS offsets of the lane's fragments: the exchanges of places touch two bits of a fragment's number only, the rest are constant distances
-    uint32_t at_k[DP == 32 ? 2 : 4], at_v[DP == 32 ? 1 : 2];
+    uint32_t at_k[DP / 16], at_v[DP / 32];      // LDS offsets of the lane's fragments in a block
 
     __device__ __forceinline__ void init(const AttnArgs &a, const Seq &s, uint32_t kvh, int64_t row) {
         const int lane = threadIdx.x & 63, half = lane >> 5;
@@ -150,12 +173,12 @@ struct Rows {
         m = NEG_INF; l = 0.0f;
         const int l31 = lane & 31, sub = lane & 15;
 #pragma unroll
-        for (int i = 0; i < (DP == 32 ? 2 : 4); ++i) {
+        for (int i = 0; i < DP / 16; ++i) {
             at_k[i] = l31 * (DP * 2) + k_place<DP>(l31, 2 * i + half) * 16;
             asm volatile("" : "+v"(at_k[i]));
         }
 #pragma unroll
-        for (int t = 0; t < (DP == 32 ? 1 : 2); ++t) {
+        for (int t = 0; t < DP / 32; ++t) {
             const int row = half * 4 + (sub >> 2);
             at_v[t] = row * (DP * 2) + v_place<DP>(row, t * 4 + ((lane >> 4) & 1) * 2 + ((sub & 3) >> 1)) * 16 + (sub & 1) * 8;
             asm volatile("" : "+v"(at_v[t]));
@@ -165,16 +188,20 @@ struct Rows {
     // Scores of NB blocks of 32 keys in LDS at Ks.
     template <int NB>
     __device__ __forceinline__ void scores(const unsigned char *Ks, f32x16 (&s)[NB]) const {
+        V8 k[NB][DP / 16];
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
+        for (int i = 0; i < DP / 16; ++i)
+#pragma unroll
+            for (int b = 0; b < NB; ++b) k[b][i] = *reinterpret_cast<const V8 *>(Ks + at_k[i] + b * (32 * DP * 2));
+        __builtin_amdgcn_sched_barrier(0);          // (all of them on their way before the first is waited for)
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[b][r] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < DP / 16; ++i) {
-                const V8 k = *reinterpret_cast<const V8 *>(Ks + at_k[i & 3] + b * (32 * DP * 2) + (i >> 2) * 128);
-                s[b] = mma32(k, q[i], s[b]);
-            }
-        }
+        for (int i = 0; i < DP / 16; ++i)
+#pragma unroll
+            for (int b = 0; b < NB; ++b) s[b] = mma32(k[b][i], q[i], s[b]);
     }
     // Scores to probabilities. Keys from `limit` on belong to no one here; masked: some row does not see some key of these.
     template <int NB>
@@ -210,25 +237,21 @@ struct Rows {
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], a.scale2, -base));
-                ls[r & 3] += v;
-                p[b][r >> 3][r & 7] = (T)v;
+            for (int r = 0; r < 16; r += 2) {
+                f32x2 v;
+                v[0] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], a.scale2, -base));
+                v[1] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r + 1], a.scale2, -base));
+                ls[r & 3] += v[0];
+                ls[(r & 3) + 1] += v[1];
+                const auto c = __builtin_convertvector(v, typename Vec8<T>::V2);
+                p[b][r >> 3][r & 7] = c[0];
+                p[b][r >> 3][(r & 7) + 1] = c[1];
             }
         l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
     }
     // Probabilities times values in LDS at Vs.
     template <int NB>
-    __device__ __forceinline__ void values(const AttnArgs &a, const unsigned char *Vs, const V8 (&p)[NB][2], int key, int limit, bool masked) {
-        if (masked) {
-            bool bad = false;
-            for (int e = threadIdx.x & 63; e < NB * 32 * DP / 8; e += 64) bad |= any_nonfinite<T>(*reinterpret_cast<const u32x4 *>(Vs + e * 16));
-            if (__builtin_expect(__any(bad), 0)) {
-#pragma unroll
-                for (int b = 0; b < NB; ++b) spoiled_block(a, Vs, key, b, min(hi, limit), p[b]);
-                return;
-            }
-        }
+    __device__ __forceinline__ void values(const unsigned char *Vs, const V8 (&p)[NB][2]) {
         V8 f[2][DP / 32];           // the fragments of 16 keys are on their way while those of the 16 before them are multiplied
 #pragma unroll
         for (int t = 0; t < DP / 32; ++t) f[0][t] = v_frag(Vs, 0, 0, t);
@@ -247,48 +270,30 @@ struct Rows {
         s16x4 v[2];
 #pragma unroll
         for (int x = 0; x < 2; ++x)
-            v[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(Vs + at_v[t & 1] + (b * 32 + u * 16 + x * 8) * (DP * 2) + (t >> 1) * 128));
+            v[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(Vs + at_v[t] + (b * 32 + u * 16 + x * 8) * (DP * 2)));
         V8 f;
         __builtin_memcpy(&f, v, 16);
         return f;
     }
 
-    // The same for a block that some rows see in part and whose V holds a NaN or an infinity: those values are left out of the matrix product and
-    // multiplied one by one into the rows that see their key.
-    __device__ __forceinline__ void spoiled_block(const AttnArgs &a, const unsigned char *Vs, int key, int b, int end, const V8 (&p)[2]) {
-        const int lane = threadIdx.x & 63, half = lane >> 5;
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int t = 0; t < DP / 32; ++t) {
-                V8 f = v_frag(Vs, b, u, t);
-                u32x4 w;
-                __builtin_memcpy(&w, &f, 16);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t bad = ((w[i] & Vec8<T>::EXP) + Vec8<T>::ONE) & 0x80008000u;
-                    w[i] &= (bad & 0x8000u ? 0u : 0x0000FFFFu) | (bad & 0x80000000u ? 0u : 0xFFFF0000u);
-                }
-                __builtin_memcpy(&f, &w, 16);
-                o[t] = mma32(f, p[u], o[t]);
-                asm volatile("" ::: "memory");
-            }
-#pragma clang loop unroll(disable)
-        for (int kk = 0; kk < 32; ++kk) {
-            const int h = (kk >> 2) & 1, r0 = (kk & 3) + 4 * (kk >> 3), j = key + b * 32 + kk, row = b * 32 + kk;
-            float mine = 0.0f;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) mine = r == r0 ? (float)p[r >> 3][r & 7] : mine;
-            const float pv = __shfl(mine, (lane & 31) + 32 * h);
+    // Values that are no numbers were taken out of the tiles that some row sees in part (clear_values): here they go into the rows that do see them, as
+    // what they make of any sum. (A row that took one in already is what it is.)
+    __device__ __forceinline__ void spoil(const AttnArgs &a, const T *vb, int j0, int j1, int limit) {
+        const int lane = threadIdx.x & 63, half = lane >> 5, end = min(hi, limit);
+        for (int j = j0; j < j1; ++j) {
+            const T *v = vb + (uint64_t)j * a.v_stride;
+            bool bad = false;
+            for (uint32_t d = lane; d < a.dim; d += 64) bad |= !(__builtin_fabsf((float)v[d]) < __builtin_inff());
+            if (!__any(bad)) continue;
             const bool sees = j < end && (j >= lo || j < (int)a.sinks);
 #pragma unroll
             for (int t = 0; t < DP / 32; ++t)
 #pragma unroll
                 for (int x = 0; x < 16; ++x) {
-                    const int d = t * 32 + (x & 3) + 8 * (x >> 2) + 4 * half;
-                    const float f = (float)*reinterpret_cast<const T *>(Vs + row * (DP * 2) + v_place<DP>(row, d >> 3) * 16 + (d & 7) * 2);
-                    if (sees && !(__builtin_fabsf(f) < __builtin_inff())) o[t][x] += pv * f;
-                    asm volatile("" ::: "memory");       // (one value at a time: this path must not cost the other one registers)
+                    const uint32_t d = t * 32 + (x & 3) + 8 * (x >> 2) + 4 * half;
+                    const float f = d < a.dim ? (float)v[d] : 0.0f;
+                    if (sees && !(__builtin_fabsf(f) < __builtin_inff())) o[t][x] += f;
+                    asm volatile("" ::: "memory");       // (one at a time: registers for this would be taken from the loop before)
                 }
         }
     }
@@ -339,8 +344,8 @@ template <class T, int DP, int KEYS, int NT, bool DMA, class Place>
 __device__ __forceinline__ void stage(unsigned char *lds, const T *base, uint64_t stride, int last, uint32_t dim, int t, Place place) {
     constexpr int N = KEYS * DP / 8 / NT, STEP = NT / (DP / 8);          // 16-byte places of a thread, rows between them
     auto to = [&](int i) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)(lds + (size_t)(i * NT + (t & ~63)) * 16)); };
-    if constexpr (DMA && STEP % 8 == 0) {
-        // (places are exchanged by the row's last three bits: the same ones in every step)
+    if constexpr (DMA && STEP % 16 == 0) {
+        // (places are exchanged by the row's last four bits: the same ones in every step)
         if (last == KEYS - 1) {
             const int row = t / (DP / 8), c = place(row, t % (DP / 8));
             if ((uint32_t)(c * 8) < dim)
@@ -380,7 +385,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs a) {
     // neighbouring items (tiles of one key head) on one XCD: it takes every eighth workgroup
     const uint32_t per = items / 8, xcd = blockIdx.x & 7, item = blockIdx.x < per * 8 ? xcd * per + (blockIdx.x >> 3) : blockIdx.x;
     const uint32_t kvh = item / a.slots, slot = item % a.slots;
-    const int b = find_seq(a, slot, BM);
+    const int b = __builtin_amdgcn_readfirstlane(find_seq(a, slot, BM));
     const Seq s = seq_of(a, b);
     const int64_t row0 = ((int64_t)slot - (s.q0 * a.group / BM + b)) * BM;
     if (row0 < 0 || row0 >= (int64_t)s.nq * a.group) return;
@@ -396,6 +401,8 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs a) {
         lo_max = max(lo_max, __shfl_xor(lo_max, o)); hi_min = min(hi_min, __shfl_xor(hi_min, o));
         lo_min = min(lo_min, __shfl_xor(lo_min, o)); hi_max = max(hi_max, __shfl_xor(hi_max, o));
     }
+    lo_max = __builtin_amdgcn_readfirstlane(lo_max); hi_min = __builtin_amdgcn_readfirstlane(hi_min);
+    lo_min = __builtin_amdgcn_readfirstlane(lo_min); hi_max = __builtin_amdgcn_readfirstlane(hi_max);
     const T *kb = (const T *)a.k + (uint64_t)s.k0 * a.k_stride + (uint64_t)kvh * a.k_head, *vb = (const T *)a.v + (uint64_t)s.k0 * a.v_stride + (uint64_t)kvh * a.v_head;
     auto start_of = [&](int i) { return i < n_first ? i * KT : g.begin + (i - n_first) * KT; };
     auto limit_of = [&](int i) { return i < n_first ? g.first : g.end; };
@@ -409,22 +416,31 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs a) {
         for (int e = t; e < 4 * TILE / 16; e += 256) *reinterpret_cast<u32x4 *>(smem + e * 16) = u32x4{0, 0, 0, 0};
         __syncthreads();
     }
+    // the keys that every row of the workgroup sees: from the last row's first one to the first row's last one
+    const int64_t rows_here = (int64_t)s.nq * a.group - row0, p0 = row0 / a.group + s.nk - s.nq, p1 = (row0 + (rows_here < BM ? rows_here : BM) - 1) / a.group + s.nk - s.nq;
+    const int all_hi = a.right < 0 ? s.nk : (int)max((int64_t)0, min((int64_t)s.nk, p0 + a.right + 1)), all_lo = a.left < 0 ? 0 : (int)max((int64_t)0, min((int64_t)s.nk, p1 - a.left));
+    bool spoiled = false;
     if (n > 0) fetch(0);
     for (int i = 0; i < n; ++i) {
         // this tile has arrived, for every wave; nobody reads the other buffer any more
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         if (i + 1 < n) fetch(i + 1);
-        const unsigned char *Ks = smem + (i & 1) * 2 * TILE;
+        unsigned char *Ks = smem + (i & 1) * 2 * TILE;
         const int j = start_of(i), limit = limit_of(i);
+        if (!(j + KT <= min(all_hi, limit) && (j >= all_lo || j + KT <= (int)a.sinks))) {        // some row of the workgroup sees it in part
+            const int found = __syncthreads_or(clear_values<T, 256>(Ks + TILE, TILE, t));
+            spoiled |= found != 0;
+        }
         if (j < hi_max && (j + KT > lo_min || j < (int)a.sinks)) {
             const bool masked = !(j + KT <= min(hi_min, limit) && (j >= lo_max || j + KT <= (int)a.sinks));
             f32x16 sc[KT / 32];
             typename Rows<T, DP>::V8 p[KT / 32][2];
             rows.scores(Ks, sc);
             rows.softmax(a, sc, p, j, limit, masked);
-            rows.values(a, Ks + TILE, p, j, limit, masked);
+            rows.values(Ks + TILE, p);
         }
     }
+    if (spoiled) { rows.spoil(a, vb, 0, g.first, g.first); rows.spoil(a, vb, g.begin, g.end, g.end); }
     rows.store(a, s, half_sum(rows.l));
 }
 
@@ -434,7 +450,7 @@ __global__ __launch_bounds__(256, 2) void attn_split_kernel(const AttnArgs a) {
     constexpr int BM = 32, KT = 32, TILE = KT * DP * 2;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];      // [4 waves][K | V]; then the waves' sums
     const uint32_t kvh = blockIdx.y, slot = blockIdx.x, split = blockIdx.z;
-    const int b = find_seq(a, slot, BM);
+    const int b = __builtin_amdgcn_readfirstlane(find_seq(a, slot, BM));
     const Seq s = seq_of(a, b);
     const int64_t row0 = ((int64_t)slot - (s.q0 * a.group / BM + b)) * BM;
     if (row0 < 0 || row0 >= (int64_t)s.nq * a.group) return;
@@ -447,6 +463,7 @@ __global__ __launch_bounds__(256, 2) void attn_split_kernel(const AttnArgs a) {
     int lo_max = rows.live ? rows.lo : 0, hi_min = rows.live ? rows.hi : 0x7FFFFFFF;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) { lo_max = max(lo_max, __shfl_xor(lo_max, o)); hi_min = min(hi_min, __shfl_xor(hi_min, o)); }
+    lo_max = __builtin_amdgcn_readfirstlane(lo_max); hi_min = __builtin_amdgcn_readfirstlane(hi_min);
     const T *kb = (const T *)a.k + (uint64_t)s.k0 * a.k_stride + (uint64_t)kvh * a.k_head, *vb = (const T *)a.v + (uint64_t)s.k0 * a.v_stride + (uint64_t)kvh * a.v_head;
     unsigned char *Ks = smem + wave * 2 * TILE, *Vs = Ks + TILE;
     auto start_of = [&](int i) { return i < n_first ? i * KT : g.begin + (i - n_first) * KT; };
@@ -471,6 +488,7 @@ __global__ __launch_bounds__(256, 2) void attn_split_kernel(const AttnArgs a) {
         else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_wave_barrier();
     };
+    bool spoiled = false;
     if (i0 + wave < i1) { fetch_k(i0 + wave); fetch_v(i0 + wave); }
     for (int i = i0 + wave; i < i1; i += 4) {
         const int j = start_of(i), limit = limit_of(i);
@@ -483,10 +501,13 @@ __global__ __launch_bounds__(256, 2) void attn_split_kernel(const AttnArgs a) {
         if (more) fetch_k(i + 4);
         rows.softmax(a, sc, p, j, limit, masked);
         arrived(!more);                       // V
-        rows.values(a, Vs, p, j, limit, masked);
+        if (masked) spoiled |= __any(clear_values<T, 64>(Vs, TILE, lane));
+        rows.values(Vs, p);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         if (more) fetch_v(i + 4);
     }
+    if (spoiled)
+        for (int i = i0 + wave; i < i1; i += 4) rows.spoil(a, vb, start_of(i), min(start_of(i) + KT, limit_of(i)), limit_of(i));
     // the four waves' parts, in their order: statistics first, then the sums, 32 features at a time
     float *stat = reinterpret_cast<float *>(smem + 8 * TILE);       // [4][32][2]
     const float part = half_sum(rows.l);
