@@ -342,18 +342,8 @@ __device__ __forceinline__ Range range_of(const AttnArgs &a, const Seq &s, int64
 // scores are replaced, and what V holds there counts as any masked place does.
 template <class T, int DP, int KEYS, int NT, bool DMA, class Place>
 __device__ __forceinline__ void stage(unsigned char *lds, const T *base, uint64_t stride, int last, uint32_t dim, int t, Place place) {
-    constexpr int N = KEYS * DP / 8 / NT, STEP = NT / (DP / 8);          // 16-byte places of a thread, rows between them
+    constexpr int N = KEYS * DP / 8 / NT;          // 16-byte places of a thread
     auto to = [&](int i) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)(lds + (size_t)(i * NT + (t & ~63)) * 16)); };
-    if constexpr (DMA && STEP % 16 == 0) {
-        // (places are exchanged by the row's last four bits: the same ones in every step)
-        if (last == KEYS - 1) {
-            const int row = t / (DP / 8), c = place(row, t % (DP / 8));
-            if ((uint32_t)(c * 8) < dim)
-#pragma unroll
-                for (int i = 0; i < N; ++i) glds16(uniform_ptr((const unsigned char *)(base + (uint64_t)(i * STEP) * stride)), ((uint32_t)row * (uint32_t)stride + c * 8) * 2, to(i));
-            return;
-        }
-    }
     int t2 = t;
     asm volatile("" : "+v"(t2));           // (addresses are formed here, not kept in registers through the loop around)
 #pragma unroll
@@ -373,6 +363,23 @@ __device__ __forceinline__ void stage(unsigned char *lds, const T *base, uint64_
         }
     }
 }
+// 1 .. 4 transfers of 16 bytes a lane from one base to LDS places `step` bytes apart, as one statement
+template <int N>
+__device__ __forceinline__ void glds16_n(const void *base, const uint32_t (&off)[N], uint32_t lds, uint32_t step) {
+    unsigned keep;
+    if constexpr (N == 1)
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0" : "=&s"(keep) : "v"(off[0]), "s"(base), "s"(lds) : "memory");
+    else if constexpr (N == 2)
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %4\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\ts_add_u32 m0, m0, %5\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
+                     : "=&s"(keep) : "v"(off[0]), "v"(off[1]), "s"(base), "s"(lds), "s"(step) : "memory", "scc");
+    else {
+        static_assert(N == 4, "");
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %6\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %5\n\ts_add_u32 m0, m0, %7\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %5\n\t"
+                     "s_add_u32 m0, m0, %7\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %5\n\ts_add_u32 m0, m0, %7\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %4, %5\n\ts_mov_b32 m0, %0"
+                     : "=&s"(keep) : "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base), "s"(lds), "s"(step) : "memory", "scc");
+    }
+}
+__device__ __forceinline__ uint32_t lds_address(const void *p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) unsigned char *)p; }
 template <int DP> struct KPlace { __device__ __forceinline__ int operator()(int row, int c) const { return k_place<DP>(row, c); } };
 template <int DP> struct VPlace { __device__ __forceinline__ int operator()(int row, int c) const { return v_place<DP>(row, c); } };
 
@@ -406,11 +413,32 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs a) {
     const T *kb = (const T *)a.k + (uint64_t)s.k0 * a.k_stride + (uint64_t)kvh * a.k_head, *vb = (const T *)a.v + (uint64_t)s.k0 * a.v_stride + (uint64_t)kvh * a.v_head;
     auto start_of = [&](int i) { return i < n_first ? i * KT : g.begin + (i - n_first) * KT; };
     auto limit_of = [&](int i) { return i < n_first ? g.first : g.end; };
+    // whole tiles: the lane's offsets from a base that moves on with the tiles
+    constexpr int N = KT * DP / 8 / 256, STEP = 256 / (DP / 8);
+    uint32_t off_k[N], off_v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int row = i * STEP + t / (DP / 8), x = t % (DP / 8);
+        off_k[i] = ((uint32_t)row * (uint32_t)a.k_stride + k_place<DP>(row, x) * 8) * 2;
+        off_v[i] = ((uint32_t)row * (uint32_t)a.v_stride + v_place<DP>(row, x) * 8) * 2;
+    }
+    const uint32_t lds0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds_address(smem) + wave * 1024));
+    const T *kn = kb + (n_first ? 0 : (uint64_t)g.begin * a.k_stride), *vn = vb + (n_first ? 0 : (uint64_t)g.begin * a.v_stride);       // the next tile's
+    const uint64_t k_step = (uint64_t)KT * a.k_stride, v_step = (uint64_t)KT * a.v_stride;
+    const bool whole = a.dim == DP;
     auto fetch = [&](int i) {
-        const int j = start_of(i), last = min(KT, limit_of(i) - j) - 1;
-        unsigned char *Ks = smem + (i & 1) * 2 * TILE;
-        stage<T, DP, KT, 256, DMA>(Ks, kb + (uint64_t)j * a.k_stride, a.k_stride, last, a.dim, t, KPlace<DP>());
-        stage<T, DP, KT, 256, DMA>(Ks + TILE, vb + (uint64_t)j * a.v_stride, a.v_stride, last, a.dim, t, VPlace<DP>());
+        const int last = min(KT, limit_of(i) - start_of(i)) - 1;
+        if (DMA && whole && last == KT - 1) {
+            const uint32_t to = lds0 + (i & 1) * 2 * TILE;
+            glds16_n(uniform_ptr((const unsigned char *)kn), off_k, to, 4096);
+            glds16_n(uniform_ptr((const unsigned char *)vn), off_v, to + TILE, 4096);
+        } else {
+            unsigned char *Ks = smem + (i & 1) * 2 * TILE;
+            stage<T, DP, KT, 256, DMA>(Ks, kn, a.k_stride, last, a.dim, t, KPlace<DP>());
+            stage<T, DP, KT, 256, DMA>(Ks + TILE, vn, a.v_stride, last, a.dim, t, VPlace<DP>());
+        }
+        if (i + 1 == n_first) { kn = kb + (uint64_t)g.begin * a.k_stride; vn = vb + (uint64_t)g.begin * a.v_stride; }
+        else { kn += k_step; vn += v_step; }
     };
     if (DMA && a.dim < DP) {
         for (int e = t; e < 4 * TILE / 16; e += 256) *reinterpret_cast<u32x4 *>(smem + e * 16) = u32x4{0, 0, 0, 0};
