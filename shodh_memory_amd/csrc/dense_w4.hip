@@ -8,7 +8,7 @@
 //  * a 4-bit number becomes a matrix operand with a shift and an and-or per PAIR: or-ed into the mantissa of 16.0 it reads as 16 + q, in bf16 as in
 //    fp16, exactly. sum x (16 + q) - (16 + z) sum x is the group's sum; sum x comes from the same matrix instruction with ones for weights, in the same
 //    order. int8 rows multiply q as a byte: sums exact in int32, (q - z) likewise;
-//  * f32 rows are split into three bf16 parts (8 + 8 + 8 bits, by truncation, exact): three products, sums in f32;
+//  * f32 rows are split into three bf16 parts (8 + 8 + 8 bits, by truncation, exact): three products with q - z itself, sums in f32;
 //  * scales multiply the f32 sum of a group, so no weight is rounded to 16 bits on the way.
 // A row of x that holds a NaN or an infinity gives NaN in all its outputs (16 x - 16 x).
 #include "layers.h"
@@ -158,13 +158,15 @@ __device__ __forceinline__ void x_convert(XFrag<X> &f, const typename XFrag<X>::
         f.v[0][1] = __builtin_amdgcn_perm(hi, lo, 0x07030602u);
     }
 }
-template <int X>
-__device__ __forceinline__ void x_load(XFrag<X> &f, const typename XFrag<X>::E *p, uint32_t n /* elements in the row from here on */) {
+template <int X, bool END>
+__device__ __forceinline__ XFrag<X> x_load(const typename XFrag<X>::E *p, uint32_t n /* END: elements left in the row */) {
     typename XFrag<X>::E e[8];
-    if (n >= 8) load_any(e, p);
+    if (!END || n >= 8) load_any(e, p);
     else
         for (int i = 0; i < 8; ++i) e[i] = (uint32_t)i < n ? p[i] : (typename XFrag<X>::E)0;
+    XFrag<X> f;
     x_convert<X>(f, e);
+    return f;
 }
 
 template <int X> struct WFrag { u32x4 v; };
@@ -181,6 +183,17 @@ __device__ __forceinline__ WFrag<X> w_expand(uint32_t w) {
         f.v[2] = ((w >> 5) & 0x00780078u) | 0x41804180u; f.v[3] = ((w >> 9) & 0x00780078u) | 0x41804180u;
     }
     return f;
+}
+// f32 rows: the weights' own numbers q - z (exact in bf16), so that nothing cancels; zero = 16 + z of the lane's output
+__device__ __forceinline__ WFrag<W4_F32> w_expand_exact(uint32_t w, float zero) {
+    const WFrag<W4_F32> f = w_expand<W4_F32>(w);
+    WFrag<W4_F32> r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float lo = __uint_as_float(f.v[i] << 16) - zero, hi = __uint_as_float(f.v[i] & 0xFFFF0000u) - zero;
+        r.v[i] = __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+    }
+    return r;
 }
 template <int X>
 __device__ __forceinline__ WFrag<X> w_ones() {
@@ -202,96 +215,144 @@ __device__ __forceinline__ typename Acc<X>::V mma(const WFrag<X> &a, const XFrag
     }
 }
 
-// A workgroup of `waves` waves: 16 outputs, MT x 16 rows; wave i takes the records i, i + waves, ... of its outputs, and the waves' sums are added in
-// their order. Matrix layouts: operand lane = output (weights) or row (x) lane & 15, inputs 8 (lane >> 4) ..; result lane = row lane & 15,
-// outputs 4 (lane >> 4) .. + 3.
-template <int X, int GROUP, int MT>
-__global__ __launch_bounds__(512) void w4_dense_kernel(const W4Args a) {
-    using F = XFrag<X>;
-    using E = typename F::E;
-    using V = typename Acc<X>::V;
-    extern __shared__ float sums[];              // [waves][MT][64][4]
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, quad = lane >> 4;
-    const uint32_t m0 = blockIdx.y * 64u;
-    constexpr int PER = W4_TK / GROUP, STEPS = GROUP / 32;       // groups of a record; steps of 32 inputs of a group
-    const E *xr[MT];
-    bool in[MT];
+// What a wave holds of NT records of one block of inputs, and of x next to them.
+template <int X, int GROUP, int MT, int NT>
+struct Block {
+    static constexpr int PER = W4_TK / GROUP, STEPS = GROUP / 32;       // groups of a record; steps of 32 inputs of a group
+    static constexpr bool EXACT = X == W4_F32;
+    u32x4 w[NT];
+    u32x2 s[NT][PER];
+    uint32_t z[NT][PER];
+    XFrag<X> x[4][MT];
+
+    __device__ __forceinline__ void load_w(const W4Args &a, const uint8_t *const (&rec)[NT], size_t at, int lane) {
+        const int quad = lane >> 4;
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        const uint32_t m = m0 + i * 16 + (lane & 15);
-        in[i] = m < a.M;
-        xr[i] = (const E *)a.x + (uint64_t)(in[i] ? m : 0) * a.x_stride + 8 * quad;
+        for (int j = 0; j < NT; ++j) {
+            const uint8_t *r = rec[j] + at;
+            w[j] = *reinterpret_cast<const u32x4 *>(r + lane * 16);
+#pragma unroll
+            for (int g = 0; g < PER; ++g) {
+                s[j][g] = *reinterpret_cast<const u32x2 *>(r + 1024 + g * 32 + quad * 8);
+                z[j][g] = !a.zeros ? 0x18181818u : EXACT ? r[1024 + PER * 32 + g * 16 + (lane & 15)] : *reinterpret_cast<const uint32_t *>(r + 1024 + PER * 32 + g * 16 + quad * 4);
+            }
+        }
     }
-    f32x4 acc[MT];
+    template <bool END>
+    __device__ __forceinline__ void load_x(const W4Args &a, const typename XFrag<X>::E *const (&xr)[MT], uint32_t k, int lane) {
+        const uint32_t k0 = k + 8 * (lane >> 4);
 #pragma unroll
-    for (int i = 0; i < MT; ++i) acc[i] = f32x4{0, 0, 0, 0};
-    const WFrag<X> ones = w_ones<X>();
-    const uint8_t *rec = a.w + ((size_t)blockIdx.x * a.blocks + wave) * a.record;
-    for (uint32_t block = wave; block < a.blocks; block += waves, rec += (size_t)waves * a.record) {
-        const u32x4 w = *reinterpret_cast<const u32x4 *>(rec + lane * 16);
-        const uint32_t k0 = block * W4_TK + 8 * quad;
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) x[t][i] = x_load<X, END>(xr[i] + k + 32 * t, k0 + 32 * t < a.K ? a.K - k0 - 32 * t : 0);
+    }
+    __device__ __forceinline__ void multiply(const W4Args &a, f32x4 (&acc)[NT][MT]) const {
+        using V = typename Acc<X>::V;
+        const WFrag<X> ones = w_ones<X>();
 #pragma unroll
         for (int g = 0; g < PER; ++g) {
-            V d[MT], s[MT];
+            V d[NT][MT], sum[MT];
 #pragma unroll
-            for (int i = 0; i < MT; ++i) { d[i] = V{0, 0, 0, 0}; s[i] = V{0, 0, 0, 0}; }
+            for (int i = 0; i < MT; ++i) {
+                sum[i] = V{0, 0, 0, 0};
 #pragma unroll
-            for (int j = 0; j < STEPS; ++j) {
-                const int step = g * STEPS + j;
-                const uint32_t k = k0 + 32 * step;
-                const WFrag<X> wf = w_expand<X>(w[step]);
-#pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    F xf;
-                    x_load<X>(xf, xr[i] + block * W4_TK + 32 * step, in[i] && k < a.K ? a.K - k : 0);
-                    d[i] = mma<X>(wf, xf, d[i]);
-                    s[i] = mma<X>(ones, xf, s[i]);
-                }
-            }
-            float scale[4], zero[4];
-            {
-                const u32x2 raw = *reinterpret_cast<const u32x2 *>(rec + 1024 + g * 32 + quad * 8);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const uint16_t h = (uint16_t)(raw[r >> 1] >> (16 * (r & 1)));
-                    scale[r] = a.scale_f16 ? (float)__builtin_bit_cast(_Float16, h) : __uint_as_float((uint32_t)h << 16);
-                }
-                const uint32_t zb = a.zeros ? *reinterpret_cast<const uint32_t *>(rec + 1024 + PER * 32 + g * 16 + quad * 4) : 0x18181818u;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) zero[r] = (float)((zb >> (8 * r)) & 255u);
+                for (int j = 0; j < NT; ++j) d[j][i] = V{0, 0, 0, 0};
             }
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
+            for (int t = g * STEPS; t < (g + 1) * STEPS; ++t) {
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    WFrag<X> wf;
+                    if constexpr (EXACT) wf = w_expand_exact(w[j][t], (float)(z[j][g] & 255u));
+                    else wf = w_expand<X>(w[j][t]);
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) d[j][i] = mma<X>(wf, x[t][i], d[j][i]);
+                }
+                if constexpr (!EXACT)
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) sum[i] = mma<X>(ones, x[t][i], sum[i]);
+            }
+            if constexpr (PER > 1) __builtin_amdgcn_sched_barrier(0);          // (groups one after another: side by side they would only cost registers)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    float v;
-                    if constexpr (X == W4_I8) v = (float)(d[i][r] - ((int)zero[r] - 16) * s[i][r]);
-                    else v = __builtin_fmaf(-zero[r], s[i][r], d[i][r]);
-                    acc[i][r] = __builtin_fmaf(v, scale[r], acc[i][r]);
+                    const uint16_t h = (uint16_t)(s[j][g][r >> 1] >> (16 * (r & 1)));
+                    const float scale = a.scale_f16 ? (float)__builtin_bit_cast(_Float16, h) : __uint_as_float((uint32_t)h << 16);
+                    const int zero = (int)((z[j][g] >> (8 * r)) & 255u);
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        float v;
+                        if constexpr (X == W4_I8) v = (float)(d[j][i][r] - (zero - 16) * sum[i][r]);
+                        else if constexpr (EXACT) v = d[j][i][r];
+                        else v = __builtin_fmaf(-(float)zero, sum[i][r], d[j][i][r]);
+                        acc[j][i][r] = __builtin_fmaf(v, scale, acc[j][i][r]);
+                    }
                 }
         }
     }
+};
+
+// A workgroup of `waves` waves: NT x 16 outputs, MT x 16 rows; wave i takes the blocks of 128 inputs i, i + waves, ..., and the waves' sums are added in
+// their order. Matrix layouts: operand lane = output (weights) or row (x) lane & 15, inputs 8 (lane >> 4) ..; result lane = row lane & 15,
+// outputs 4 (lane >> 4) .. + 3. The next U blocks are on their way while U are multiplied.
+template <int X, int GROUP, int MT, int NT, int U>
+__global__ __launch_bounds__(512) void w4_dense_kernel(const W4Args a) {
+    using E = typename XFrag<X>::E;
+    extern __shared__ float sums[];              // [waves][NT][MT][64][4]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const uint32_t m0 = blockIdx.y * 64u, tiles = (a.N + W4_TN - 1) / W4_TN;
+    const E *xr[MT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) *reinterpret_cast<f32x4 *>(sums + ((wave * MT + i) * 64 + lane) * 4) = acc[i];
+    for (int i = 0; i < MT; ++i) xr[i] = (const E *)a.x + (uint64_t)min(m0 + i * 16 + (lane & 15), a.M - 1) * a.x_stride + 8 * (lane >> 4);     // (rows behind the last repeat it: not written)
+    const uint8_t *rec[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) rec[j] = a.w + (size_t)min(blockIdx.x * NT + j, tiles - 1) * a.blocks * a.record;
+    f32x4 acc[NT][MT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0, 0, 0, 0};
+    const uint32_t whole = a.K / W4_TK;          // blocks without the row's end
+    Block<X, GROUP, MT, NT> b[U];
+    uint32_t at = wave;
+    for (; at + (U - 1) * waves < whole; at += U * waves) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) b[u].load_w(a, rec, (size_t)(at + u * waves) * a.record, lane);
+#pragma unroll
+        for (int u = 0; u < U; ++u) b[u].template load_x<false>(a, xr, (at + u * waves) * W4_TK, lane);
+#pragma unroll
+        for (int u = 0; u < U; ++u) b[u].multiply(a, acc);
+    }
+    for (; at < a.blocks; at += waves) {
+        b[0].load_w(a, rec, (size_t)at * a.record, lane);
+        if (at < whole) b[0].template load_x<false>(a, xr, at * W4_TK, lane);
+        else b[0].template load_x<true>(a, xr, at * W4_TK, lane);
+        b[0].multiply(a, acc);
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) *reinterpret_cast<f32x4 *>(sums + (((wave * NT + j) * MT + i) * 64 + lane) * 4) = acc[j][i];
     __syncthreads();
-    for (int e = threadIdx.x; e < MT * 64; e += blockDim.x) {
+    for (int e = threadIdx.x; e < NT * MT * 64; e += blockDim.x) {
         f32x4 v = *reinterpret_cast<const f32x4 *>(sums + e * 4);
-        for (int w2 = 1; w2 < waves; ++w2) v += *reinterpret_cast<const f32x4 *>(sums + (w2 * MT * 64 + e) * 4);
-        const uint32_t m = m0 + (e >> 6) * 16 + (e & 15), n = blockIdx.x * W4_TN + ((e & 63) >> 4) * 4;
+        for (int w2 = 1; w2 < waves; ++w2) v += *reinterpret_cast<const f32x4 *>(sums + (w2 * NT * MT * 64 + e) * 4);
+        const uint32_t m = m0 + ((e >> 6) % MT) * 16 + (e & 15), n = (blockIdx.x * NT + (e >> 6) / MT) * W4_TN + ((e & 63) >> 4) * 4;
         if (m >= a.M || n >= a.N) continue;
         const float xs = X == W4_I8 ? a.x_scale[m] : 1.0f;
         float o[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) o[r] = (X == W4_I8 ? v[r] * xs : v[r]) + (a.bias && n + r < a.N ? a.bias[n + r] : 0.0f);
-        const uint64_t at = (uint64_t)m * a.y_stride + n;
+        const uint64_t to = (uint64_t)m * a.y_stride + n;
         auto put = [&](auto *y) {
             using Y = std::remove_reference_t<decltype(*y)>;
             Y t[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) t[r] = (Y)o[r];
-            if (n + 4 <= a.N) store_any(y + at, t);
+            if (n + 4 <= a.N) store_any(y + to, t);
             else
-                for (int r = 0; r < 4; ++r) if (n + r < a.N) y[at + r] = t[r];
+                for (int r = 0; r < 4; ++r) if (n + r < a.N) y[to + r] = t[r];
         };
         if (a.y_dtype == SHODH_DTYPE_FP32) put((float *)a.y);
         else if (a.y_dtype == SHODH_DTYPE_BF16) put((__bf16 *)a.y);
@@ -300,20 +361,25 @@ __global__ __launch_bounds__(512) void w4_dense_kernel(const W4Args a) {
 }
 
 template <int X, int GROUP>
-static int launch_w4(const W4Args &a, uint32_t tiles, hipStream_t st) {
-    const uint32_t waves = a.blocks >= 8 ? 8 : a.blocks >= 4 ? 4 : a.blocks >= 2 ? 2 : 1;
-    auto go = [&](auto kern, int mt) {
-        hipLaunchKernelGGL(kern, dim3(tiles, (a.M + 63) / 64), dim3(64 * waves), (size_t)waves * mt * 1024, st, a);
+static int launch_w4(const W4Args &a, uint32_t tiles, int cus, hipStream_t st) {
+    auto go = [&](auto kern, uint32_t mt, uint32_t nt, uint32_t most) -> int {
+        uint32_t waves = 1;
+        while (waves < most && waves * 2 <= a.blocks) waves *= 2;
+        const size_t lds = (size_t)waves * mt * nt * 1024;
+        SHODH_TRY(ensure_dynamic_lds((const void *)kern, lds));
+        hipLaunchKernelGGL(kern, dim3((tiles + nt - 1) / nt, (a.M + 63) / 64), dim3(64 * waves), lds, st, a);
+        SHODH_HIP_TRY(hipGetLastError());
+        return SHODH_OK;
     };
-    if (a.M <= 16) go(w4_dense_kernel<X, GROUP, 1>, 1);
-    else if (a.M <= 32) go(w4_dense_kernel<X, GROUP, 2>, 2);
-    else go(w4_dense_kernel<X, GROUP, 4>, 4);
-    SHODH_HIP_TRY(hipGetLastError());
-    return SHODH_OK;
+    const uint32_t wide = (uint32_t)cus;          // more outputs a wave once there are workgroups for every CU all the same
+    if (a.M <= 16) return go(w4_dense_kernel<X, GROUP, 1, 1, 4>, 1, 1, 8);
+    if (a.M <= 32) return tiles >= 2 * wide ? go(w4_dense_kernel<X, GROUP, 2, 2, 1>, 2, 2, 8) : go(w4_dense_kernel<X, GROUP, 2, 1, 2>, 2, 1, 8);
+    return tiles >= 2 * wide ? go(w4_dense_kernel<X, GROUP, 4, 2, 1>, 4, 2, 8) : go(w4_dense_kernel<X, GROUP, 4, 1, 1>, 4, 1, 8);
 }
 template <int X>
 static int pick_w4(const W4Args &a, const shodh_w4_weight *w, hipStream_t st) {
-    return w->group == 32 ? launch_w4<X, 32>(a, w->tiles, st) : w->group == 64 ? launch_w4<X, 64>(a, w->tiles, st) : launch_w4<X, 128>(a, w->tiles, st);
+    const int cus = compute_units(w->device);
+    return w->group == 32 ? launch_w4<X, 32>(a, w->tiles, cus, st) : w->group == 64 ? launch_w4<X, 64>(a, w->tiles, cus, st) : launch_w4<X, 128>(a, w->tiles, cus, st);
 }
 
 static int check_w4(uint32_t N, uint32_t K, uint32_t group, uint32_t scale_dtype, shodh_w4_weight **out) {
