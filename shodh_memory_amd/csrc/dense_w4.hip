@@ -120,7 +120,9 @@ struct W4Args {
     const float *x_scale, *bias;
     void *y;
     uint64_t x_stride, y_stride;
-    uint32_t M, N, K, blocks, record, y_dtype, scale_f16, zeros;
+    uint32_t M, N, K, blocks, record, y_dtype;
+    uint32_t f16_mask;          // all ones: scales are fp16; 0: bf16
+    uint32_t zero_at, zero_mask, zero_else;     // place of the zero points in a record, or (mask 0) of anything, and what stands in for them
 };
 
 enum { W4_BF16 = 0, W4_F16 = 1, W4_F32 = 2, W4_I8 = 3 };      // type of x
@@ -158,16 +160,39 @@ __device__ __forceinline__ void x_convert(XFrag<X> &f, const typename XFrag<X>::
         f.v[0][1] = __builtin_amdgcn_perm(hi, lo, 0x07030602u);
     }
 }
-template <int X, bool END>
-__device__ __forceinline__ XFrag<X> x_load(const typename XFrag<X>::E *p, uint32_t n /* END: elements left in the row */) {
-    typename XFrag<X>::E e[8];
-    if (!END || n >= 8) load_any(e, p);
-    else
-        for (int i = 0; i < 8; ++i) e[i] = (uint32_t)i < n ? p[i] : (typename XFrag<X>::E)0;
-    XFrag<X> f;
-    x_convert<X>(f, e);
-    return f;
-}
+// A block of 128 inputs of a row is PLACES pieces of 16 bytes, loaded by neighbouring lanes (a wave's load of fragments straight from memory would be 64
+// separate lines) and turned into fragments through LDS. There a piece's place is exchanged by the row's number, so that 16 rows' same place meets on
+// no LDS banks.
+template <int X>
+struct Piece {
+    using E = typename XFrag<X>::E;
+    static constexpr int PER = 16 / (int)sizeof(E), ROW = W4_TK * (int)sizeof(E), PLACES = ROW / 16;
+    static __device__ __forceinline__ int place(int row, int c) { return sizeof(E) == 1 ? c ^ ((row >> 1) & 7) : sizeof(E) == 2 ? c ^ (row & 15) : c ^ ((row & 15) << 1); }
+    static __device__ __forceinline__ u32x4 load(const E *row, uint32_t k0, int c, uint32_t K) {
+        const uint32_t k = k0 + c * PER;
+        E v[PER];
+        if (k0 + W4_TK <= K) load_any(v, row + k);          // (the same for all lanes)
+        else
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const E w = row[min(k + i, K - 1)];
+                v[i] = k + i < K ? w : (E)0;
+            }
+        return __builtin_bit_cast(u32x4, v);
+    }
+    static __device__ __forceinline__ void store(unsigned char *xs, int row, int c, u32x4 v) { *reinterpret_cast<u32x4 *>(xs + row * ROW + place(row, c) * 16) = v; }
+    // the lane's 8 inputs of step s of a row
+    static __device__ __forceinline__ XFrag<X> fragment(const unsigned char *xs, int row, int s, int quad) {
+        E e[8];
+        const unsigned char *r = xs + row * ROW;
+        if constexpr (sizeof(E) == 1) __builtin_memcpy(e, r + place(row, 2 * s + (quad >> 1)) * 16 + (quad & 1) * 8, 8);
+        else if constexpr (sizeof(E) == 2) __builtin_memcpy(e, r + place(row, 4 * s + quad) * 16, 16);
+        else __builtin_memcpy(e, r + place(row, 2 * (4 * s + quad)) * 16, 32);
+        XFrag<X> f;
+        x_convert<X>(f, e);
+        return f;
+    }
+};
 
 template <int X> struct WFrag { u32x4 v; };
 template <> struct WFrag<W4_I8> { u32x2 v; };
@@ -176,11 +201,15 @@ __device__ __forceinline__ WFrag<X> w_expand(uint32_t w) {
     WFrag<X> f;
     if constexpr (X == W4_I8) { f.v[0] = w & 0x0F0F0F0Fu; f.v[1] = (w >> 4) & 0x0F0F0F0Fu; }
     else if constexpr (X == W4_F16) {
-        f.v[0] = ((w << 6) & 0x03C003C0u) | 0x4C004C00u; f.v[1] = ((w << 2) & 0x03C003C0u) | 0x4C004C00u;
-        f.v[2] = ((w >> 2) & 0x03C003C0u) | 0x4C004C00u; f.v[3] = ((w >> 6) & 0x03C003C0u) | 0x4C004C00u;
+        uint32_t base = 0x4C004C00u;
+        asm("" : "+v"(base));             // (in a vector register: and and or are one instruction then)
+        f.v[0] = ((w << 6) & 0x03C003C0u) | base; f.v[1] = ((w << 2) & 0x03C003C0u) | base;
+        f.v[2] = ((w >> 2) & 0x03C003C0u) | base; f.v[3] = ((w >> 6) & 0x03C003C0u) | base;
     } else {
-        f.v[0] = ((w << 3) & 0x00780078u) | 0x41804180u; f.v[1] = ((w >> 1) & 0x00780078u) | 0x41804180u;
-        f.v[2] = ((w >> 5) & 0x00780078u) | 0x41804180u; f.v[3] = ((w >> 9) & 0x00780078u) | 0x41804180u;
+        uint32_t base = 0x41804180u;
+        asm("" : "+v"(base));
+        f.v[0] = ((w << 3) & 0x00780078u) | base; f.v[1] = ((w >> 1) & 0x00780078u) | base;
+        f.v[2] = ((w >> 5) & 0x00780078u) | base; f.v[3] = ((w >> 9) & 0x00780078u) | base;
     }
     return f;
 }
@@ -215,7 +244,7 @@ __device__ __forceinline__ typename Acc<X>::V mma(const WFrag<X> &a, const XFrag
     }
 }
 
-// What a wave holds of NT records of one block of inputs, and of x next to them.
+// What a wave holds of NT records of one block of inputs.
 template <int X, int GROUP, int MT, int NT>
 struct Block {
     static constexpr int PER = W4_TK / GROUP, STEPS = GROUP / 32;       // groups of a record; steps of 32 inputs of a group
@@ -223,7 +252,6 @@ struct Block {
     u32x4 w[NT];
     u32x2 s[NT][PER];
     uint32_t z[NT][PER];
-    XFrag<X> x[4][MT];
 
     __device__ __forceinline__ void load_w(const W4Args &a, const uint8_t *const (&rec)[NT], size_t at, int lane) {
         const int quad = lane >> 4;
@@ -234,19 +262,13 @@ struct Block {
 #pragma unroll
             for (int g = 0; g < PER; ++g) {
                 s[j][g] = *reinterpret_cast<const u32x2 *>(r + 1024 + g * 32 + quad * 8);
-                z[j][g] = !a.zeros ? 0x18181818u : EXACT ? r[1024 + PER * 32 + g * 16 + (lane & 15)] : *reinterpret_cast<const uint32_t *>(r + 1024 + PER * 32 + g * 16 + quad * 4);
+                z[j][g] = (EXACT ? (uint32_t)r[a.zero_at + g * 16 + (lane & 15)] : *reinterpret_cast<const uint32_t *>(r + a.zero_at + g * 16 + quad * 4)) & a.zero_mask | a.zero_else;
             }
         }
     }
-    template <bool END>
-    __device__ __forceinline__ void load_x(const W4Args &a, const typename XFrag<X>::E *const (&xr)[MT], uint32_t k, int lane) {
-        const uint32_t k0 = k + 8 * (lane >> 4);
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int i = 0; i < MT; ++i) x[t][i] = x_load<X, END>(xr[i] + k + 32 * t, k0 + 32 * t < a.K ? a.K - k0 - 32 * t : 0);
-    }
-    __device__ __forceinline__ void multiply(const W4Args &a, f32x4 (&acc)[NT][MT]) const {
+    // fragment(t, i): x's step t of tile i
+    template <class Fragment>
+    __device__ __forceinline__ void multiply(const W4Args &a, f32x4 (&acc)[NT][MT], Fragment fragment) const {
         using V = typename Acc<X>::V;
         const WFrag<X> ones = w_ones<X>();
 #pragma unroll
@@ -260,17 +282,20 @@ struct Block {
             }
 #pragma unroll
             for (int t = g * STEPS; t < (g + 1) * STEPS; ++t) {
+                XFrag<X> x[MT];
+#pragma unroll
+                for (int i = 0; i < MT; ++i) x[i] = fragment(t, i);
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
                     WFrag<X> wf;
                     if constexpr (EXACT) wf = w_expand_exact(w[j][t], (float)(z[j][g] & 255u));
                     else wf = w_expand<X>(w[j][t]);
 #pragma unroll
-                    for (int i = 0; i < MT; ++i) d[j][i] = mma<X>(wf, x[t][i], d[j][i]);
+                    for (int i = 0; i < MT; ++i) d[j][i] = mma<X>(wf, x[i], d[j][i]);
                 }
                 if constexpr (!EXACT)
 #pragma unroll
-                    for (int i = 0; i < MT; ++i) sum[i] = mma<X>(ones, x[t][i], sum[i]);
+                    for (int i = 0; i < MT; ++i) sum[i] = mma<X>(ones, x[i], sum[i]);
             }
             if constexpr (PER > 1) __builtin_amdgcn_sched_barrier(0);          // (groups one after another: side by side they would only cost registers)
 #pragma unroll
@@ -278,7 +303,7 @@ struct Block {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const uint16_t h = (uint16_t)(s[j][g][r >> 1] >> (16 * (r & 1)));
-                    const float scale = a.scale_f16 ? (float)__builtin_bit_cast(_Float16, h) : __uint_as_float((uint32_t)h << 16);
+                    const float scale = __uint_as_float((__float_as_uint((float)__builtin_bit_cast(_Float16, h)) & a.f16_mask) | (((uint32_t)h << 16) & ~a.f16_mask));
                     const int zero = (int)((z[j][g] >> (8 * r)) & 255u);
 #pragma unroll
                     for (int i = 0; i < MT; ++i) {
@@ -293,52 +318,19 @@ struct Block {
     }
 };
 
-// A workgroup of `waves` waves: NT x 16 outputs, MT x 16 rows; wave i takes the blocks of 128 inputs i, i + waves, ..., and the waves' sums are added in
-// their order. Matrix layouts: operand lane = output (weights) or row (x) lane & 15, inputs 8 (lane >> 4) ..; result lane = row lane & 15,
-// outputs 4 (lane >> 4) .. + 3. The next U blocks are on their way while U are multiplied.
-template <int X, int GROUP, int MT, int NT, int U>
-__global__ __launch_bounds__(512) void w4_dense_kernel(const W4Args a) {
-    using E = typename XFrag<X>::E;
-    extern __shared__ float sums[];              // [waves][NT][MT][64][4]
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    const uint32_t m0 = blockIdx.y * 64u, tiles = (a.N + W4_TN - 1) / W4_TN;
-    const E *xr[MT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) xr[i] = (const E *)a.x + (uint64_t)min(m0 + i * 16 + (lane & 15), a.M - 1) * a.x_stride + 8 * (lane >> 4);     // (rows behind the last repeat it: not written)
-    const uint8_t *rec[NT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) rec[j] = a.w + (size_t)min(blockIdx.x * NT + j, tiles - 1) * a.blocks * a.record;
-    f32x4 acc[NT][MT];
+// The waves' sums in their order (through LDS), the row's scale, the bias, the output's type. `first` of `parts` waves that share outputs; t of nt threads.
+template <int X, int MT, int NT>
+__device__ __forceinline__ void finish(const W4Args &a, const f32x4 (&acc)[NT][MT], float *sums /* [parts][NT][MT][64][4], free when called */, int part, int parts, int t, int nt, uint32_t m0,
+                                       uint32_t tile0, int lane) {
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0, 0, 0, 0};
-    const uint32_t whole = a.K / W4_TK;          // blocks without the row's end
-    Block<X, GROUP, MT, NT> b[U];
-    uint32_t at = wave;
-    for (; at + (U - 1) * waves < whole; at += U * waves) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) b[u].load_w(a, rec, (size_t)(at + u * waves) * a.record, lane);
-#pragma unroll
-        for (int u = 0; u < U; ++u) b[u].template load_x<false>(a, xr, (at + u * waves) * W4_TK, lane);
-#pragma unroll
-        for (int u = 0; u < U; ++u) b[u].multiply(a, acc);
-    }
-    for (; at < a.blocks; at += waves) {
-        b[0].load_w(a, rec, (size_t)at * a.record, lane);
-        if (at < whole) b[0].template load_x<false>(a, xr, at * W4_TK, lane);
-        else b[0].template load_x<true>(a, xr, at * W4_TK, lane);
-        b[0].multiply(a, acc);
-    }
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int i = 0; i < MT; ++i) *reinterpret_cast<f32x4 *>(sums + (((wave * NT + j) * MT + i) * 64 + lane) * 4) = acc[j][i];
+        for (int i = 0; i < MT; ++i) *reinterpret_cast<f32x4 *>(sums + (((part * NT + j) * MT + i) * 64 + lane) * 4) = acc[j][i];
     __syncthreads();
-    for (int e = threadIdx.x; e < NT * MT * 64; e += blockDim.x) {
+    for (int e = t; e < NT * MT * 64; e += nt) {
         f32x4 v = *reinterpret_cast<const f32x4 *>(sums + e * 4);
-        for (int w2 = 1; w2 < waves; ++w2) v += *reinterpret_cast<const f32x4 *>(sums + (w2 * NT * MT * 64 + e) * 4);
-        const uint32_t m = m0 + ((e >> 6) % MT) * 16 + (e & 15), n = (blockIdx.x * NT + (e >> 6) / MT) * W4_TN + ((e & 63) >> 4) * 4;
+        for (int w2 = 1; w2 < parts; ++w2) v += *reinterpret_cast<const f32x4 *>(sums + (w2 * NT * MT * 64 + e) * 4);
+        const uint32_t m = m0 + ((e >> 6) % MT) * 16 + (e & 15), n = (tile0 + (e >> 6) / MT) * W4_TN + ((e & 63) >> 4) * 4;
         if (m >= a.M || n >= a.N) continue;
         const float xs = X == W4_I8 ? a.x_scale[m] : 1.0f;
         float o[4];
@@ -360,21 +352,149 @@ __global__ __launch_bounds__(512) void w4_dense_kernel(const W4Args a) {
     }
 }
 
+// A workgroup of `waves` waves: NT x 16 outputs, MT x 16 rows; wave i takes the blocks of 128 inputs i, i + waves, ..., and the waves' sums are added in
+// their order. Matrix layouts: operand lane = output (weights) or row (x) lane & 15, inputs 8 (lane >> 4) ..; result lane = row lane & 15,
+// outputs 4 (lane >> 4) .. + 3. U blocks are asked for before the first is multiplied; with U = 1 the next one is on its way meanwhile.
+// FEW: there are no more rows than one piece a lane covers (2, 4 or 8 by type): the others' columns hold whatever LDS held, and are not written.
+template <int X, int GROUP, int MT, int NT, int U, bool FEW>
+__global__ __launch_bounds__(512, FEW && GROUP != 32 ? 6 : MT == 1 ? 4 : 2) void w4_dense_kernel(const W4Args a) {
+    using P = Piece<X>;
+    using E = typename P::E;
+    constexpr int STEP = 64 / P::PLACES, PIECES = FEW ? 1 : MT * 16 / STEP, TILE = MT * 16 * P::ROW;         // rows between a lane's pieces of a block, their number
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];           // [waves][TILE]; then the sums
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const uint32_t m0 = blockIdx.y * (MT * 16u), tiles = (a.N + W4_TN - 1) / W4_TN;
+    unsigned char *xs = smem + wave * TILE;
+    const int piece_row = lane / P::PLACES, piece_place = lane % P::PLACES;
+    const uint8_t *rec[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) rec[j] = a.w + (size_t)min(blockIdx.x * NT + j, tiles - 1) * a.blocks * a.record;
+    f32x4 acc[NT][MT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0, 0, 0, 0};
+    auto load_x = [&](u32x4 (&v)[PIECES], uint32_t block) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i)       // (rows behind the last repeat it: not written)
+            v[i] = P::load((const E *)a.x + (uint64_t)min(m0 + i * STEP + piece_row, a.M - 1) * a.x_stride, block * W4_TK, piece_place, a.K);
+    };
+    auto store_x = [&](const u32x4 (&v)[PIECES]) {          // (LDS serves a wave's accesses in order: only the compiler has to be held)
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) P::store(xs, i * STEP + piece_row, piece_place, v[i]);
+        asm volatile("" ::: "memory");
+    };
+    auto fragment = [&](int s, int i) { return P::fragment(xs, i * 16 + (lane & 15), s, lane >> 4); };
+    u32x4 x[U][PIECES];
+    Block<X, GROUP, MT, NT> b[U];
+    uint32_t at = wave;
+    if constexpr (U > 1) {
+        for (; at + (U - 1) * waves < a.blocks; at += U * waves) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) { b[u].load_w(a, rec, (size_t)(at + u * waves) * a.record, lane); load_x(x[u], at + u * waves); }
+#pragma unroll
+            for (int u = 0; u < U; ++u) { store_x(x[u]); b[u].multiply(a, acc, fragment); }
+        }
+    }
+    if (at < a.blocks) { b[0].load_w(a, rec, (size_t)at * a.record, lane); load_x(x[0], at); }
+    for (; at < a.blocks; at += waves) {
+        store_x(x[0]);
+        const Block<X, GROUP, MT, NT> cur = b[0];
+        if (at + waves < a.blocks) { b[0].load_w(a, rec, (size_t)(at + waves) * a.record, lane); load_x(x[0], at + waves); }
+        cur.multiply(a, acc, fragment);
+    }
+    __syncthreads();
+    finish<X, MT, NT>(a, acc, reinterpret_cast<float *>(smem), wave, waves, threadIdx.x, blockDim.x, m0, blockIdx.x * NT, lane);
+}
+
+// More than 16 rows and many outputs: x's blocks are shared by WN waves of 2 x 16 outputs each; WK such sets of waves take every WK-th block. Blocks are
+// asked for two rounds ahead.
+template <int X, int GROUP, int MT, int WN, int WK>
+__global__ __launch_bounds__(512, 2) void w4_dense_shared_kernel(const W4Args a) {
+    using P = Piece<X>;
+    using E = typename P::E;
+    constexpr int NT = 2, ROWS = MT * 16, TILE = ROWS * P::ROW, NTH = WN * 64, N = ROWS * P::PLACES / NTH, STEP = NTH / P::PLACES;
+    static_assert(WN * WK == 8 && N >= 1, "");
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];           // [WK][2][TILE]; then the sums
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % WN, wk = wave / WN, t = wn * 64 + lane;
+    const uint32_t m0 = blockIdx.y * (MT * 16u), tiles = (a.N + W4_TN - 1) / W4_TN, tile0 = (blockIdx.x * WN + wn) * NT;
+    const int piece_row = t / P::PLACES, piece_place = t % P::PLACES;
+    const uint8_t *rec[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) rec[j] = a.w + (size_t)min(tile0 + j, tiles - 1) * a.blocks * a.record;
+    f32x4 acc[NT][MT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0, 0, 0, 0};
+    u32x4 x[2][N];
+    Block<X, GROUP, MT, NT> b[2];
+    auto load = [&](u32x4 (&v)[N], Block<X, GROUP, MT, NT> &w, uint32_t block) {
+        if (block >= a.blocks) return;
+        w.load_w(a, rec, (size_t)block * a.record, lane);
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = P::load((const E *)a.x + (uint64_t)min(m0 + i * STEP + piece_row, a.M - 1) * a.x_stride, block * W4_TK, piece_place, a.K);
+    };
+    unsigned char *mine = smem + wk * 2 * TILE;
+    auto round = [&](u32x4 (&v)[N], Block<X, GROUP, MT, NT> &w, unsigned char *xs, uint32_t block) {
+        if (block < a.blocks)
+#pragma unroll
+            for (int i = 0; i < N; ++i) P::store(xs, i * STEP + piece_row, piece_place, v[i]);
+        __syncthreads();
+        const Block<X, GROUP, MT, NT> cur = w;
+        load(v, w, block + 2 * WK);
+        if (block < a.blocks) cur.multiply(a, acc, [&](int s, int i) { return P::fragment(xs, i * 16 + (lane & 15), s, lane >> 4); });
+    };
+    load(x[0], b[0], wk);
+    load(x[1], b[1], wk + WK);
+    const uint32_t rounds = (a.blocks + WK - 1) / WK;
+    for (uint32_t r = 0; r < rounds; r += 2) {
+        round(x[0], b[0], mine, r * WK + wk);
+        if (r + 1 < rounds) round(x[1], b[1], mine + TILE, (r + 1) * WK + wk);
+    }
+    __syncthreads();
+    finish<X, MT, NT>(a, acc, reinterpret_cast<float *>(smem) + wn * WK * NT * MT * 256, wk, WK, wk * 64 + lane, WK * 64, m0, tile0, lane);
+}
+
+// Which kernel. Measured at 4096 inputs, group 128, bf16 (us; weights cold):
+//   rows that one piece a lane covers (4 in 16 bits): 4096 outputs 5.3, 14336 outputs 10.8 (all rows' pieces loaded: 9.1 and 29);  16 rows: 6.2 and 16
+//   64 rows:  outputs    4096   8192  14336  28672         32 rows:  4096   8192  14336  28672
+//     own pieces         13.1   15.5   29.3   53.5                    8.3   11.0   20.1   35.8
+//     shared by 2 waves  22.8   23.2   25.8   48.8                   16.5   16.7   19.4   36.1
+//     shared by 4 waves  36.8   37.0   41.2   42.4                   27.4   27.5   32.0   33.0
+// Sharing pays once there are workgroups for every CU all the same: 4 waves x 32 outputs at 7 x 16 outputs a CU, 2 waves at half of that.
 template <int X, int GROUP>
 static int launch_w4(const W4Args &a, uint32_t tiles, int cus, hipStream_t st) {
-    auto go = [&](auto kern, uint32_t mt, uint32_t nt, uint32_t most) -> int {
+    auto own = [&](auto kern, uint32_t mt) -> int {
         uint32_t waves = 1;
-        while (waves < most && waves * 2 <= a.blocks) waves *= 2;
-        const size_t lds = (size_t)waves * mt * nt * 1024;
+        while (waves < 8 && waves * 2 <= a.blocks) waves *= 2;
+        const size_t lds = (size_t)waves * mt * 16 * Piece<X>::ROW;          // (more than the sums)
         SHODH_TRY(ensure_dynamic_lds((const void *)kern, lds));
-        hipLaunchKernelGGL(kern, dim3((tiles + nt - 1) / nt, (a.M + 63) / 64), dim3(64 * waves), lds, st, a);
+        hipLaunchKernelGGL(kern, dim3(tiles, (a.M + 16 * mt - 1) / (16 * mt)), dim3(64 * waves), lds, st, a);
         SHODH_HIP_TRY(hipGetLastError());
         return SHODH_OK;
     };
-    const uint32_t wide = (uint32_t)cus;          // more outputs a wave once there are workgroups for every CU all the same
-    if (a.M <= 16) return go(w4_dense_kernel<X, GROUP, 1, 1, 4>, 1, 1, 8);
-    if (a.M <= 32) return tiles >= 2 * wide ? go(w4_dense_kernel<X, GROUP, 2, 2, 1>, 2, 2, 8) : go(w4_dense_kernel<X, GROUP, 2, 1, 2>, 2, 1, 8);
-    return tiles >= 2 * wide ? go(w4_dense_kernel<X, GROUP, 4, 2, 1>, 4, 2, 8) : go(w4_dense_kernel<X, GROUP, 4, 1, 1>, 4, 1, 8);
+    if (a.M <= 64 / Piece<X>::PLACES) return own(w4_dense_kernel<X, GROUP, 1, 1, 2, true>, 1);
+    if (a.M <= 16) return own(w4_dense_kernel<X, GROUP, 1, 1, X == W4_F32 ? 1 : 2, false>, 1);
+    if constexpr (X == W4_F32) return own(w4_dense_kernel<X, GROUP, 2, 1, 1, false>, 2);           // (three parts of each value: registers for no more)
+    else {
+        auto shared = [&](auto kern, uint32_t mt, uint32_t wn) -> int {
+            const size_t x = (size_t)(8 / wn) * 2 * mt * 16 * Piece<X>::ROW, sums = (size_t)8 * 2 * mt * 1024, lds = x > sums ? x : sums;
+            SHODH_TRY(ensure_dynamic_lds((const void *)kern, lds));
+            hipLaunchKernelGGL(kern, dim3((tiles + 2 * wn - 1) / (2 * wn), (a.M + 16 * mt - 1) / (16 * mt)), dim3(512), lds, st, a);
+            SHODH_HIP_TRY(hipGetLastError());
+            return SHODH_OK;
+        };
+        const bool four = 2 * tiles >= 14u * (uint32_t)cus, two = 2 * tiles >= 7u * (uint32_t)cus;
+        if (a.M <= 32) return four ? shared(w4_dense_shared_kernel<X, GROUP, 2, 4, 2>, 2, 4) : two ? shared(w4_dense_shared_kernel<X, GROUP, 2, 2, 4>, 2, 2)
+                                   : own(w4_dense_kernel<X, GROUP, 2, 1, 1, false>, 2);
+        if constexpr (GROUP > 32) {            // (four scales a record, two records, 64 rows: registers spill)
+            if (four) return shared(w4_dense_shared_kernel<X, GROUP, 4, 4, 2>, 4, 4);
+            if (two) return shared(w4_dense_shared_kernel<X, GROUP, 4, 2, 4>, 4, 2);
+        }
+        return own(w4_dense_kernel<X, GROUP, 4, 1, 1, false>, 4);
+    }
 }
 template <int X>
 static int pick_w4(const W4Args &a, const shodh_w4_weight *w, hipStream_t st) {
@@ -534,7 +654,7 @@ int shodh_w4_dense_device(const shodh_w4_weight *w, const void *d_x, uint32_t x_
     if ((x_dtype == SHODH_DTYPE_INT8) != (d_x_scale != nullptr)) { set_error("w4: int8 rows come with a scale each, others with none"); return SHODH_ERR_INVALID; }
     const uint64_t xs = x_stride ? x_stride : w->K, ys = y_stride ? y_stride : w->N;
     if (rows > 1 && ys < w->N) { set_error("w4: y's rows overlap (stride %llu below %u)", (unsigned long long)ys, w->N); return SHODH_ERR_DIM; }
-    if (rows > 64u * 65535u) { set_error("w4: %u rows: at most 4194240", rows); return SHODH_ERR_UNSUPPORTED; }
+    if (rows > 32u * 65535u) { set_error("w4: %u rows: at most 2097120", rows); return SHODH_ERR_UNSUPPORTED; }
     if (!aligned_to(d_x, dtype_bytes(x_dtype)) || !aligned_to(d_y, dtype_bytes(y_dtype)) || !aligned_to(d_x_scale, 4) || !aligned_to(d_bias, 4)) {
         set_error("w4: a pointer is not a multiple of its element's size"); return SHODH_ERR_INVALID;
     }
@@ -543,7 +663,8 @@ int shodh_w4_dense_device(const shodh_w4_weight *w, const void *d_x, uint32_t x_
     W4Args a;
     a.w = w->data; a.x = d_x; a.x_scale = d_x_scale; a.bias = d_bias; a.y = d_y; a.x_stride = xs; a.y_stride = ys;
     a.M = rows; a.N = w->N; a.K = w->K; a.blocks = w->blocks; a.record = w->record; a.y_dtype = y_dtype;
-    a.scale_f16 = w->scale_dtype == SHODH_DTYPE_FP16; a.zeros = w->zeros;
+    a.f16_mask = w->scale_dtype == SHODH_DTYPE_FP16 ? 0xFFFFFFFFu : 0u;
+    a.zero_at = w->zeros ? 1024 + (W4_TK / w->group) * 32 : 1024; a.zero_mask = w->zeros ? 0xFFFFFFFFu : 0u; a.zero_else = w->zeros ? 0u : 0x18181818u;
     hipStream_t st = (hipStream_t)stream;
     switch (x_dtype) {
         case SHODH_DTYPE_BF16: return pick_w4<W4_BF16>(a, w, st);
