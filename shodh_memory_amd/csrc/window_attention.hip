@@ -31,10 +31,10 @@ struct AttnArgs {
     const int32_t *cu;
     const int64_t *kv_start;
     const int32_t *kv_len;
-    float *part;               // split form: [splits][rows of out][DP] sums, then [splits][rows][2] maxima and sums
+    float *part;               // split form: [splits][rows of out][DP] sums, [splits][rows][2] maxima and sums, [rows] numbers of parts (0: the row is done)
     uint64_t q_stride, q_head, k_stride, k_head, v_stride, v_head, o_stride, o_head;
     int64_t q_tokens, kv_tokens;
-    uint32_t heads, kv_heads, group, dim, seqs, slots, splits, sinks;
+    uint32_t heads, kv_heads, group, dim, seqs, slots, splits, chunk /* blocks of 32 keys of a part */, sinks;
     int32_t left, right;       // negative: no bound
     float scale2;              // |scale| * log2(e)
     uint32_t sign;             // 0, or the sign bits of two 16-bit numbers
@@ -117,7 +117,7 @@ struct Seq {
     int64_t q0, k0;
     int nq, nk;
 };
-__device__ __forceinline__ Seq seq_of(const AttnArgs &a, int b) {
+__device__ __forceinline__ Seq seq_at(const AttnArgs &a, int b) {
     Seq s;
     int64_t t0 = a.cu[b], t1 = a.cu[b + 1];
     if (t0 < 0 || t1 < t0 || t1 > a.q_tokens) t0 = t1 = 0;            // no such rows: nothing is done for them
@@ -126,6 +126,10 @@ __device__ __forceinline__ Seq seq_of(const AttnArgs &a, int b) {
         s.k0 = a.kv_start[b]; s.nk = a.kv_len[b];
         if (s.k0 < 0 || s.nk < 0 || s.k0 > a.kv_tokens || s.nk > a.kv_tokens - s.k0) { s.k0 = 0; s.nk = 0; }      // no such keys: none is seen
     } else { s.k0 = t0; s.nk = s.nq; }
+    return s;
+}
+__device__ __forceinline__ Seq seq_of(const AttnArgs &a, int b) {           // b alike in all lanes
+    Seq s = seq_at(a, b);
     s.q0 = uniform64(s.q0); s.k0 = uniform64(s.k0);
     s.nq = __builtin_amdgcn_readfirstlane(s.nq); s.nk = __builtin_amdgcn_readfirstlane(s.nk);
     return s;
@@ -135,6 +139,7 @@ __device__ __forceinline__ Seq seq_of(const AttnArgs &a, int b) {
 template <class T, int DP>
 struct Rows {
     using V8 = typename Vec8<T>::V;
+    int lane;                  // (kept apart from threadIdx: what is formed from it is not kept in registers around a loop over items)
     V8 q[DP / 16];
     f32x16 o[DP / 32];
     float m, l;                // reference maximum (powers of two) and this half's part of the sum
@@ -144,7 +149,9 @@ struct Rows {
     uint32_t at_k[DP / 16], at_v[DP / 32];      // LDS offsets of the lane's fragments in a block
 
     __device__ __forceinline__ void init(const AttnArgs &a, const Seq &s, uint32_t kvh, int64_t row) {
-        const int lane = threadIdx.x & 63, half = lane >> 5;
+        lane = threadIdx.x & 63;
+        asm volatile("" : "+v"(lane));
+        const int half = lane >> 5;
         const int64_t r = row + (lane & 31);
         live = r < (int64_t)s.nq * a.group;
         token = live ? (uint32_t)(r / a.group) : 0;
@@ -193,7 +200,7 @@ struct Rows {
         for (int i = 0; i < DP / 16; ++i)
 #pragma unroll
             for (int b = 0; b < NB; ++b) k[b][i] = *reinterpret_cast<const V8 *>(Ks + at_k[i] + b * (32 * DP * 2));
-        __builtin_amdgcn_sched_barrier(0);          // (all of them on their way before the first is waited for)
+        if constexpr (NB > 1) __builtin_amdgcn_sched_barrier(0);          // (all of them on their way before the first is waited for)
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -203,10 +210,18 @@ struct Rows {
 #pragma unroll
             for (int b = 0; b < NB; ++b) s[b] = mma32(k[b][i], q[i], s[b]);
     }
+    // The same for one block, with the queries' fragments in LDS: [DP / 16][64 lanes] x 16 bytes at Qs.
+    __device__ __forceinline__ void scores_lds(const unsigned char *Ks, const unsigned char *Qs, f32x16 &s) const {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i)
+            s = mma32(*reinterpret_cast<const V8 *>(Ks + at_k[i]), *reinterpret_cast<const V8 *>(Qs + i * 1024 + lane * 16), s);
+    }
     // Scores to probabilities. Keys from `limit` on belong to no one here; masked: some row does not see some key of these.
     template <int NB>
     __device__ __forceinline__ void softmax(const AttnArgs &a, f32x16 (&s)[NB], V8 (&p)[NB][2], int key, int limit, bool masked) {
-        const int half = (threadIdx.x & 63) >> 5, end = min(hi, limit);
+        const int half = lane >> 5, end = min(hi, limit);
         if (masked) {
 #pragma unroll
             for (int b = 0; b < NB; ++b)
@@ -279,42 +294,46 @@ struct Rows {
     // Values that are no numbers were taken out of the tiles that some row sees in part (clear_values): here they go into the rows that do see them, as
     // what they make of any sum. (A row that took one in already is what it is.)
     __device__ __forceinline__ void spoil(const AttnArgs &a, const T *vb, int j0, int j1, int limit) {
-        const int lane = threadIdx.x & 63, half = lane >> 5, end = min(hi, limit);
+        const int half = lane >> 5, end = min(hi, limit);
         for (int j = j0; j < j1; ++j) {
             const T *v = vb + (uint64_t)j * a.v_stride;
             bool bad = false;
             for (uint32_t d = lane; d < a.dim; d += 64) bad |= !(__builtin_fabsf((float)v[d]) < __builtin_inff());
             if (!__any(bad)) continue;
             const bool sees = j < end && (j >= lo || j < (int)a.sinks);
+            const T *mine = v + half * 4;
 #pragma unroll
             for (int t = 0; t < DP / 32; ++t)
 #pragma unroll
-                for (int x = 0; x < 16; ++x) {
-                    const uint32_t d = t * 32 + (x & 3) + 8 * (x >> 2) + 4 * half;
-                    const float f = d < a.dim ? (float)v[d] : 0.0f;
-                    if (sees && !(__builtin_fabsf(f) < __builtin_inff())) o[t][x] += f;
-                    asm volatile("" ::: "memory");       // (one at a time: registers for this would be taken from the loop before)
+                for (int g = 0; g < 4; ++g) {
+                    if ((uint32_t)(t * 32 + g * 8) >= a.dim) continue;
+                    T e[4];
+                    load_any(e, mine + t * 32 + g * 8);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const float f = (float)e[x];
+                        o[t][4 * g + x] += sees && !(__builtin_fabsf(f) < __builtin_inff()) ? f : 0.0f;
+                    }
+                    asm volatile("" ::: "memory");       // (four at a time: registers for this would be taken from the loop before)
                 }
         }
     }
 
-    __device__ __forceinline__ void store(const AttnArgs &a, const Seq &s, float total) {
-        const int half = (threadIdx.x & 63) >> 5;
-        if (!live) return;
+    // 32 features (of tile t), and what goes with a row
+    __device__ __forceinline__ void store(const AttnArgs &a, const Seq &s, const f32x16 &v, int t, float total) const {
         const float inv = total > 0.0f || total != total ? 1.0f / total : 0.0f;
         T *dst = (T *)a.out + (uint64_t)(s.q0 + token) * a.o_stride + (uint64_t)head * a.o_head;
 #pragma unroll
-        for (int t = 0; t < DP / 32; ++t)
+        for (int g = 0; g < 4; ++g) {
+            const uint32_t d = t * 32 + g * 8 + (lane >> 5) * 4;
+            T e[4];
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const uint32_t d = t * 32 + g * 8 + half * 4;
-                T e[4];
-#pragma unroll
-                for (int x = 0; x < 4; ++x) e[x] = (T)(total == 0.0f ? 0.0f : o[t][4 * g + x] * inv);
-                if (d < a.dim) store_any(dst + d, e);
-            }
-        if (a.lse && half == 0)
-            a.lse[(uint64_t)(s.q0 + token) * a.heads + head] = total == 0.0f ? NEG_INF : (m + __builtin_amdgcn_logf(total)) * 0.69314718055994530942f;
+            for (int x = 0; x < 4; ++x) e[x] = (T)(total == 0.0f ? 0.0f : v[4 * g + x] * inv);
+            if (d < a.dim) store_any(dst + d, e);
+        }
+    }
+    __device__ __forceinline__ void store_lse(const AttnArgs &a, const Seq &s, float total) const {
+        if (a.lse) a.lse[(uint64_t)(s.q0 + token) * a.heads + head] = total == 0.0f ? NEG_INF : (m + __builtin_amdgcn_logf(total)) * 0.69314718055994530942f;
     }
 };
 
@@ -378,6 +397,22 @@ __device__ __forceinline__ void glds16_n(const void *base, const uint32_t (&off)
                      "s_add_u32 m0, m0, %7\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %5\n\ts_add_u32 m0, m0, %7\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %4, %5\n\ts_mov_b32 m0, %0"
                      : "=&s"(keep) : "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base), "s"(lds), "s"(step) : "memory", "scc");
     }
+}
+// the same with one lane offset and a base that moves on by `rows` bytes
+template <int N>
+__device__ __forceinline__ void glds16_rows(const void *base, uint32_t off, uint32_t rows, uint32_t lds) {
+    unsigned keep;
+    uint64_t b = (uint64_t)base;
+    if constexpr (N == 1)
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %1\n\ts_mov_b32 m0, %0" : "=&s"(keep), "+s"(b) : "v"(off), "s"(lds) : "memory");
+    else
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            uint64_t b2 = b + rows;
+            asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %4\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %1\n\ts_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %2\n\ts_mov_b32 m0, %0"
+                         : "=&s"(keep) : "s"(b), "s"(b2), "v"(off), "s"(lds + i * 1024) : "memory", "scc");
+            b = b2 + rows;
+        }
 }
 __device__ __forceinline__ uint32_t lds_address(const void *p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) unsigned char *)p; }
 template <int DP> struct KPlace { __device__ __forceinline__ int operator()(int row, int c) const { return k_place<DP>(row, c); } };
@@ -469,7 +504,11 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs a) {
         }
     }
     if (spoiled) { rows.spoil(a, vb, 0, g.first, g.first); rows.spoil(a, vb, g.begin, g.end, g.end); }
-    rows.store(a, s, half_sum(rows.l));
+    const float total = half_sum(rows.l);
+    if (!rows.live) return;
+#pragma unroll
+    for (int t2 = 0; t2 < DP / 32; ++t2) rows.store(a, s, rows.o[t2], t2, total);
+    if (rows.lane < 32) rows.store_lse(a, s, total);
 }
 
 // ---- split: 32 rows, every wave its own blocks of 32 keys, every workgroup its own part of them ------------------------------------------------
@@ -477,17 +516,63 @@ template <class T, int DP, bool DMA>
 __global__ __launch_bounds__(256, 2) void attn_split_kernel(const AttnArgs a) {
     constexpr int BM = 32, KT = 32, TILE = KT * DP * 2;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];      // [4 waves][K | V]; then the waves' sums
-    const uint32_t kvh = blockIdx.y, slot = blockIdx.x, split = blockIdx.z;
-    const int b = __builtin_amdgcn_readfirstlane(find_seq(a, slot, BM));
-    const Seq s = seq_of(a, b);
-    const int64_t row0 = ((int64_t)slot - (s.q0 * a.group / BM + b)) * BM;
-    if (row0 < 0 || row0 >= (int64_t)s.nq * a.group) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    // Items of work: (sequence, tile of its rows, part of its keys) x key head, counted off over the sequences, 64 of them at a time in a table: a
+    // workgroup takes every gridDim.x-th of them, so that short sequences cost what they are.
+    struct Table {
+        int64_t q0[64], k0[64];
+        int nq[64], nk[64], parts[64], begin[64], end[64];       // items of sequences base .. : [begin, end)
+    };
+    Table &table = *reinterpret_cast<Table *>(smem + 8 * TILE + 1024);
+    auto count = [&](int base) {          // by wave 0; the items of 64 sequences
+        const int b = base + lane;
+        int64_t q0 = 0, k0 = 0;
+        int nq = 0, nk = 0, parts = 1;
+        if (b < (int)a.seqs) {
+            const Seq s = seq_at(a, b);
+            q0 = s.q0; k0 = s.k0; nq = s.nq; nk = s.nk;
+            int64_t seen = nk;
+            if (a.left >= 0 && a.right >= 0) seen = min(seen, (int64_t)a.left + a.right + 1 + BM + 64 + (int64_t)a.sinks);
+            parts = (int)min((int64_t)a.splits, max((int64_t)1, ((seen + 31) / 32 + a.chunk - 1) / a.chunk));
+        }
+        const int items = (int)(((int64_t)nq * a.group + BM - 1) / BM) * parts;
+        int end = items;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) { const int v = __shfl_up(end, o); if (lane >= o) end += v; }
+        table.q0[lane] = q0; table.k0[lane] = k0; table.nq[lane] = nq; table.nk[lane] = nk; table.parts[lane] = parts;
+        table.begin[lane] = end - items; table.end[lane] = end;
+    };
+    int base = 0;
+    uint32_t before = 0;                 // items of the sequences before base
+    if (wave == 0) count(0);
+    __syncthreads();
+    for (uint32_t id = blockIdx.x;; id += gridDim.x) {
+    // (heads in turn, shifted from item to item: an XCD, which takes every eighth workgroup, sees all of them)
+    const uint32_t item = id / a.kv_heads, kvh = (id + (item >> 1)) % a.kv_heads;
+    while (item - before >= (uint32_t)table.end[63]) {
+        before += (uint32_t)table.end[63];
+        base += 64;
+        if (base >= (int)a.seqs) return;
+        __syncthreads();
+        if (wave == 0) count(base);
+        __syncthreads();
+    }
+    const int at_lane = __ffsll((unsigned long long)__ballot((uint32_t)table.end[lane] > item - before)) - 1;
+    const int within = __builtin_amdgcn_readfirstlane((int)(item - before) - table.begin[at_lane]), parts = __builtin_amdgcn_readfirstlane(table.parts[at_lane]), split = within % parts;
+    Seq s;
+    s.q0 = uniform64(table.q0[at_lane]); s.k0 = uniform64(table.k0[at_lane]);
+    s.nq = __builtin_amdgcn_readfirstlane(table.nq[at_lane]); s.nk = __builtin_amdgcn_readfirstlane(table.nk[at_lane]);
+    const int64_t row0 = (int64_t)(within / parts) * BM;
     Rows<T, DP> rows;
     rows.init(a, s, kvh, row0);
+    unsigned char *Qs = smem + 8 * TILE + 1024 + 64 * 36;          // the queries' fragments, the same for all four waves (registers for them would spill)
+    if (wave == 0)
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) *reinterpret_cast<typename Rows<T, DP>::V8 *>(Qs + i * 1024 + rows.lane * 16) = rows.q[i];
+    __syncthreads();
     const Range g = range_of(a, s, row0, row0 + BM);
     const int n_first = (g.first + KT - 1) / KT, n = n_first + (g.end - g.begin + KT - 1) / KT;
-    const int i0 = (int)((int64_t)n * split / a.splits), i1 = (int)((int64_t)n * (split + 1) / a.splits);
+    const int i0 = (int)((int64_t)n * split / parts), i1 = (int)((int64_t)n * (split + 1) / parts);
     int lo_max = rows.live ? rows.lo : 0, hi_min = rows.live ? rows.hi : 0x7FFFFFFF;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) { lo_max = max(lo_max, __shfl_xor(lo_max, o)); hi_min = min(hi_min, __shfl_xor(hi_min, o)); }
@@ -496,21 +581,41 @@ __global__ __launch_bounds__(256, 2) void attn_split_kernel(const AttnArgs a) {
     unsigned char *Ks = smem + wave * 2 * TILE, *Vs = Ks + TILE;
     auto start_of = [&](int i) { return i < n_first ? i * KT : g.begin + (i - n_first) * KT; };
     auto limit_of = [&](int i) { return i < n_first ? g.first : g.end; };
+    // Whole blocks: DP / 16 transfers of 512 / DP rows each. K's exchange of places repeats after DP / 32 of them, V's is the same in all: so many lane
+    // offsets, and bases that move on by rows.
+    constexpr int RPT = 512 / DP, VAR = DP / 32;
+    uint32_t off_k[VAR], off_v;
+    {
+        const int x = rows.lane % (DP / 8), r = rows.lane / (DP / 8);
+#pragma unroll
+        for (int i = 0; i < VAR; ++i) off_k[i] = ((uint32_t)(i * RPT + r) * (uint32_t)a.k_stride + k_place<DP>(i * RPT + r, x) * 8) * 2;
+        off_v = ((uint32_t)r * (uint32_t)a.v_stride + v_place<DP>(r, x) * 8) * 2;
+    }
+    const uint32_t lds_k = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds_address(Ks)), lds_v = lds_k + TILE;
+    const bool whole = a.dim == DP;
     auto fetch_k = [&](int i) {
-        const int j = start_of(i);
-        stage<T, DP, KT, 64, DMA>(Ks, kb + (uint64_t)j * a.k_stride, a.k_stride, min(KT, limit_of(i) - j) - 1, a.dim, lane, KPlace<DP>());
+        const int j = start_of(i), last = min(KT, limit_of(i) - j) - 1;
+        const T *p = kb + (uint64_t)j * a.k_stride;
+        if (DMA && whole && last == KT - 1) {
+            glds16_n(uniform_ptr((const unsigned char *)p), off_k, lds_k, 1024);
+            glds16_n(uniform_ptr((const unsigned char *)(p + (uint64_t)(VAR * RPT) * a.k_stride)), off_k, lds_k + VAR * 1024, 1024);
+        } else stage<T, DP, KT, 64, DMA>(Ks, p, a.k_stride, last, a.dim, rows.lane, KPlace<DP>());
     };
     auto fetch_v = [&](int i) {
-        const int j = start_of(i);
-        stage<T, DP, KT, 64, DMA>(Vs, vb + (uint64_t)j * a.v_stride, a.v_stride, min(KT, limit_of(i) - j) - 1, a.dim, lane, VPlace<DP>());
+        const int j = start_of(i), last = min(KT, limit_of(i) - j) - 1;
+        const T *p = vb + (uint64_t)j * a.v_stride;
+        if (DMA && whole && last == KT - 1) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+                glds16_rows<VAR>(uniform_ptr((const unsigned char *)(p + (uint64_t)(u * VAR * RPT) * a.v_stride)), off_v, (uint32_t)a.v_stride * (RPT * 2), lds_v + u * VAR * 1024);
+        } else stage<T, DP, KT, 64, DMA>(Vs, p, a.v_stride, last, a.dim, rows.lane, VPlace<DP>());
     };
     if (DMA && a.dim < DP) {
-        for (int e = lane; e < 2 * TILE / 16; e += 64) *reinterpret_cast<u32x4 *>(Ks + e * 16) = u32x4{0, 0, 0, 0};
+        for (int e = rows.lane; e < 2 * TILE / 16; e += 64) *reinterpret_cast<u32x4 *>(Ks + e * 16) = u32x4{0, 0, 0, 0};
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
     // K's next block is fetched while this one's values are multiplied, V's next while the next scores are: each wait leaves the other's loads (one
     // per 64 lanes x 16 bytes: DP / 16 of them) in flight. (With a head smaller than DP some are left out: there all are waited for.)
-    const bool whole = a.dim == DP;
     auto arrived = [&](bool all) {
         if (DMA && whole && !all) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(DP / 16) : "memory");
         else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -524,12 +629,12 @@ __global__ __launch_bounds__(256, 2) void attn_split_kernel(const AttnArgs a) {
         f32x16 sc[1];
         typename Rows<T, DP>::V8 p[1][2];
         arrived(false);                       // K
-        rows.scores(Ks, sc);
+        rows.scores_lds(Ks, Qs, sc[0]);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         if (more) fetch_k(i + 4);
         rows.softmax(a, sc, p, j, limit, masked);
         arrived(!more);                       // V
-        if (masked) spoiled |= __any(clear_values<T, 64>(Vs, TILE, lane));
+        if (masked) spoiled |= __any(clear_values<T, 64>(Vs, TILE, rows.lane));
         rows.values(Vs, p);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         if (more) fetch_v(i + 4);
@@ -539,50 +644,53 @@ __global__ __launch_bounds__(256, 2) void attn_split_kernel(const AttnArgs a) {
     // the four waves' parts, in their order: statistics first, then the sums, 32 features at a time
     float *stat = reinterpret_cast<float *>(smem + 8 * TILE);       // [4][32][2]
     const float part = half_sum(rows.l);
-    if (lane < 32) { stat[(wave * 32 + lane) * 2] = rows.m; stat[(wave * 32 + lane) * 2 + 1] = part; }
+    if (rows.lane < 32) { stat[(wave * 32 + rows.lane) * 2] = rows.m; stat[(wave * 32 + rows.lane) * 2 + 1] = part; }
     __syncthreads();
     float top = NEG_INF, total = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) top = fmaxf(top, stat[(w * 32 + (lane & 31)) * 2]);
+    for (int w = 0; w < 4; ++w) top = fmaxf(top, stat[(w * 32 + (rows.lane & 31)) * 2]);
     const float base = top == NEG_INF ? 0.0f : top;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) total += stat[(w * 32 + (lane & 31)) * 2 + 1] * __builtin_amdgcn_exp2f(stat[(w * 32 + (lane & 31)) * 2] - base);
+    for (int w = 0; w < 4; ++w) total += stat[(w * 32 + (rows.lane & 31)) * 2 + 1] * __builtin_amdgcn_exp2f(stat[(w * 32 + (rows.lane & 31)) * 2] - base);
     const float mine = __builtin_amdgcn_exp2f(rows.m - base);
-    float *sums = reinterpret_cast<float *>(smem);                  // [4 waves][16][64]
+    // (every wave's tiles are done with at the barrier above: their place takes the sums, 32 features of which each wave adds up)
+    float *sums = reinterpret_cast<float *>(smem);                  // [4 waves][DP / 32][16][64]
 #pragma unroll
-    for (int t = 0; t < DP / 32; ++t) {
-        __syncthreads();
+    for (int t = 0; t < DP / 32; ++t)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) sums[(wave * 16 + r) * 64 + lane] = rows.o[t][r] * mine;
-        __syncthreads();
+        for (int r = 0; r < 16; ++r) sums[((wave * (DP / 32) + t) * 16 + r) * 64 + rows.lane] = rows.o[t][r] * mine;
+    __syncthreads();
+    const uint64_t all = (uint64_t)a.q_tokens * a.heads, at = (uint64_t)(s.q0 + rows.token) * a.heads + rows.head;
+    float *stats = a.part + (uint64_t)a.splits * all * DP;
+    rows.m = top;
+    if (wave == 0 && rows.live && rows.lane < 32) {
+        if (a.splits > 1 && split == 0) reinterpret_cast<uint32_t *>(stats + (uint64_t)a.splits * all * 2)[at] = parts == 1 ? 0 : parts;
+        if (parts > 1) { stats[(split * all + at) * 2] = top; stats[(split * all + at) * 2 + 1] = total; }
+        else rows.store_lse(a, s, total);
+    }
+    if (wave < DP / 32 && rows.live) {
+        f32x16 o;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             float v = 0.0f;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) v += sums[(w * 16 + r) * 64 + lane];
-            rows.o[t][r] = v;
+            for (int w = 0; w < 4; ++w) v += sums[((w * (DP / 32) + wave) * 16 + r) * 64 + rows.lane];
+            o[r] = v;
         }
-    }
-    rows.m = top;
-    if (a.splits == 1) {
-        if (wave == 0) rows.store(a, s, total);
-        return;
-    }
-    if (!rows.live || wave >= DP / 32) return;
-    const uint64_t all = (uint64_t)a.q_tokens * a.heads, at = (uint64_t)(s.q0 + rows.token) * a.heads + rows.head;
-    float *stats = a.part + (uint64_t)a.splits * all * DP;
-    if (wave == 0 && lane < 32) { stats[(split * all + at) * 2] = top; stats[(split * all + at) * 2 + 1] = total; }
-    float *dst = a.part + (split * all + at) * DP;
-#pragma unroll
-    for (int t = 0; t < DP / 32; ++t)
-        if (t == wave)
+        if (parts == 1) rows.store(a, s, o, wave, total);
+        else {
+            float *dst = a.part + (split * all + at) * DP + wave * 32 + (rows.lane >> 5) * 4;
 #pragma unroll
             for (int gq = 0; gq < 4; ++gq) {
                 f32x4 e;
 #pragma unroll
-                for (int x = 0; x < 4; ++x) e[x] = rows.o[t][4 * gq + x];
-                *reinterpret_cast<f32x4 *>(dst + t * 32 + gq * 8 + (lane >> 5) * 4) = e;
+                for (int x = 0; x < 4; ++x) e[x] = o[4 * gq + x];
+                *reinterpret_cast<f32x4 *>(dst + gq * 8) = e;
             }
+        }
+    }
+    __syncthreads();                     // the sums' place is the next item's tiles'
+    }
 }
 
 // the parts of a row, in their order: one wave a row
@@ -593,8 +701,10 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
     int64_t last = a.cu[a.seqs];
     if (at >= all || (int64_t)(at / a.heads) < (int64_t)a.cu[0] || (int64_t)(at / a.heads) >= last) return;       // rows behind the last sequence stay as they were
     const float *stats = a.part + (uint64_t)a.splits * all * DP;
+    const uint32_t parts = reinterpret_cast<const uint32_t *>(stats + (uint64_t)a.splits * all * 2)[at];
+    if (parts == 0 || parts > a.splits) return;
     float m = NEG_INF, l = 0.0f;
-    if ((uint32_t)lane < a.splits) { m = stats[(lane * all + at) * 2]; l = stats[(lane * all + at) * 2 + 1]; }
+    if ((uint32_t)lane < parts) { m = stats[(lane * all + at) * 2]; l = stats[(lane * all + at) * 2 + 1]; }
     float top = m;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
@@ -605,11 +715,18 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
     constexpr int PER = DP >= 64 ? DP / 64 : 1;
     float v[PER] = {};
     const int d = lane * PER;
-    for (uint32_t i = 0; i < a.splits; ++i) {
-        const float c = __shfl(w, (int)i);
-        if (d < DP)
+    for (uint32_t i = 0; i < parts; i += 8) {          // eight parts' loads on their way at once; those behind the last repeat it with weight 0
+        float r[8][PER];
 #pragma unroll
-            for (int x = 0; x < PER; ++x) v[x] += c * a.part[(i * all + at) * DP + d + x];
+        for (int u = 0; u < 8; ++u)
+#pragma unroll
+            for (int x = 0; x < PER; ++x) r[u][x] = a.part[(min(i + u, parts - 1) * all + at) * DP + (d < DP ? d : 0) + x];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const float c = __shfl(w, (int)min(i + u, 63u));
+#pragma unroll
+            for (int x = 0; x < PER; ++x) v[x] += i + u < parts ? c * r[u][x] : 0.0f;
+        }
     }
     T *dst = (T *)a.out + (at / a.heads) * a.o_stride + (at % a.heads) * a.o_head;
 #pragma unroll
@@ -622,7 +739,7 @@ static int padded_dim(uint32_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 
 struct AttnPlan {
     bool split;
-    uint32_t slots, splits;
+    uint32_t slots, splits, chunk, grid;
     uint64_t workspace;
 };
 // Which form, and into how many parts the keys are cut.
@@ -632,7 +749,7 @@ static AttnPlan plan_attention(const shodh_attention_cfg *c, int cus) {
     const uint64_t tiles = (rows / 128 + c->seqs) * c->kv_heads;
     p.split = rows <= 32ull * c->seqs || tiles < (uint64_t)cus;
     p.slots = (uint32_t)(rows / (p.split ? 32 : 128) + c->seqs);
-    p.splits = 1;
+    p.splits = p.chunk = p.grid = 1;
     p.workspace = 0;
     if (p.split) {
         uint64_t seen = c->kv_tokens;
@@ -640,10 +757,17 @@ static AttnPlan plan_attention(const shodh_attention_cfg *c, int cus) {
             const uint64_t w = (uint64_t)c->left + (uint64_t)c->right + 1 + c->sinks + 32;
             if (w < seen) seen = w;
         }
-        const uint64_t groups = (uint64_t)p.slots * c->kv_heads, want = ceil_div(4ull * cus, groups ? groups : 1), most = ceil_div(seen, 256);
-        uint64_t n = want < most ? want : most;
-        p.splits = (uint32_t)(n < 1 ? 1 : n > 64 ? 64 : n);
-        if (p.splits > 1) p.workspace = p.splits * c->q_tokens * c->heads * (uint64_t)(padded_dim(c->head_dim) + 2) * 4;
+        // A part is 256 KiB of K and V (a workgroup's share of the bandwidth for some 25 us), less where that leaves CUs without work, 128 keys at least.
+        const uint64_t groups = (uint64_t)p.slots * c->kv_heads, blocks = ceil_div(seen ? seen : 1, 32), dp = padded_dim(c->head_dim);
+        uint64_t chunk = blocks * groups / (4ull * cus);
+        const uint64_t most = 2048 / dp;
+        chunk = chunk < 4 ? 4 : chunk > most ? most : chunk;
+        const uint64_t n = ceil_div(blocks, chunk);
+        p.splits = (uint32_t)(n > 64 ? 64 : n);
+        p.chunk = (uint32_t)chunk;
+        const uint64_t items = groups * p.splits, resident = (uint64_t)cus * (dp == 128 ? 2 : 4);
+        p.grid = (uint32_t)(items < resident ? items : resident);
+        if (p.splits > 1) p.workspace = (p.splits * (uint64_t)(dp + 2) + 1) * c->q_tokens * c->heads * 4;
     }
     return p;
 }
@@ -668,9 +792,9 @@ static int launch_attention(const AttnArgs &a, const AttnPlan &p, hipStream_t st
         SHODH_HIP_TRY(hipGetLastError());
         return SHODH_OK;
     }
-    constexpr size_t tiles = 8 * 32 * DP * 2, lds = (tiles < 16384 ? 16384 : tiles) + 1024;
+    constexpr size_t lds = 8 * 32 * DP * 2 + 1024 + 64 * 36 + DP * 64;          // tiles or sums, statistics, the table of sequences, queries
     SHODH_TRY(ensure_dynamic_lds((const void *)attn_split_kernel<T, DP, DMA>, lds));
-    hipLaunchKernelGGL((attn_split_kernel<T, DP, DMA>), dim3(p.slots, a.kv_heads, p.splits), dim3(256), lds, st, a);
+    hipLaunchKernelGGL((attn_split_kernel<T, DP, DMA>), dim3(p.grid), dim3(256), lds, st, a);
     SHODH_HIP_TRY(hipGetLastError());
     if (p.splits > 1) {
         hipLaunchKernelGGL((attn_join_kernel<T, DP>), dim3((uint32_t)ceil_div((uint64_t)a.q_tokens * a.heads, 4)), dim3(256), 0, st, a);
@@ -742,7 +866,7 @@ int shodh_window_attention_device(int device, const shodh_attention_cfg *cfg, co
     a.q = d_q; a.k = d_k; a.v = d_v; a.out = d_out; a.lse = d_lse; a.cu = d_cu; a.kv_start = d_kv_start; a.kv_len = d_kv_len; a.part = (float *)d_workspace;
     a.q_tokens = (int64_t)cfg->q_tokens; a.kv_tokens = (int64_t)cfg->kv_tokens;
     a.heads = cfg->heads; a.kv_heads = cfg->kv_heads; a.group = cfg->heads / cfg->kv_heads; a.dim = cfg->head_dim; a.seqs = cfg->seqs;
-    a.slots = p.slots; a.splits = p.splits; a.sinks = cfg->sinks; a.left = cfg->left; a.right = cfg->right;
+    a.slots = p.slots; a.splits = p.splits; a.chunk = p.chunk; a.sinks = cfg->sinks; a.left = cfg->left; a.right = cfg->right;
     const float scale = cfg->scale == 0.0f ? 1.0f / __builtin_sqrtf((float)d) : cfg->scale;
     a.scale2 = __builtin_fabsf(scale) * 1.44269504088896340736f;
     a.sign = scale < 0.0f ? 0x80008000u : 0u;
