@@ -38,6 +38,8 @@ struct AttnArgs {
     int32_t left, right;       // negative: no bound
     float scale2;              // |scale| * log2(e)
     uint32_t sign;             // 0, or the sign bits of two 16-bit numbers
+    int shift;                 // log2(group), or -1
+    __device__ __forceinline__ uint32_t over_group(uint32_t x) const { return shift >= 0 ? x >> shift : x / group; }
 };
 
 constexpr float NEG_INF = -__builtin_inff();
@@ -57,22 +59,22 @@ template <> struct Vec8<_Float16> { using V = f16x8; using V2 = f16x2; static co
 __device__ __forceinline__ f32x16 mma32(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16 mma32(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
+// Does a wave find a value that is no number in `bytes` of V in LDS?
 template <class T>
-__device__ __forceinline__ bool any_nonfinite(u32x4 w) {     // an exponent of all ones in any of 8 values (a carry into the sign's place)
+__device__ __forceinline__ bool find_values(const unsigned char *Vs, int bytes, int lane) {
     uint32_t m = 0;
+    for (int e = lane * 16; e < bytes; e += 1024) {
+        const u32x4 w = *reinterpret_cast<const u32x4 *>(Vs + e);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) m |= (w[i] & Vec8<T>::EXP) + Vec8<T>::ONE;
-    return (m & 0x80008000u) != 0;
+        for (int i = 0; i < 4; ++i) m |= (w[i] & Vec8<T>::EXP) + Vec8<T>::ONE;          // an exponent of all ones carries into the sign's place
+    }
+    return __any((m & 0x80008000u) != 0);
 }
-
-// Takes the values that are no numbers out of `bytes` of V in LDS, by NT threads; true for a thread that found one.
+// Takes them out, by NT threads.
 template <class T, int NT>
-__device__ __forceinline__ bool clear_values(unsigned char *Vs, int bytes, int t) {
-    bool found = false;
+__device__ __forceinline__ void clear_values(unsigned char *Vs, int bytes, int t) {
     for (int e = t * 16; e < bytes; e += NT * 16) {
         u32x4 w = *reinterpret_cast<const u32x4 *>(Vs + e);
-        if (!any_nonfinite<T>(w)) continue;
-        found = true;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const uint32_t bad = ((w[i] & Vec8<T>::EXP) + Vec8<T>::ONE) & 0x80008000u;
@@ -80,7 +82,6 @@ __device__ __forceinline__ bool clear_values(unsigned char *Vs, int bytes, int t
         }
         *reinterpret_cast<u32x4 *>(Vs + e) = w;
     }
-    return found;
 }
 
 // 16-byte places of a row of DP values, exchanged so that neither 16 rows' same place (a fragment of K) nor 4 rows' same four places (of V, read across)
@@ -90,23 +91,36 @@ template <int DP> __device__ __forceinline__ int v_place(int row, int c) { retur
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-// Sequence of a tile slot: the largest b with cu[b] * group / BM + b <= slot (those starts rise strictly). 64 probes at a time.
-__device__ __forceinline__ int find_seq(const AttnArgs &a, int64_t slot, int bm) {
-    const int lane = threadIdx.x & 63;
-    int lo = 0, n = (int)a.seqs;            // the answer is in [lo, lo + n)
+// Sequence of a tile slot: the largest b with cu[b] * group / BM + b <= slot (those starts rise strictly), and its tokens [t0, t1).
+__device__ __forceinline__ int find_seq(const AttnArgs &a, int64_t slot, int bm, int &t0, int &t1) {
+    const int lane = threadIdx.x & 63, seqs = (int)a.seqs;
+    auto starts_by = [&](int b, int c) { return ((int64_t)(c < 0 ? 0 : min((int64_t)c, a.q_tokens)) * a.group) / bm + b <= slot; };
+    if (seqs < 256) {                       // all of cu at once
+        int c[4], got = 0;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) c[u] = u * 64 <= seqs ? a.cu[min(u * 64 + lane, seqs)] : 0;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) got += __popcll(__ballot(u * 64 + lane < seqs && starts_by(u * 64 + lane, c[u])));
+        const int b = max(got, 1) - 1;
+        t0 = t1 = 0;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int x = __builtin_amdgcn_readlane(c[u], b & 63), y = __builtin_amdgcn_readlane(c[u], (b + 1) & 63);
+            t0 = (b >> 6) == u ? x : t0;
+            t1 = ((b + 1) >> 6) == u ? y : t1;
+        }
+        return b;
+    }
+    int lo = 0, n = seqs;                   // the answer is in [lo, lo + n); 64 probes at a time
     while (n > 1) {
         const int step = (n + 63) / 64, b = lo + lane * step;
-        bool le = false;
-        if (lane * step < n) {
-            int64_t c = a.cu[b];
-            c = c < 0 ? 0 : c > a.q_tokens ? a.q_tokens : c;
-            le = c * a.group / bm + b <= slot;
-        }
-        const int got = __popcll(__ballot(le));       // (lane 0's start is never above the slot)
+        const int got = __popcll(__ballot(lane * step < n && starts_by(b, a.cu[min(b, seqs)])));       // (lane 0's start is never above the slot)
         const int at = got > 0 ? got - 1 : 0;
         lo += at * step;
         n = min(step, n - at * step);
     }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    t0 = __builtin_amdgcn_readfirstlane(a.cu[lo]); t1 = __builtin_amdgcn_readfirstlane(a.cu[lo + 1]);
     return lo;
 }
 
@@ -117,9 +131,8 @@ struct Seq {
     int64_t q0, k0;
     int nq, nk;
 };
-__device__ __forceinline__ Seq seq_at(const AttnArgs &a, int b) {
+__device__ __forceinline__ Seq seq_at(const AttnArgs &a, int b, int64_t t0, int64_t t1) {        // of the tokens [t0, t1)
     Seq s;
-    int64_t t0 = a.cu[b], t1 = a.cu[b + 1];
     if (t0 < 0 || t1 < t0 || t1 > a.q_tokens) t0 = t1 = 0;            // no such rows: nothing is done for them
     s.q0 = t0; s.nq = (int)(t1 - t0);
     if (a.kv_start) {
@@ -128,8 +141,8 @@ __device__ __forceinline__ Seq seq_at(const AttnArgs &a, int b) {
     } else { s.k0 = t0; s.nk = s.nq; }
     return s;
 }
-__device__ __forceinline__ Seq seq_of(const AttnArgs &a, int b) {           // b alike in all lanes
-    Seq s = seq_at(a, b);
+__device__ __forceinline__ Seq seq_of(const AttnArgs &a, int b, int t0, int t1) {           // all alike in all lanes
+    Seq s = seq_at(a, b, t0, t1);
     s.q0 = uniform64(s.q0); s.k0 = uniform64(s.k0);
     s.nq = __builtin_amdgcn_readfirstlane(s.nq); s.nk = __builtin_amdgcn_readfirstlane(s.nk);
     return s;
@@ -152,27 +165,15 @@ struct Rows {
         lane = threadIdx.x & 63;
         asm volatile("" : "+v"(lane));
         const int half = lane >> 5;
-        const int64_t r = row + (lane & 31);
-        live = r < (int64_t)s.nq * a.group;
-        token = live ? (uint32_t)(r / a.group) : 0;
-        head = kvh * a.group + (live ? (uint32_t)(r % a.group) : 0);
+        const uint32_t r = (uint32_t)row + (lane & 31);          // (a sequence has fewer than 2^31 rows)
+        live = r < (uint32_t)s.nq * a.group;
+        token = live ? a.over_group(r) : 0;
+        head = kvh * a.group + (live ? r - token * a.group : 0);
         const int64_t p = (int64_t)token + s.nk - s.nq;
         const int64_t h = a.right < 0 ? s.nk : p + a.right + 1, w = a.left < 0 ? 0 : p - a.left;
         hi = live ? (int)(h < 0 ? 0 : h > s.nk ? s.nk : h) : 0;
         lo = (int)(w < 0 ? 0 : w > s.nk ? s.nk : w);
-        const T *src = (const T *)a.q + (uint64_t)(s.q0 + token) * a.q_stride + (uint64_t)head * a.q_head;
-#pragma unroll
-        for (int i = 0; i < DP / 16; ++i) {
-            const uint32_t d = i * 16 + half * 8;
-            T e[8];
-            if (live && d < a.dim) load_any(e, src + d);
-            else
-                for (int x = 0; x < 8; ++x) e[x] = (T)0.0f;
-            u32x4 w;
-            __builtin_memcpy(&w, e, 16);
-            w ^= a.sign;                // a negative scale: its sign goes to q (exact), so that the largest score has the largest product
-            __builtin_memcpy(&q[i], &w, 16);
-        }
+        load_q(a, s);
 #pragma unroll
         for (int t = 0; t < DP / 32; ++t)
 #pragma unroll
@@ -189,6 +190,22 @@ struct Rows {
             const int row = half * 4 + (sub >> 2);
             at_v[t] = row * (DP * 2) + v_place<DP>(row, t * 4 + ((lane >> 4) & 1) * 2 + ((sub & 3) >> 1)) * 16 + (sub & 1) * 8;
             asm volatile("" : "+v"(at_v[t]));
+        }
+    }
+    __device__ __forceinline__ void load_q(const AttnArgs &a, const Seq &s) {
+        const int half = lane >> 5;
+        const T *src = (const T *)a.q + (uint64_t)(s.q0 + token) * a.q_stride + (uint64_t)head * a.q_head;
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+            const uint32_t d = i * 16 + half * 8;
+            T e[8];
+            if (live && d < a.dim) load_any(e, src + d);
+            else
+                for (int x = 0; x < 8; ++x) e[x] = (T)0.0f;
+            u32x4 w;
+            __builtin_memcpy(&w, e, 16);
+            w ^= a.sign;                // a negative scale: its sign goes to q (exact), so that the largest score has the largest product
+            __builtin_memcpy(&q[i], &w, 16);
         }
     }
 
@@ -221,15 +238,20 @@ struct Rows {
     // Scores to probabilities. Keys from `limit` on belong to no one here; masked: some row does not see some key of these.
     template <int NB>
     __device__ __forceinline__ void softmax(const AttnArgs &a, f32x16 (&s)[NB], V8 (&p)[NB][2], int key, int limit, bool masked) {
-        const int half = lane >> 5, end = min(hi, limit);
         if (masked) {
+            const int half = lane >> 5, end = min(hi, limit);
+            auto first = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; };
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
+            for (int b = 0; b < NB; ++b) {
+                // a bit for each of the block's keys that the row sees; in the order of the registers after a shift by the half's 4
+                const int j = key + b * 32;
+                const uint32_t seen = (first(end - j) & (~first(lo - j) | first((int)a.sinks - j))) >> (4 * half);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const int j = key + b * 32 + (r & 3) + 8 * (r >> 2) + 4 * half;
-                    s[b][r] = j < end && (j >= lo || j < (int)a.sinks) ? s[b][r] : NEG_INF;
+                    const uint32_t keep = (uint32_t)((int)(seen << (31 - (r & 3) - 8 * (r >> 2))) >> 31);
+                    s[b][r] = __uint_as_float((__float_as_uint(s[b][r]) & keep) | (~keep & 0xFF800000u));
                 }
+            }
         }
         float tops[4] = {NEG_INF, NEG_INF, NEG_INF, NEG_INF};
 #pragma unroll
@@ -337,6 +359,18 @@ struct Rows {
     }
 };
 
+// What the live rows [r0, r1) of a sequence see: the last begin and the first end (everybody's), the first begin and the last end (anybody's). No such rows: nothing.
+struct Bounds {
+    int lo_max, hi_min, lo_min, hi_max;
+};
+__device__ __forceinline__ Bounds bounds_of(const AttnArgs &a, const Seq &s, int64_t r0, int64_t r1) {
+    const int64_t rows = (int64_t)s.nq * a.group;
+    if (r1 > rows) r1 = rows;
+    if (r0 >= r1) return Bounds{0, 0x7FFFFFFF, 0x7FFFFFFF, 0};
+    const int64_t p0 = (int64_t)(a.over_group((uint32_t)r0)) + s.nk - s.nq, p1 = (int64_t)(a.over_group((uint32_t)(r1 - 1))) + s.nk - s.nq;
+    auto clamped = [&](int64_t x) { return (int)(x < 0 ? 0 : x > s.nk ? s.nk : x); };
+    return Bounds{a.left < 0 ? 0 : clamped(p1 - a.left), a.right < 0 ? s.nk : clamped(p0 + a.right + 1), a.left < 0 ? 0 : clamped(p0 - a.left), a.right < 0 ? s.nk : clamped(p1 + a.right + 1)};
+}
 // Range of keys that the rows [r0, r1) of a sequence see: sinks [0, first) and [begin, end); a multiple of 32 begins the second.
 struct Range {
     int first, begin, end;
@@ -344,7 +378,7 @@ struct Range {
 __device__ __forceinline__ Range range_of(const AttnArgs &a, const Seq &s, int64_t r0, int64_t r1) {
     const int64_t rows = (int64_t)s.nq * a.group;
     r1 = r1 < rows ? r1 : rows;
-    const int64_t p0 = r0 / a.group + s.nk - s.nq, p1 = (r1 - 1) / a.group + s.nk - s.nq;
+    const int64_t p0 = (int64_t)(a.over_group((uint32_t)r0)) + s.nk - s.nq, p1 = (int64_t)(a.over_group((uint32_t)(r1 - 1))) + s.nk - s.nq;
     int64_t end = a.right < 0 ? s.nk : p1 + a.right + 1, begin = a.left < 0 ? 0 : p0 - a.left;
     end = end < 0 ? 0 : end > s.nk ? s.nk : end;
     begin = begin < 0 ? 0 : begin > end ? end : begin;
@@ -427,24 +461,15 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs a) {
     // neighbouring items (tiles of one key head) on one XCD: it takes every eighth workgroup
     const uint32_t per = items / 8, xcd = blockIdx.x & 7, item = blockIdx.x < per * 8 ? xcd * per + (blockIdx.x >> 3) : blockIdx.x;
     const uint32_t kvh = item / a.slots, slot = item % a.slots;
-    const int b = __builtin_amdgcn_readfirstlane(find_seq(a, slot, BM));
-    const Seq s = seq_of(a, b);
+    int t0, t1;
+    const int b = find_seq(a, slot, BM, t0, t1);
+    const Seq s = seq_of(a, b, t0, t1);
     const int64_t row0 = ((int64_t)slot - (s.q0 * a.group / BM + b)) * BM;
     if (row0 < 0 || row0 >= (int64_t)s.nq * a.group) return;
-    const int t = threadIdx.x, wave = t >> 6;
-    Rows<T, DP> rows;
-    rows.init(a, s, kvh, row0 + wave * 32);
+    const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const Range g = range_of(a, s, row0, row0 + BM);
     const int n_first = (g.first + KT - 1) / KT, n = n_first + (g.end - g.begin + KT - 1) / KT;
-    // what all of the wave's rows see, and what any of them does
-    int lo_max = rows.live ? rows.lo : 0, hi_min = rows.live ? rows.hi : 0x7FFFFFFF, lo_min = rows.live ? rows.lo : 0x7FFFFFFF, hi_max = rows.hi;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        lo_max = max(lo_max, __shfl_xor(lo_max, o)); hi_min = min(hi_min, __shfl_xor(hi_min, o));
-        lo_min = min(lo_min, __shfl_xor(lo_min, o)); hi_max = max(hi_max, __shfl_xor(hi_max, o));
-    }
-    lo_max = __builtin_amdgcn_readfirstlane(lo_max); hi_min = __builtin_amdgcn_readfirstlane(hi_min);
-    lo_min = __builtin_amdgcn_readfirstlane(lo_min); hi_max = __builtin_amdgcn_readfirstlane(hi_max);
+    const Bounds own = bounds_of(a, s, row0 + wave * 32, row0 + wave * 32 + 32), all = bounds_of(a, s, row0, row0 + BM);
     const T *kb = (const T *)a.k + (uint64_t)s.k0 * a.k_stride + (uint64_t)kvh * a.k_head, *vb = (const T *)a.v + (uint64_t)s.k0 * a.v_stride + (uint64_t)kvh * a.v_head;
     auto start_of = [&](int i) { return i < n_first ? i * KT : g.begin + (i - n_first) * KT; };
     auto limit_of = [&](int i) { return i < n_first ? g.first : g.end; };
@@ -479,23 +504,26 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs a) {
         for (int e = t; e < 4 * TILE / 16; e += 256) *reinterpret_cast<u32x4 *>(smem + e * 16) = u32x4{0, 0, 0, 0};
         __syncthreads();
     }
-    // the keys that every row of the workgroup sees: from the last row's first one to the first row's last one
-    const int64_t rows_here = (int64_t)s.nq * a.group - row0, p0 = row0 / a.group + s.nk - s.nq, p1 = (row0 + (rows_here < BM ? rows_here : BM) - 1) / a.group + s.nk - s.nq;
-    const int all_hi = a.right < 0 ? s.nk : (int)max((int64_t)0, min((int64_t)s.nk, p0 + a.right + 1)), all_lo = a.left < 0 ? 0 : (int)max((int64_t)0, min((int64_t)s.nk, p1 - a.left));
     bool spoiled = false;
     if (n > 0) fetch(0);
+    Rows<T, DP> rows;
+    rows.init(a, s, kvh, row0 + wave * 32);
     for (int i = 0; i < n; ++i) {
         // this tile has arrived, for every wave; nobody reads the other buffer any more
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         if (i + 1 < n) fetch(i + 1);
         unsigned char *Ks = smem + (i & 1) * 2 * TILE;
         const int j = start_of(i), limit = limit_of(i);
-        if (!(j + KT <= min(all_hi, limit) && (j >= all_lo || j + KT <= (int)a.sinks))) {        // some row of the workgroup sees it in part
-            const int found = __syncthreads_or(clear_values<T, 256>(Ks + TILE, TILE, t));
-            spoiled |= found != 0;
+        if (!(j + KT <= min(all.hi_min, limit) && (j >= all.lo_max || j + KT <= (int)a.sinks))) {        // some row of the workgroup sees it in part
+            if (__builtin_expect(find_values<T>(Ks + TILE, TILE, t & 63), 0)) {       // (every wave looks through all of it: all find the same)
+                __syncthreads();
+                clear_values<T, 256>(Ks + TILE, TILE, t);
+                __syncthreads();
+                spoiled = true;
+            }
         }
-        if (j < hi_max && (j + KT > lo_min || j < (int)a.sinks)) {
-            const bool masked = !(j + KT <= min(hi_min, limit) && (j >= lo_max || j + KT <= (int)a.sinks));
+        if (j < own.hi_max && (j + KT > own.lo_min || j < (int)a.sinks)) {
+            const bool masked = !(j + KT <= min(own.hi_min, limit) && (j >= own.lo_max || j + KT <= (int)a.sinks));
             f32x16 sc[KT / 32];
             typename Rows<T, DP>::V8 p[KT / 32][2];
             rows.scores(Ks, sc);
@@ -529,7 +557,7 @@ __global__ __launch_bounds__(256, 2) void attn_split_kernel(const AttnArgs a) {
         int64_t q0 = 0, k0 = 0;
         int nq = 0, nk = 0, parts = 1;
         if (b < (int)a.seqs) {
-            const Seq s = seq_at(a, b);
+            const Seq s = seq_at(a, b, a.cu[b], a.cu[b + 1]);
             q0 = s.q0; k0 = s.k0; nq = s.nq; nk = s.nk;
             int64_t seen = nk;
             if (a.left >= 0 && a.right >= 0) seen = min(seen, (int64_t)a.left + a.right + 1 + BM + 64 + (int64_t)a.sinks);
@@ -573,10 +601,7 @@ __global__ __launch_bounds__(256, 2) void attn_split_kernel(const AttnArgs a) {
     const Range g = range_of(a, s, row0, row0 + BM);
     const int n_first = (g.first + KT - 1) / KT, n = n_first + (g.end - g.begin + KT - 1) / KT;
     const int i0 = (int)((int64_t)n * split / parts), i1 = (int)((int64_t)n * (split + 1) / parts);
-    int lo_max = rows.live ? rows.lo : 0, hi_min = rows.live ? rows.hi : 0x7FFFFFFF;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) { lo_max = max(lo_max, __shfl_xor(lo_max, o)); hi_min = min(hi_min, __shfl_xor(hi_min, o)); }
-    lo_max = __builtin_amdgcn_readfirstlane(lo_max); hi_min = __builtin_amdgcn_readfirstlane(hi_min);
+    const Bounds own = bounds_of(a, s, row0, row0 + BM);
     const T *kb = (const T *)a.k + (uint64_t)s.k0 * a.k_stride + (uint64_t)kvh * a.k_head, *vb = (const T *)a.v + (uint64_t)s.k0 * a.v_stride + (uint64_t)kvh * a.v_head;
     unsigned char *Ks = smem + wave * 2 * TILE, *Vs = Ks + TILE;
     auto start_of = [&](int i) { return i < n_first ? i * KT : g.begin + (i - n_first) * KT; };
@@ -625,7 +650,7 @@ __global__ __launch_bounds__(256, 2) void attn_split_kernel(const AttnArgs a) {
     if (i0 + wave < i1) { fetch_k(i0 + wave); fetch_v(i0 + wave); }
     for (int i = i0 + wave; i < i1; i += 4) {
         const int j = start_of(i), limit = limit_of(i);
-        const bool masked = !(j + KT <= min(hi_min, limit) && (j >= lo_max || j + KT <= (int)a.sinks)), more = i + 4 < i1;
+        const bool masked = !(j + KT <= min(own.hi_min, limit) && (j >= own.lo_max || j + KT <= (int)a.sinks)), more = i + 4 < i1;
         f32x16 sc[1];
         typename Rows<T, DP>::V8 p[1][2];
         arrived(false);                       // K
@@ -634,7 +659,10 @@ __global__ __launch_bounds__(256, 2) void attn_split_kernel(const AttnArgs a) {
         if (more) fetch_k(i + 4);
         rows.softmax(a, sc, p, j, limit, masked);
         arrived(!more);                       // V
-        if (masked) spoiled |= __any(clear_values<T, 64>(Vs, TILE, rows.lane));
+        if (masked && __builtin_expect(find_values<T>(Vs, TILE, rows.lane), 0)) {
+            clear_values<T, 64>(Vs, TILE, rows.lane);
+            spoiled = true;
+        }
         rows.values(Vs, p);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         if (more) fetch_v(i + 4);
@@ -778,7 +806,7 @@ static int check_attention(const shodh_attention_cfg *c) {
     if (c->heads == 0 || c->kv_heads == 0 || c->heads % c->kv_heads != 0) { set_error("attention: %u heads over %u key heads", c->heads, c->kv_heads); return SHODH_ERR_INVALID; }
     if (c->head_dim == 0 || c->head_dim % 8 != 0 || c->head_dim > 128) { set_error("attention: head_dim %u is no multiple of 8 up to 128", c->head_dim); return SHODH_ERR_UNSUPPORTED; }
     if (!(c->scale == c->scale) || c->scale > 3.0e38f || c->scale < -3.0e38f) { set_error("attention: scale is no number"); return SHODH_ERR_INVALID; }
-    if (c->q_tokens > 0x7FFFFFFFull || c->kv_tokens > (1ull << 40) || c->heads > 65535u || c->seqs > 0x3FFFFFFFu || c->sinks > 0x7FFFFFFFu) { set_error("attention: a size is out of range"); return SHODH_ERR_UNSUPPORTED; }
+    if (c->q_tokens > 0x7FFFFFFFull / (c->heads / c->kv_heads) || c->kv_tokens > (1ull << 40) || c->heads > 65535u || c->seqs > 0x3FFFFFFFu || c->sinks > 0x7FFFFFFFu) { set_error("attention: a size is out of range"); return SHODH_ERR_UNSUPPORTED; }
     if (c->q_tokens * (c->heads / c->kv_heads) / 32 + c->seqs > 0x7FFFFFFFull / c->kv_heads) { set_error("attention: too many rows for one launch"); return SHODH_ERR_UNSUPPORTED; }
     return SHODH_OK;
 }
@@ -865,7 +893,7 @@ int shodh_window_attention_device(int device, const shodh_attention_cfg *cfg, co
     }
     a.q = d_q; a.k = d_k; a.v = d_v; a.out = d_out; a.lse = d_lse; a.cu = d_cu; a.kv_start = d_kv_start; a.kv_len = d_kv_len; a.part = (float *)d_workspace;
     a.q_tokens = (int64_t)cfg->q_tokens; a.kv_tokens = (int64_t)cfg->kv_tokens;
-    a.heads = cfg->heads; a.kv_heads = cfg->kv_heads; a.group = cfg->heads / cfg->kv_heads; a.dim = cfg->head_dim; a.seqs = cfg->seqs;
+    a.heads = cfg->heads; a.kv_heads = cfg->kv_heads; a.group = cfg->heads / cfg->kv_heads; a.shift = (a.group & (a.group - 1)) == 0 ? __builtin_ctz(a.group) : -1; a.dim = cfg->head_dim; a.seqs = cfg->seqs;
     a.slots = p.slots; a.splits = p.splits; a.chunk = p.chunk; a.sinks = cfg->sinks; a.left = cfg->left; a.right = cfg->right;
     const float scale = cfg->scale == 0.0f ? 1.0f / __builtin_sqrtf((float)d) : cfg->scale;
     a.scale2 = __builtin_fabsf(scale) * 1.44269504088896340736f;
