@@ -3,6 +3,7 @@ output, dense layers on 4-bit weights, attention with a sliding window and alway
 current stream unless `stream` names another (a raw hipStream_t), and can be captured into a graph. Nothing here computes on the host."""
 import collections
 import ctypes as C
+import functools
 
 import torch
 
@@ -30,19 +31,27 @@ def _on(t, device, name):
         _refuse("%s is on %s, not on %s" % (name, t.device, device))
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)         # (0.1 us; the Stream object of the line below takes 2 us to make)
+
+
 def _stream(device, stream):
-    return torch.cuda.current_stream(device).cuda_stream if stream is None else stream
+    if stream is not None:
+        return stream
+    return _raw_stream(device.index) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
 
 
 def _matrix(t, name):
     """(rows, columns, row stride) of [..., columns] with neighbouring elements next to each other: a view of rows at one distance."""
     if t.dim() == 2:
         rows, cols = t.shape
-        if cols > 1 and t.stride(1) != 1:
+        step, one = t.stride()
+        if cols > 1 and one != 1:
             _refuse("%s: the last dimension has to be contiguous" % name)
-        if rows > 1 and t.stride(0) == 0:
-            _refuse("%s: rows at distance 0 (an expanded tensor)" % name)
-        return rows, cols, t.stride(0) if rows > 1 else cols
+        if rows > 1:
+            if step == 0:
+                _refuse("%s: rows at distance 0 (an expanded tensor)" % name)
+            return rows, cols, step
+        return rows, cols, cols
     if t.dim() == 0:
         _refuse("%s has no dimension" % name)
     cols = t.shape[-1]
@@ -73,23 +82,25 @@ def rms_norm(x, weight, eps=1e-6, residual=None, want_y=True, quant=None, group=
             _refuse("residual has to be of x's shape and type", L.ERR_DIM)
         _on(residual, device, "residual")
         rs = _matrix(residual, "residual")[2]
-        total = torch.empty(x.shape, dtype=x.dtype, device=device) if sum_out is None else sum_out
-        if sum_out is not None:
+        if sum_out is None:
+            total = x.new_empty(x.shape)
+        else:
+            total = sum_out
             if total.shape != x.shape or total.dtype != x.dtype:
                 _refuse("sum_out has to be of x's shape and type", L.ERR_DIM)
             _on(total, device, "sum_out")
-        ss = _matrix(total, "sum_out")[2]
+            ss = _matrix(total, "sum_out")[2]
     elif sum_out is not None:
         _refuse("sum_out without a residual")
-    y = torch.empty(x.shape, dtype=x.dtype, device=device) if want_y else None
+    y = x.new_empty(x.shape) if want_y else None
     q = scale = None
     qd = L.DTYPE_INT8
     if quant is not None:
         if quant not in _QUANT:
             _refuse("quant %r is neither 'int8' nor 'e4m3'" % (quant,))
         qd, qt = _QUANT[quant]
-        q = torch.empty(x.shape, dtype=qt, device=device)
-        scale = torch.empty((rows, -(-dim // group) if group else 1), dtype=torch.float32, device=device)
+        q = x.new_empty(x.shape, dtype=qt)
+        scale = x.new_empty((rows, -(-dim // group) if group else 1), dtype=torch.float32)
     if rows == 0:
         return RmsNorm(y, q, scale, total)
     cfg = L.RmsNormCfg(rows, xs, rs, ss, 0, 0, dim, dt, wd, qd, group, eps)
@@ -189,14 +200,16 @@ class W4Weight:
             bp = bias.data_ptr()
         shape = x.shape[:-1] + (self.n,)
         if out is None:
-            out = torch.empty(shape, dtype=out_dtype or (torch.bfloat16 if xd == L.DTYPE_INT8 else x.dtype), device=self.device)
+            out = x.new_empty(shape, dtype=out_dtype or (torch.bfloat16 if xd == L.DTYPE_INT8 else x.dtype))
+            os_ = self.n
         else:
             if out.shape != shape or (out_dtype is not None and out.dtype != out_dtype):
                 _refuse("out has to be %s" % (tuple(shape),), L.ERR_DIM)
             _on(out, self.device, "out")
+            os_ = _matrix(out, "out")[2]
         if rows == 0:
             return out
-        L.check(L.lib().shodh_w4_dense_device(self._h, x.data_ptr(), xd, xs, sp, rows, bp, out.data_ptr(), _dtype(out, "out"), _matrix(out, "out")[2],
+        L.check(L.lib().shodh_w4_dense_device(self._h, x.data_ptr(), xd, xs, sp, rows, bp, out.data_ptr(), _dtype(out, "out"), os_,
                                               _stream(self.device, stream)))
         return out
 
@@ -225,9 +238,18 @@ def _heads(t, name, device, dtype):
 
 
 def _descriptor(t, name, device, dtype, n):
-    if t.dtype != dtype or t.device != device or tuple(t.shape) != (n,) or not t.is_contiguous():
+    if t.dtype != dtype or t.device != device or t.shape != (n,) or not t.is_contiguous():
         _refuse("%s has to be contiguous %s [%d] on %s" % (name, dtype, n, device))
     return t.data_ptr()
+
+
+@functools.lru_cache(maxsize=1024)
+def _attention_workspace(device, n, kn, dt, heads, kv_heads, dim, seqs, sinks, left, right):
+    """shodh_window_attention_workspace: a function of sizes alone"""
+    cfg = L.AttentionCfg(n, kn, 0, 0, 0, 0, 0, 0, 0, 0, dt, heads, kv_heads, dim, seqs, sinks, left, right, 0.0, 0)
+    need = C.c_uint64()
+    L.check(L.lib().shodh_window_attention_workspace(device, C.byref(cfg), C.byref(need)))
+    return need.value
 
 
 def window_attention(q, k, v, cu, left=-1, right=-1, sinks=0, kv_start=None, kv_len=None, scale=None, return_lse=False, out=None, stream=None):
@@ -258,23 +280,24 @@ def window_attention(q, k, v, cu, left=-1, right=-1, sinks=0, kv_start=None, kv_
     if kv_start is not None:
         sp, lp = _descriptor(kv_start, "kv_start", device, torch.int64, seqs), _descriptor(kv_len, "kv_len", device, torch.int32, seqs)
     if out is None:
-        out = torch.empty((n, heads, dim), dtype=q.dtype, device=device)
-    elif out.shape != q.shape:
-        _refuse("out has to be of q's shape", L.ERR_DIM)
-    os_, oh = _heads(out, "out", device, q.dtype)
+        out = q.new_empty((n, heads, dim))
+        os_, oh = heads * dim, dim
+    else:
+        if out.shape != q.shape:
+            _refuse("out has to be of q's shape", L.ERR_DIM)
+        os_, oh = _heads(out, "out", device, q.dtype)
     if sinks < 0 or not -2 ** 31 <= left < 2 ** 31 or not -2 ** 31 <= right < 2 ** 31:
         _refuse("left, right and sinks are 32-bit numbers, sinks 0 or more")
     if scale is not None and not scale != 0:
         _refuse("scale 0 (or no number)")
-    lse = torch.empty((n, heads), dtype=torch.float32, device=device) if return_lse else None
+    lse = q.new_empty((n, heads), dtype=torch.float32) if return_lse else None
     if n and seqs:
         cfg = L.AttentionCfg(n, kn, qs, qh, ks, kh, vs, vh, os_, oh, dt, heads, kv_heads, dim, seqs, sinks, left, right, scale or 0.0, 0)
-        need = C.c_uint64()
-        L.check(L.lib().shodh_window_attention_workspace(device.index, C.byref(cfg), C.byref(need)))
-        work = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
+        need = _attention_workspace(device.index, n, kn, dt, heads, kv_heads, dim, seqs, sinks, left, right)
+        work = q.new_empty(need, dtype=torch.uint8) if need else None
         st = _stream(device, stream)
         if work is not None and stream is not None:
             work.record_stream(torch.cuda.ExternalStream(stream, device=device))
         L.check(L.lib().shodh_window_attention_device(device.index, C.byref(cfg), q.data_ptr(), k.data_ptr(), v.data_ptr(), cup, sp, lp, out.data_ptr(),
-                                                      lse.data_ptr() if return_lse else None, work.data_ptr() if work is not None else None, need.value, st))
+                                                      lse.data_ptr() if return_lse else None, work.data_ptr() if work is not None else None, need, st))
     return (out, lse) if return_lse else out
