@@ -25,22 +25,41 @@ struct RmsArgs {
     float eps;
 };
 
-template <class T>
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
+
+// 8 values (n of them at a row's end). STREAM: past the caches, for data that is larger than they are.
+template <bool STREAM, class T>
 __device__ __forceinline__ void load8(float (&v)[8], const T *p, uint32_t n) {
     T t[8];
-    if (n >= 8) load_any(t, p);
-    else
+    if (n >= 8) {
+        if constexpr (STREAM) {
+#pragma unroll
+            for (int k = 0; k < (int)sizeof(T) / 2; ++k) {
+                const u32x4_any w = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any *>(p) + k);
+                __builtin_memcpy(t + 16 / sizeof(T) * k, &w, 16);
+            }
+        } else load_any(t, p);
+    } else
         for (int i = 0; i < 8; ++i) t[i] = (uint32_t)i < n ? p[i] : (T)0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = (float)t[i];
 }
-template <class T>
+template <bool STREAM, class T>
 __device__ __forceinline__ void store8(T *p, const float (&v)[8], uint32_t n) {
     T t[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) t[i] = (T)v[i];
-    if (n >= 8) store_any(p, t);
-    else
+    if (n >= 8) {
+        if constexpr (STREAM) {
+#pragma unroll
+            for (int k = 0; k < (int)sizeof(T) / 2; ++k) {
+                u32x4_any w;
+                __builtin_memcpy(&w, t + 16 / sizeof(T) * k, 16);
+                __builtin_nontemporal_store(w, reinterpret_cast<u32x4_any *>(p) + k);
+            }
+        } else store_any(p, t);
+    } else
         for (int i = 0; i < 8; ++i) if ((uint32_t)i < n) p[i] = t[i];
 }
 
@@ -55,7 +74,7 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v, int lanes) {
 }
 
 // TPR threads own a row of at most TPR * 8 * C values; a workgroup of max(TPR, 256) threads holds 256 / TPR rows (TPR = 64) or one.
-template <class T, int TPR, int C>
+template <class T, int TPR, int C, bool STREAM>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(const RmsArgs a) {
     constexpr int WAVES = TPR / 64, ROWS = TPR < 256 ? 256 / TPR : 1;
     __shared__ float part[2][WAVES];
@@ -67,8 +86,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(const R
     for (int c = 0; c < C; ++c) {
         const uint32_t at = (uint32_t)(c * TPR + t) * 8;
         left[c] = at < a.dim ? a.dim - at : 0;
-        if (a.weight_f32) load8(w[c], (const float *)a.weight + at, left[c]);
-        else load8(w[c], (const T *)a.weight + at, left[c]);
+        if (a.weight_f32) load8<false>(w[c], (const float *)a.weight + at, left[c]);
+        else load8<false>(w[c], (const T *)a.weight + at, left[c]);
     }
     auto row_sum = [&](float v, int slot) -> float {
         v = wave_sum(v);
@@ -86,12 +105,12 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(const R
         float h[C][8];
         float ss = 0.0f;
 #pragma unroll
-        for (int c = 0; c < C; ++c) load8(h[c], (const T *)a.x + row * a.x_stride + (c * TPR + t) * 8, left[c]);
+        for (int c = 0; c < C; ++c) load8<STREAM>(h[c], (const T *)a.x + row * a.x_stride + (c * TPR + t) * 8, left[c]);
         if (a.residual) {
 #pragma unroll
             for (int c = 0; c < C; ++c) {
                 float r[8];
-                load8(r, (const T *)a.residual + row * a.residual_stride + (c * TPR + t) * 8, left[c]);
+                load8<STREAM>(r, (const T *)a.residual + row * a.residual_stride + (c * TPR + t) * 8, left[c]);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) h[c][i] += r[i];
             }
@@ -102,7 +121,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(const R
             for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(h[c][i], h[c][i], ss);
         if (a.sum)
 #pragma unroll
-            for (int c = 0; c < C; ++c) store8((T *)a.sum + row * a.sum_stride + (c * TPR + t) * 8, h[c], left[c]);
+            for (int c = 0; c < C; ++c) store8<STREAM>((T *)a.sum + row * a.sum_stride + (c * TPR + t) * 8, h[c], left[c]);
         ss = row_sum(ss, slot);
         slot ^= 1;
         float eps = a.eps;
@@ -123,7 +142,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(const R
             for (int i = 0; i < 8; ++i) h[c][i] = h[c][i] * rstd * w[c][i];
         if (a.y)
 #pragma unroll
-            for (int c = 0; c < C; ++c) store8((T *)a.y + row * a.y_stride + (c * TPR + t) * 8, h[c], left[c]);
+            for (int c = 0; c < C; ++c) store8<STREAM>((T *)a.y + row * a.y_stride + (c * TPR + t) * 8, h[c], left[c]);
         if (a.q_dtype) {
             // |y| as bits: for magnitudes the order of unsigned integers is that of the numbers, with infinity and then NaN above all of them
             uint32_t m[C];
@@ -177,28 +196,34 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(const R
                     __builtin_memcpy(b + 4, &hi, 4);
                 }
                 uint8_t *dst = (uint8_t *)a.q + row * a.q_stride + at;
-                if (left[c] >= 8) store_any(dst, b);
-                else
+                if (left[c] >= 8) {
+                    if constexpr (STREAM) {
+                        u32x2_any w;
+                        __builtin_memcpy(&w, b, 8);
+                        __builtin_nontemporal_store(w, reinterpret_cast<u32x2_any *>(dst));
+                    } else store_any(dst, b);
+                } else
                     for (int i = 0; i < 8; ++i) if ((uint32_t)i < left[c]) dst[i] = b[i];
             }
         }
     }
 }
 
-template <class T>
-static int launch_rms(const RmsArgs &a, int cus, hipStream_t st) {
-    // (workgroups resident at 8 waves a SIMD) x CUs: further rows are taken in a loop, with the weights kept in registers
+template <class T, bool STREAM>
+static int launch_rms(const RmsArgs &a, hipStream_t st) {
+    // one workgroup for every one or four rows: its neighbours on the CU hide its waits (a loop over rows with the weights kept: 213 instead of 198 us
+    // for 32768 x 4096 bf16 with residual, sum and e4m3)
     auto go = [&](auto kern, int threads, int rows_per_wg) {
-        const uint64_t wgs = ceil_div(a.rows, rows_per_wg), most = (uint64_t)cus * (2048 / threads);
+        const uint64_t wgs = ceil_div(a.rows, rows_per_wg), most = 1u << 24;
         hipLaunchKernelGGL(kern, dim3((uint32_t)(wgs < most ? wgs : most)), dim3(threads), 0, st, a);
     };
-    if (a.dim <= 512) go(rms_norm_kernel<T, 64, 1>, 256, 4);
-    else if (a.dim <= 1024) go(rms_norm_kernel<T, 64, 2>, 256, 4);
-    else if (a.dim <= 2048) go(rms_norm_kernel<T, 256, 1>, 256, 1);
-    else if (a.dim <= 4096) go(rms_norm_kernel<T, 256, 2>, 256, 1);
-    else if (a.dim <= 8192) go(rms_norm_kernel<T, 256, 4>, 256, 1);
-    else if (a.dim <= 16384) go(rms_norm_kernel<T, 1024, 2>, 1024, 1);
-    else go(rms_norm_kernel<T, 1024, 4>, 1024, 1);
+    if (a.dim <= 512) go(rms_norm_kernel<T, 64, 1, STREAM>, 256, 4);
+    else if (a.dim <= 1024) go(rms_norm_kernel<T, 64, 2, STREAM>, 256, 4);
+    else if (a.dim <= 2048) go(rms_norm_kernel<T, 256, 1, STREAM>, 256, 1);
+    else if (a.dim <= 4096) go(rms_norm_kernel<T, 256, 2, STREAM>, 256, 1);
+    else if (a.dim <= 8192) go(rms_norm_kernel<T, 256, 4, STREAM>, 256, 1);
+    else if (a.dim <= 16384) go(rms_norm_kernel<T, 1024, 2, STREAM>, 1024, 1);
+    else go(rms_norm_kernel<T, 1024, 4, STREAM>, 1024, 1);
     SHODH_HIP_TRY(hipGetLastError());
     return SHODH_OK;
 }
@@ -257,11 +282,15 @@ int shodh_rms_norm_device(int device, const shodh_rms_norm_cfg *cfg, const void 
     a.rows = cfg->rows; a.x_stride = xs; a.residual_stride = rs; a.sum_stride = ss; a.y_stride = ys; a.q_stride = qs;
     a.dim = cfg->dim; a.group_lanes = cfg->q_group / 8; a.groups = cfg->q_group ? (uint32_t)ceil_div(dim, cfg->q_group) : 1;
     a.weight_f32 = cfg->weight_dtype == SHODH_DTYPE_FP32; a.q_dtype = d_q ? cfg->q_dtype : 0; a.eps = cfg->eps;
-    const int cus = compute_units(device);
     hipStream_t st = (hipStream_t)stream;
-    if (cfg->dtype == SHODH_DTYPE_FP32) return launch_rms<float>(a, cus, st);
-    if (cfg->dtype == SHODH_DTYPE_BF16) return launch_rms<__bf16>(a, cus, st);
-    return launch_rms<_Float16>(a, cus, st);
+    // 16-bit types, whole 16-byte pieces: past the caches from 256 MiB on, the size of the last level (what is written does not stay there anyway).
+    // With residual, sum and e4m3, us through / past them: 65536 x 1024 bf16 102 / 79, 16384 x 4096 102 / 80, 32768 x 4096 198 / 155; f32 65536 x 1024
+    // 163 / 168; rows of 771, 16384 of them, 24.5 / 26.7.
+    const uint64_t each = b * (1 + (d_residual ? 1 : 0) + (d_sum ? 1 : 0) + (d_y ? 1 : 0)) + (d_q ? 1 : 0);
+    const bool past = cfg->rows * dim * each > (256ull << 20) && ((dim | xs | rs | ss | ys | qs) & 7) == 0;
+    if (cfg->dtype == SHODH_DTYPE_FP32) return launch_rms<float, false>(a, st);
+    if (cfg->dtype == SHODH_DTYPE_BF16) return past ? launch_rms<__bf16, true>(a, st) : launch_rms<__bf16, false>(a, st);
+    return past ? launch_rms<_Float16, true>(a, st) : launch_rms<_Float16, false>(a, st);
 }
 
 }  // extern "C"

@@ -146,6 +146,20 @@ def test_many_rows_each_its_own(layers):
     check_rounded(r.y, y, torch.float16, 70 * U)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_more_data_than_the_caches_hold(layers, dtype):
+    """the form that goes past the caches: rows are what they are alone"""
+    x = torch.randn(66000, 1024, device="cuda").to(TYPES[dtype])
+    res, w = x.flip(0).contiguous(), torch.rand(1024, device="cuda").to(TYPES[dtype])
+    r = layers.rms_norm(x, w, residual=res, quant="e4m3", group=128)
+    at = torch.tensor([0, 1, 33000, 65999], device="cuda")
+    s = layers.rms_norm(x[at].contiguous(), w, residual=res[at].contiguous(), quant="e4m3", group=128)
+    assert torch.equal(r.y[at], s.y) and torch.equal(r.sum[at], s.sum) and torch.equal(r.scale[at], s.scale)
+    assert torch.equal(r.q.view(torch.uint8)[at], s.q.view(torch.uint8))
+    h, y = defined(x, w, res, 1e-6)
+    check_rounded(r.y, y, TYPES[dtype], 70 * U)
+
+
 def test_streams_and_graph(layers):
     x, w = torch.randn(50, 1024, device="cuda").bfloat16(), torch.rand(1024, device="cuda").bfloat16()
     res = torch.randn(50, 1024, device="cuda").bfloat16()
