@@ -168,16 +168,19 @@ struct Piece {
     using E = typename XFrag<X>::E;
     static constexpr int PER = 16 / (int)sizeof(E), ROW = W4_TK * (int)sizeof(E), PLACES = ROW / 16;
     static __device__ __forceinline__ int place(int row, int c) { return sizeof(E) == 1 ? c ^ ((row >> 1) & 7) : sizeof(E) == 2 ? c ^ (row & 15) : c ^ ((row & 15) << 1); }
-    static __device__ __forceinline__ u32x4 load(const E *row, uint32_t k0, int c, uint32_t K) {
+    static __device__ __forceinline__ u32x4 load(const E *row, uint32_t k0, int c) {          // of a block within the row
+        E v[PER];
+        load_any(v, row + k0 + c * PER);
+        return __builtin_bit_cast(u32x4, v);
+    }
+    static __device__ __forceinline__ u32x4 load_part(const E *row, uint32_t k0, int c, uint32_t K) {      // of the last block: zeros behind the row's end
         const uint32_t k = k0 + c * PER;
         E v[PER];
-        if (k0 + W4_TK <= K) load_any(v, row + k);          // (the same for all lanes)
-        else
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                const E w = row[min(k + i, K - 1)];
-                v[i] = k + i < K ? w : (E)0;
-            }
+        for (int i = 0; i < PER; ++i) {
+            const E w = row[min(k + i, K - 1)];
+            v[i] = k + i < K ? w : (E)0;
+        }
         return __builtin_bit_cast(u32x4, v);
     }
     static __device__ __forceinline__ void store(unsigned char *xs, int row, int c, u32x4 v) { *reinterpret_cast<u32x4 *>(xs + row * ROW + place(row, c) * 16) = v; }
@@ -374,10 +377,11 @@ __global__ __launch_bounds__(512, FEW && GROUP != 32 ? 6 : MT == 1 ? 4 : 2) void
     for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0, 0, 0, 0};
-    auto load_x = [&](u32x4 (&v)[PIECES], uint32_t block) {
+    auto x_row = [&](int i) { return (const E *)a.x + (uint64_t)min(m0 + i * STEP + piece_row, a.M - 1) * a.x_stride; };     // (rows behind the last repeat it: not written)
+    auto load = [&](u32x4 (&v)[PIECES], Block<X, GROUP, MT, NT> &w, uint32_t block) {
+        w.load_w(a, rec, (size_t)block * a.record, lane);
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i)       // (rows behind the last repeat it: not written)
-            v[i] = P::load((const E *)a.x + (uint64_t)min(m0 + i * STEP + piece_row, a.M - 1) * a.x_stride, block * W4_TK, piece_place, a.K);
+        for (int i = 0; i < PIECES; ++i) v[i] = P::load(x_row(i), block * W4_TK, piece_place);
     };
     auto store_x = [&](const u32x4 (&v)[PIECES]) {          // (LDS serves a wave's accesses in order: only the compiler has to be held)
         asm volatile("" ::: "memory");
@@ -388,21 +392,31 @@ __global__ __launch_bounds__(512, FEW && GROUP != 32 ? 6 : MT == 1 ? 4 : 2) void
     auto fragment = [&](int s, int i) { return P::fragment(xs, i * 16 + (lane & 15), s, lane >> 4); };
     u32x4 x[U][PIECES];
     Block<X, GROUP, MT, NT> b[U];
+    const uint32_t full = a.K / W4_TK;         // blocks that no row ends in; loads of these are never behind a branch: a wait after one would be for all of them
     uint32_t at = wave;
     if constexpr (U > 1) {
-        for (; at + (U - 1) * waves < a.blocks; at += U * waves) {
+        for (; at + (U - 1) * waves < full; at += U * waves) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) { b[u].load_w(a, rec, (size_t)(at + u * waves) * a.record, lane); load_x(x[u], at + u * waves); }
+            for (int u = 0; u < U; ++u) load(x[u], b[u], at + u * waves);
 #pragma unroll
             for (int u = 0; u < U; ++u) { store_x(x[u]); b[u].multiply(a, acc, fragment); }
         }
     }
-    if (at < a.blocks) { b[0].load_w(a, rec, (size_t)at * a.record, lane); load_x(x[0], at); }
-    for (; at < a.blocks; at += waves) {
+    if (at < full) {
+        load(x[0], b[0], at);
+        for (; at < full; at += waves) {
+            store_x(x[0]);
+            const Block<X, GROUP, MT, NT> cur = b[0];
+            load(x[0], b[0], min(at + waves, full - 1));          // (the last one once more: not used)
+            cur.multiply(a, acc, fragment);
+        }
+    }
+    if (at < a.blocks) {
+        b[0].load_w(a, rec, (size_t)at * a.record, lane);
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) x[0][i] = P::load_part(x_row(i), at * W4_TK, piece_place, a.K);
         store_x(x[0]);
-        const Block<X, GROUP, MT, NT> cur = b[0];
-        if (at + waves < a.blocks) { b[0].load_w(a, rec, (size_t)(at + waves) * a.record, lane); load_x(x[0], at + waves); }
-        cur.multiply(a, acc, fragment);
+        b[0].multiply(a, acc, fragment);
     }
     __syncthreads();
     finish<X, MT, NT>(a, acc, reinterpret_cast<float *>(smem), wave, waves, threadIdx.x, blockDim.x, m0, blockIdx.x * NT, lane);
@@ -430,28 +444,47 @@ __global__ __launch_bounds__(512, 2) void w4_dense_shared_kernel(const W4Args a)
         for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0, 0, 0, 0};
     u32x4 x[2][N];
     Block<X, GROUP, MT, NT> b[2];
+    const uint32_t full = a.K / W4_TK;         // blocks that no row ends in; loads of these are never behind a branch: a wait after one would be for all of them
+    auto x_row = [&](int i) { return (const E *)a.x + (uint64_t)min(m0 + i * STEP + piece_row, a.M - 1) * a.x_stride; };
     auto load = [&](u32x4 (&v)[N], Block<X, GROUP, MT, NT> &w, uint32_t block) {
-        if (block >= a.blocks) return;
         w.load_w(a, rec, (size_t)block * a.record, lane);
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = P::load((const E *)a.x + (uint64_t)min(m0 + i * STEP + piece_row, a.M - 1) * a.x_stride, block * W4_TK, piece_place, a.K);
+        for (int i = 0; i < N; ++i) v[i] = P::load(x_row(i), block * W4_TK, piece_place);
+    };
+    auto store = [&](const u32x4 (&v)[N], unsigned char *xs) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) P::store(xs, i * STEP + piece_row, piece_place, v[i]);
     };
     unsigned char *mine = smem + wk * 2 * TILE;
+    auto multiply = [&](const Block<X, GROUP, MT, NT> &w, const unsigned char *xs) {
+        w.multiply(a, acc, [&](int s, int i) { return P::fragment(xs, i * 16 + (lane & 15), s, lane >> 4); });
+    };
     auto round = [&](u32x4 (&v)[N], Block<X, GROUP, MT, NT> &w, unsigned char *xs, uint32_t block) {
-        if (block < a.blocks)
-#pragma unroll
-            for (int i = 0; i < N; ++i) P::store(xs, i * STEP + piece_row, piece_place, v[i]);
+        store(v, xs);
         __syncthreads();
         const Block<X, GROUP, MT, NT> cur = w;
-        load(v, w, block + 2 * WK);
-        if (block < a.blocks) cur.multiply(a, acc, [&](int s, int i) { return P::fragment(xs, i * 16 + (lane & 15), s, lane >> 4); });
+        load(v, w, min(block + 2 * WK, full - 1));              // (past the end the last one once more: not used)
+        if (block < full) multiply(cur, xs);
     };
-    load(x[0], b[0], wk);
-    load(x[1], b[1], wk + WK);
-    const uint32_t rounds = (a.blocks + WK - 1) / WK;
-    for (uint32_t r = 0; r < rounds; r += 2) {
-        round(x[0], b[0], mine, r * WK + wk);
-        if (r + 1 < rounds) round(x[1], b[1], mine + TILE, (r + 1) * WK + wk);
+    if (full) {
+        load(x[0], b[0], min((uint32_t)wk, full - 1));
+        load(x[1], b[1], min((uint32_t)wk + WK, full - 1));
+        const uint32_t rounds = (full + WK - 1) / WK;
+        for (uint32_t r = 0; r < rounds; r += 2) {
+            round(x[0], b[0], mine, r * WK + wk);
+            round(x[1], b[1], mine + TILE, (r + 1) * WK + wk);
+        }
+    }
+    if (full < a.blocks) {
+        const bool turn = (int)(full % WK) == wk;
+        if (turn) {
+            b[0].load_w(a, rec, (size_t)full * a.record, lane);
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[0][i] = P::load_part(x_row(i), full * W4_TK, piece_place, a.K);
+            store(x[0], mine);              // (the last round read the other half)
+        }
+        __syncthreads();
+        if (turn) multiply(b[0], mine);
     }
     __syncthreads();
     finish<X, MT, NT>(a, acc, reinterpret_cast<float *>(smem) + wn * WK * NT * MT * 256, wk, WK, wk * 64 + lane, WK * 64, m0, tile0, lane);
