@@ -13,7 +13,9 @@
 // A row of x that holds a NaN or an infinity gives NaN in all its outputs (16 x - 16 x).
 #include "layers.h"
 
+#include <cstddef>
 #include <new>
+#include <type_traits>
 #include <vector>
 
 #pragma clang fp contract(off)
@@ -269,17 +271,18 @@ struct Block {
             }
         }
     }
-    // fragment(t, i): x's step t of tile i
-    template <class Fragment>
-    __device__ __forceinline__ void multiply(const W4Args &a, f32x4 (&acc)[NT][MT], Fragment fragment) const {
+    // fragment(t, i): x's step t of tile i; total(g, i): the sum of x over group g for the lane's row of tile i, or nullptr: it is made here
+    template <class Fragment, class Total>
+    __device__ __forceinline__ void multiply(const W4Args &a, f32x4 (&acc)[NT][MT], Fragment fragment, Total total) const {
         using V = typename Acc<X>::V;
-        const WFrag<X> ones = w_ones<X>();
+        constexpr bool OWN = std::is_same_v<Total, std::nullptr_t>;
 #pragma unroll
         for (int g = 0; g < PER; ++g) {
             V d[NT][MT], sum[MT];
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
                 sum[i] = V{0, 0, 0, 0};
+                if constexpr (!OWN) sum[i][0] = total(g, i);
 #pragma unroll
                 for (int j = 0; j < NT; ++j) d[j][i] = V{0, 0, 0, 0};
             }
@@ -296,9 +299,9 @@ struct Block {
 #pragma unroll
                     for (int i = 0; i < MT; ++i) d[j][i] = mma<X>(wf, x[i], d[j][i]);
                 }
-                if constexpr (!EXACT)
+                if constexpr (!EXACT && OWN)
 #pragma unroll
-                    for (int i = 0; i < MT; ++i) sum[i] = mma<X>(ones, x[i], sum[i]);
+                    for (int i = 0; i < MT; ++i) sum[i] = mma<X>(w_ones<X>(), x[i], sum[i]);
             }
             if constexpr (PER > 1) __builtin_amdgcn_sched_barrier(0);          // (groups one after another: side by side they would only cost registers)
 #pragma unroll
@@ -311,9 +314,9 @@ struct Block {
 #pragma unroll
                     for (int i = 0; i < MT; ++i) {
                         float v;
-                        if constexpr (X == W4_I8) v = (float)(d[j][i][r] - (zero - 16) * sum[i][r]);
+                        if constexpr (X == W4_I8) v = (float)(d[j][i][r] - (zero - 16) * sum[i][0]);          // (a row's sum: the same for all outputs)
                         else if constexpr (EXACT) v = d[j][i][r];
-                        else v = __builtin_fmaf(-(float)zero, sum[i][r], d[j][i][r]);
+                        else v = __builtin_fmaf(-(float)zero, sum[i][0], d[j][i][r]);
                         acc[j][i][r] = __builtin_fmaf(v, scale, acc[j][i][r]);
                     }
                 }
@@ -399,7 +402,7 @@ __global__ __launch_bounds__(512, FEW && GROUP != 32 ? 6 : MT == 1 ? 4 : 2) void
 #pragma unroll
             for (int u = 0; u < U; ++u) load(x[u], b[u], at + u * waves);
 #pragma unroll
-            for (int u = 0; u < U; ++u) { store_x(x[u]); b[u].multiply(a, acc, fragment); }
+            for (int u = 0; u < U; ++u) { store_x(x[u]); b[u].multiply(a, acc, fragment, nullptr); }
         }
     }
     if (at < full) {
@@ -408,7 +411,7 @@ __global__ __launch_bounds__(512, FEW && GROUP != 32 ? 6 : MT == 1 ? 4 : 2) void
             store_x(x[0]);
             const Block<X, GROUP, MT, NT> cur = b[0];
             load(x[0], b[0], min(at + waves, full - 1));          // (the last one once more: not used)
-            cur.multiply(a, acc, fragment);
+            cur.multiply(a, acc, fragment, nullptr);
         }
     }
     if (at < a.blocks) {
@@ -416,24 +419,27 @@ __global__ __launch_bounds__(512, FEW && GROUP != 32 ? 6 : MT == 1 ? 4 : 2) void
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) x[0][i] = P::load_part(x_row(i), at * W4_TK, piece_place, a.K);
         store_x(x[0]);
-        b[0].multiply(a, acc, fragment);
+        b[0].multiply(a, acc, fragment, nullptr);
     }
     __syncthreads();
     finish<X, MT, NT>(a, acc, reinterpret_cast<float *>(smem), wave, waves, threadIdx.x, blockDim.x, m0, blockIdx.x * NT, lane);
 }
 
-// More than 16 rows and many outputs: x's blocks are shared by WN waves of 2 x 16 outputs each; WK such sets of waves take every WK-th block. Blocks are
-// asked for two rounds ahead.
+// More than 16 rows and many outputs: x's blocks are shared by WN waves of 2 x 16 outputs each; WK such sets of waves take every WK-th block. A wave
+// brings MT * 16 / WN rows of a block to LDS, a block ahead of the multiplying, and makes those rows' sums there for all (a third of the matrix
+// instructions, were each wave to make its own: 28672 x 4096, 64 rows 29.9 us, 27.1 so). Blocks are asked for two rounds ahead, x's three.
 template <int X, int GROUP, int MT, int WN, int WK>
 __global__ __launch_bounds__(512, 2) void w4_dense_shared_kernel(const W4Args a) {
     using P = Piece<X>;
     using E = typename P::E;
-    constexpr int NT = 2, ROWS = MT * 16, TILE = ROWS * P::ROW, NTH = WN * 64, N = ROWS * P::PLACES / NTH, STEP = NTH / P::PLACES;
+    using V = typename Acc<X>::V;
+    using S = std::conditional_t<X == W4_I8, int, float>;
+    constexpr int NT = 2, ROWS = MT * 16, TILE = ROWS * P::ROW, MINE = ROWS / WN, STEP = 64 / P::PLACES, N = MINE / STEP, PER = W4_TK / GROUP, COLS = MINE < 16 ? MINE : 16;
     static_assert(WN * WK == 8 && N >= 1, "");
-    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];           // [WK][2][TILE]; then the sums
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % WN, wk = wave / WN, t = wn * 64 + lane;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];           // [WK][2][TILE]; [WK][2][PER][ROWS] sums of x; then the outputs' sums
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % WN, wk = wave / WN;
     const uint32_t m0 = blockIdx.y * (MT * 16u), tiles = (a.N + W4_TN - 1) / W4_TN, tile0 = (blockIdx.x * WN + wn) * NT;
-    const int piece_row = t / P::PLACES, piece_place = t % P::PLACES;
+    const int piece_row = wn * MINE + lane / P::PLACES, piece_place = lane % P::PLACES;
     const uint8_t *rec[NT];
 #pragma unroll
     for (int j = 0; j < NT; ++j) rec[j] = a.w + (size_t)min(tile0 + j, tiles - 1) * a.blocks * a.record;
@@ -442,37 +448,54 @@ __global__ __launch_bounds__(512, 2) void w4_dense_shared_kernel(const W4Args a)
     for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0, 0, 0, 0};
+    unsigned char *xs = smem + wk * 2 * TILE;
+    S *totals = reinterpret_cast<S *>(smem + WK * 2 * TILE) + wk * 2 * PER * ROWS;
     u32x4 x[2][N];
     Block<X, GROUP, MT, NT> b[2];
     const uint32_t full = a.K / W4_TK;         // blocks that no row ends in; loads of these are never behind a branch: a wait after one would be for all of them
     auto x_row = [&](int i) { return (const E *)a.x + (uint64_t)min(m0 + i * STEP + piece_row, a.M - 1) * a.x_stride; };
-    auto load = [&](u32x4 (&v)[N], Block<X, GROUP, MT, NT> &w, uint32_t block) {
-        w.load_w(a, rec, (size_t)block * a.record, lane);
+    auto nth = [&](uint32_t r) { return min(r * WK + wk, full - 1); };              // (past the end the last one once more: not used)
+    auto load_w = [&](Block<X, GROUP, MT, NT> &w, uint32_t r) { w.load_w(a, rec, (size_t)nth(r) * a.record, lane); };
+    auto load_x = [&](u32x4 (&v)[N], uint32_t r) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = P::load(x_row(i), block * W4_TK, piece_place);
+        for (int i = 0; i < N; ++i) v[i] = P::load(x_row(i), nth(r) * W4_TK, piece_place);
     };
-    auto store = [&](const u32x4 (&v)[N], unsigned char *xs) {
+    auto store = [&](const u32x4 (&v)[N], int half) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) P::store(xs, i * STEP + piece_row, piece_place, v[i]);
+        for (int i = 0; i < N; ++i) P::store(xs + half * TILE, i * STEP + piece_row, piece_place, v[i]);
+#pragma unroll
+        for (int c = 0; c < MINE; c += COLS)
+#pragma unroll
+            for (int g = 0; g < PER; ++g) {
+                V sum = V{0, 0, 0, 0};
+#pragma unroll
+                for (int s = g * GROUP / 32; s < (g + 1) * GROUP / 32; ++s) sum = mma<X>(w_ones<X>(), P::fragment(xs + half * TILE, wn * MINE + c + lane % COLS, s, lane >> 4), sum);
+                if (lane < COLS) totals[(half * PER + g) * ROWS + wn * MINE + c + lane] = sum[0];
+            }
     };
-    unsigned char *mine = smem + wk * 2 * TILE;
-    auto multiply = [&](const Block<X, GROUP, MT, NT> &w, const unsigned char *xs) {
-        w.multiply(a, acc, [&](int s, int i) { return P::fragment(xs, i * 16 + (lane & 15), s, lane >> 4); });
+    auto multiply = [&](const Block<X, GROUP, MT, NT> &w, int half) {
+        w.multiply(a, acc, [&](int s, int i) { return P::fragment(xs + half * TILE, i * 16 + (lane & 15), s, lane >> 4); },
+                   [&](int g, int i) { return totals[(half * PER + g) * ROWS + i * 16 + (lane & 15)]; });
     };
-    auto round = [&](u32x4 (&v)[N], Block<X, GROUP, MT, NT> &w, unsigned char *xs, uint32_t block) {
-        store(v, xs);
+    auto round = [&](u32x4 (&next)[N], Block<X, GROUP, MT, NT> &w, int half, uint32_t r) {
         __syncthreads();
         const Block<X, GROUP, MT, NT> cur = w;
-        load(v, w, min(block + 2 * WK, full - 1));              // (past the end the last one once more: not used)
-        if (block < full) multiply(cur, xs);
+        load_w(w, r + 2);
+        store(next, half ^ 1);
+        load_x(next, r + 3);
+        if (r * WK + wk < full) multiply(cur, half);
     };
     if (full) {
-        load(x[0], b[0], min((uint32_t)wk, full - 1));
-        load(x[1], b[1], min((uint32_t)wk + WK, full - 1));
+        load_x(x[0], 0);
+        load_w(b[0], 0);
+        load_x(x[1], 1);
+        load_w(b[1], 1);
+        store(x[0], 0);
+        load_x(x[0], 2);
         const uint32_t rounds = (full + WK - 1) / WK;
         for (uint32_t r = 0; r < rounds; r += 2) {
-            round(x[0], b[0], mine, r * WK + wk);
-            round(x[1], b[1], mine + TILE, (r + 1) * WK + wk);
+            round(x[1], b[0], 0, r);
+            round(x[0], b[1], 1, r + 1);
         }
     }
     if (full < a.blocks) {
@@ -481,10 +504,10 @@ __global__ __launch_bounds__(512, 2) void w4_dense_shared_kernel(const W4Args a)
             b[0].load_w(a, rec, (size_t)full * a.record, lane);
 #pragma unroll
             for (int i = 0; i < N; ++i) x[0][i] = P::load_part(x_row(i), full * W4_TK, piece_place, a.K);
-            store(x[0], mine);              // (the last round read the other half)
+            store(x[0], 0);              // (the last round read the other half)
         }
         __syncthreads();
-        if (turn) multiply(b[0], mine);
+        if (turn) multiply(b[0], 0);
     }
     __syncthreads();
     finish<X, MT, NT>(a, acc, reinterpret_cast<float *>(smem) + wn * WK * NT * MT * 256, wk, WK, wk * 64 + lane, WK * 64, m0, tile0, lane);
@@ -513,7 +536,7 @@ static int launch_w4(const W4Args &a, uint32_t tiles, int cus, hipStream_t st) {
     if constexpr (X == W4_F32) return own(w4_dense_kernel<X, GROUP, 2, 1, 1, false>, 2);           // (three parts of each value: registers for no more)
     else {
         auto shared = [&](auto kern, uint32_t mt, uint32_t wn) -> int {
-            const size_t x = (size_t)(8 / wn) * 2 * mt * 16 * Piece<X>::ROW, sums = (size_t)8 * 2 * mt * 1024, lds = x > sums ? x : sums;
+            const size_t x = (size_t)(8 / wn) * 2 * mt * 16 * (Piece<X>::ROW + W4_TK / GROUP * 4), sums = (size_t)8 * 2 * mt * 1024, lds = x > sums ? x : sums;
             SHODH_TRY(ensure_dynamic_lds((const void *)kern, lds));
             hipLaunchKernelGGL(kern, dim3((tiles + 2 * wn - 1) / (2 * wn), (a.M + 16 * mt - 1) / (16 * mt)), dim3(512), lds, st, a);
             SHODH_HIP_TRY(hipGetLastError());
