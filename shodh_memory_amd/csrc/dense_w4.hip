@@ -363,7 +363,7 @@ __device__ __forceinline__ void finish(const W4Args &a, const f32x4 (&acc)[NT][M
 // outputs 4 (lane >> 4) .. + 3. U blocks are asked for before the first is multiplied; with U = 1 the next one is on its way meanwhile.
 // FEW: there are no more rows than one piece a lane covers (2, 4 or 8 by type): the others' columns hold whatever LDS held, and are not written.
 template <int X, int GROUP, int MT, int NT, int U, bool FEW>
-__global__ __launch_bounds__(512, FEW && GROUP != 32 ? 6 : MT == 1 ? 4 : 2) void w4_dense_kernel(const W4Args a) {
+__global__ __launch_bounds__(512, FEW && GROUP != 32 ? 6 : MT == 1 && (FEW || X != W4_F32 || GROUP == 128) ? 4 : 2) void w4_dense_kernel(const W4Args a) {
     using P = Piece<X>;
     using E = typename P::E;
     constexpr int STEP = 64 / P::PLACES, PIECES = FEW ? 1 : MT * 16 / STEP, TILE = MT * 16 * P::ROW;         // rows between a lane's pieces of a block, their number
@@ -513,13 +513,15 @@ __global__ __launch_bounds__(512, 2) void w4_dense_shared_kernel(const W4Args a)
     finish<X, MT, NT>(a, acc, reinterpret_cast<float *>(smem) + wn * WK * NT * MT * 256, wk, WK, wk * 64 + lane, WK * 64, m0, tile0, lane);
 }
 
-// Which kernel. Measured at 4096 inputs, group 128, bf16 (us; weights cold):
-//   rows that one piece a lane covers (4 in 16 bits): 4096 outputs 5.3, 14336 outputs 10.8 (all rows' pieces loaded: 9.1 and 29);  16 rows: 6.2 and 16
-//   64 rows:  outputs    4096   8192  14336  28672         32 rows:  4096   8192  14336  28672
-//     own pieces         13.1   15.5   29.3   53.5                    8.3   11.0   20.1   35.8
-//     shared by 2 waves  22.8   23.2   25.8   48.8                   16.5   16.7   19.4   36.1
-//     shared by 4 waves  36.8   37.0   41.2   42.4                   27.4   27.5   32.0   33.0
-// Sharing pays once there are workgroups for every CU all the same: 4 waves x 32 outputs at 7 x 16 outputs a CU, 2 waves at half of that.
+// Which kernel. Up to 16 rows own pieces; measured at 4096 inputs, group 128, bf16 (us; weights cold): rows that one piece a lane covers (4 in 16 bits),
+// 4096 outputs 5.3, 14336 outputs 10.8 (all rows' pieces loaded: 9.1 and 29); 16 rows: 6.2 and 16. Beyond them the workgroups are counted in rounds over
+// the CUs, a round of each kernel by what it takes. Measured there (us):
+//   rows x outputs     32 x 4096   7168  10240  14336  20480  28672    64 x 4096   7168  10240  14336  20480  28672    256 x 4096  14336  28672
+//     own pieces             7.9   11.5   14.8   23.1   25.5   38.3         11.6   20.1   27.4   39.0   47.2   66.5          37.7  123.6  242.8
+//     shared by 2 waves     12.4   12.6   12.5   14.4   24.4   25.9         18.7   18.8   19.0   21.0   37.1   39.1          19.6   72.0  128.8
+//     shared by 4 waves     18.8   18.7   18.6   19.7   19.5   20.6         25.7   25.9   25.9   26.6   26.7   27.9          25.8   51.6  100.8
+//   int8 rows: 64 x 7168 15.7 / 17.7 / 29.1; 64 x 28672 51.3 / 35.5 / 30.7; 256 x 10240 62.6 / 49.7 / 56.7
+// At 1024 inputs the order is the same. Groups of 32 (64 rows, 28672 outputs): 90 / - / 55, of 64: 81 / 47 / 38.
 template <int X, int GROUP>
 static int launch_w4(const W4Args &a, uint32_t tiles, int cus, hipStream_t st) {
     auto own = [&](auto kern, uint32_t mt) -> int {
@@ -542,14 +544,18 @@ static int launch_w4(const W4Args &a, uint32_t tiles, int cus, hipStream_t st) {
             SHODH_HIP_TRY(hipGetLastError());
             return SHODH_OK;
         };
-        const bool four = 2 * tiles >= 14u * (uint32_t)cus, two = 2 * tiles >= 7u * (uint32_t)cus;
-        if (a.M <= 32) return four ? shared(w4_dense_shared_kernel<X, GROUP, 2, 4, 2>, 2, 4) : two ? shared(w4_dense_shared_kernel<X, GROUP, 2, 2, 4>, 2, 2)
-                                   : own(w4_dense_kernel<X, GROUP, 2, 1, 1, false>, 2);
-        if constexpr (GROUP > 32) {            // (four scales a record, two records, 64 rows: registers spill)
-            if (four) return shared(w4_dense_shared_kernel<X, GROUP, 4, 4, 2>, 4, 4);
-            if (two) return shared(w4_dense_shared_kernel<X, GROUP, 4, 2, 4>, 4, 2);
-        }
-        return own(w4_dense_kernel<X, GROUP, 4, 1, 1, false>, 4);
+        const uint32_t mt = a.M <= 32 ? 2 : 4, row_tiles = (a.M + 16 * mt - 1) / (16 * mt);
+        auto cost = [&](uint32_t per /* tiles of a workgroup */, uint32_t round) { return (((uint64_t)(tiles + per - 1) / per * row_tiles + cus - 1) / cus) * round; };
+        constexpr uint32_t TWO = X == W4_I8 ? (GROUP == 128 ? 8 : GROUP == 64 ? 10 : 14) : (GROUP == 128 ? 7 : GROUP == 64 ? 8 : 12);
+        constexpr uint32_t FOUR = X == W4_I8 ? (GROUP == 128 ? 13 : GROUP == 64 ? 16 : 23) : (GROUP == 128 ? 10 : GROUP == 64 ? 12 : 16);
+        const uint64_t one = cost(1, mt == 2 ? 3 : 4), two = GROUP == 32 && mt == 4 ? ~0ull /* (its registers spill) */ : cost(4, TWO), four = cost(8, FOUR);
+        auto pick = [&](auto MT) -> int {
+            if (one <= two && one <= four) return own(w4_dense_kernel<X, GROUP, MT.value, 1, 1, false>, MT.value);
+            if constexpr (GROUP > 32 || MT.value == 2)
+                if (two <= four) return shared(w4_dense_shared_kernel<X, GROUP, MT.value, 2, 4>, MT.value, 2);
+            return shared(w4_dense_shared_kernel<X, GROUP, MT.value, 4, 2>, MT.value, 4);
+        };
+        return mt == 2 ? pick(std::integral_constant<int, 2>{}) : pick(std::integral_constant<int, 4>{});
     }
 }
 template <int X>
