@@ -546,12 +546,12 @@ static int launch_w4(const W4Args &a, uint32_t tiles, int cus, hipStream_t st) {
         };
         const uint32_t mt = a.M <= 32 ? 2 : 4, row_tiles = (a.M + 16 * mt - 1) / (16 * mt);
         auto cost = [&](uint32_t per /* tiles of a workgroup */, uint32_t round) { return (((uint64_t)(tiles + per - 1) / per * row_tiles + cus - 1) / cus) * round; };
-        constexpr uint32_t TWO = X == W4_I8 ? (GROUP == 128 ? 8 : GROUP == 64 ? 10 : 14) : (GROUP == 128 ? 7 : GROUP == 64 ? 8 : 12);
+        constexpr uint32_t TWO = X == W4_I8 ? (GROUP == 128 ? 8 : 10) : (GROUP == 128 ? 7 : 8);
         constexpr uint32_t FOUR = X == W4_I8 ? (GROUP == 128 ? 13 : GROUP == 64 ? 16 : 23) : (GROUP == 128 ? 10 : GROUP == 64 ? 12 : 16);
-        const uint64_t one = cost(1, mt == 2 ? 3 : 4), two = GROUP == 32 && mt == 4 ? ~0ull /* (its registers spill) */ : cost(4, TWO), four = cost(8, FOUR);
+        const uint64_t one = cost(1, mt == 2 ? 3 : 4), two = GROUP == 32 ? ~0ull /* (12 or more: never the least) */ : cost(4, TWO), four = cost(8, FOUR);
         auto pick = [&](auto MT) -> int {
             if (one <= two && one <= four) return own(w4_dense_kernel<X, GROUP, MT.value, 1, 1, false>, MT.value);
-            if constexpr (GROUP > 32 || MT.value == 2)
+            if constexpr (GROUP > 32)
                 if (two <= four) return shared(w4_dense_shared_kernel<X, GROUP, MT.value, 2, 4>, MT.value, 2);
             return shared(w4_dense_shared_kernel<X, GROUP, MT.value, 4, 2>, MT.value, 4);
         };

@@ -83,6 +83,37 @@ def test_against_the_definition(layers, kind, group):
             w.close()
 
 
+# many outputs and rows: the kernels that share a block of rows among 2 or 4 waves (by rows, outputs and type), with whole blocks of 128 inputs in odd and even
+# numbers, a part of a block behind them, and nothing but a part
+MANY = [(20, 10000, 384), (20, 17000, 257), (32, 30000, 129), (33, 5000, 1408), (64, 9000, 700), (49, 17000, 513), (64, 30001, 100), (130, 5003, 300), (257, 2050, 1157)]
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16", "int8"])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_many_rows_and_outputs(layers, kind, group):
+    for i, (m, n, k) in enumerate(MANY):
+        zeros = bool((i + group // 32) % 2)
+        q, packed, scale, z = make(n, k, group, zeros, 11 * i + group)
+        w = layers.W4Weight.from_quantized(packed, scale, z, k=k, group=group, scale_dtype=torch.float16)
+        x, xs = rows_of(kind, m, k + 3, i)
+        x = x[:, 3:]                               # a stride of its own, no alignment
+        bias = torch.randn(n, device="cuda") if i % 2 else None
+        out = torch.full((m + 1, n + 5), 7.0, device="cuda")
+        w.dense(x, x_scale=xs, bias=bias, out=out[:m, :n])
+        assert (out[m] == 7).all() and (out[:, n:] == 7).all()
+        y, t = exact(x, xs, q, scale, z, bias, group)
+        check(out[:m, :n], y, t, x.dtype, k, group)
+        if kind != "int8":
+            x = x.clone()
+            clean = w.dense(x)
+            x[m // 2, k - 1] = float("nan")
+            got = w.dense(x)
+            assert torch.isnan(got[m // 2]).all()
+            keep = torch.arange(m, device="cuda") != m // 2
+            assert torch.equal(got[keep], clean[keep])
+        w.close()
+
+
 def test_host_data_and_dequantize(layers):
     q, packed, scale, z = make(37, 200, 64, True, 3, device="cpu")
     want = (q.double() - z.double()[:, torch.arange(200) // 64]) * scale.double()[:, torch.arange(200) // 64]
