@@ -460,7 +460,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs a) {
     const uint32_t items = gridDim.x;
     // neighbouring items (tiles of one key head) on one XCD: it takes every eighth workgroup
     const uint32_t per = items / 8, xcd = blockIdx.x & 7, item = blockIdx.x < per * 8 ? xcd * per + (blockIdx.x >> 3) : blockIdx.x;
-    const uint32_t kvh = item / a.slots, slot = item % a.slots;
+    const uint32_t kvh = item / a.slots, slot = a.slots - 1 - item % a.slots;          // later tiles, that tend to see more keys, first: 8192 tokens 292 -> 286 us, 96 texts 22.9 -> 21.2
     int t0, t1;
     const int b = find_seq(a, slot, BM, t0, t1);
     const Seq s = seq_of(a, b, t0, t1);
