@@ -1,6 +1,7 @@
 """Layer operators of a text tower on torch device tensors, over the C ABI (include/shodh_hip.h, "layer operators"): RMS norm with residual and 8-bit
 output, dense layers on 4-bit weights, attention with a sliding window and always-visible first tokens. They run on the tensors' device, on its
-current stream unless `stream` names another (a raw hipStream_t), and can be captured into a graph. Nothing here computes on the host."""
+current stream unless `stream` names another (a raw hipStream_t, made the current one for the call: new tensors are that stream's), and can be captured
+into a graph. They are for inference: results carry no gradients. Nothing here computes on the host."""
 import collections
 import ctypes as C
 import functools
@@ -34,10 +35,15 @@ def _on(t, device, name):
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)         # (0.1 us; the Stream object of the line below takes 2 us to make)
 
 
-def _stream(device, stream):
-    if stream is not None:
-        return stream
+def _stream(device):
     return _raw_stream(device.index) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
+
+
+def _current(stream, device):
+    """`stream` as the current one for a call"""
+    if device.type != "cuda":
+        _refuse("a stream for tensors on %s" % device)
+    return torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device))
 
 
 def _matrix(t, name):
@@ -67,6 +73,9 @@ def rms_norm(x, weight, eps=1e-6, residual=None, want_y=True, quant=None, group=
     -> RmsNorm(y, q, scale, sum): what was not asked for is None; sum (with a residual) = h in x's type, written to `sum_out` (it may be
     `residual` itself: in place) or a new tensor; scale f32 [rows, groups]."""
     device = x.device
+    if stream is not None:
+        with _current(stream, device):
+            return rms_norm(x, weight, eps, residual, want_y, quant, group, sum_out)
     if device.type != "cuda":
         _refuse("x is on %s: there is no CPU fallback" % device, L.ERR_DEVICE)
     dt = _dtype(x, "x")
@@ -106,7 +115,7 @@ def rms_norm(x, weight, eps=1e-6, residual=None, want_y=True, quant=None, group=
     cfg = L.RmsNormCfg(rows, xs, rs, ss, 0, 0, dim, dt, wd, qd, group, eps)
     L.check(L.lib().shodh_rms_norm_device(device.index, C.byref(cfg), x.data_ptr(), residual.data_ptr() if residual is not None else None, weight.data_ptr(),
                                           total.data_ptr() if total is not None else None, y.data_ptr() if want_y else None,
-                                          q.data_ptr() if q is not None else None, scale.data_ptr() if q is not None else None, _stream(device, stream)))
+                                          q.data_ptr() if q is not None else None, scale.data_ptr() if q is not None else None, _stream(device)))
     return RmsNorm(y, q, scale, total)
 
 
@@ -162,7 +171,7 @@ class W4Weight:
         zeros = None if zeros is None else zeros.contiguous()
         h, zp = C.c_void_p(), zeros.data_ptr() if zeros is not None else None
         if q.device.type == "cuda":
-            L.check(L.lib().shodh_w4_weight_create_device(q.device.index, q.data_ptr(), scale.data_ptr(), zp, n, k, group, sd, _stream(q.device, None), C.byref(h)))
+            L.check(L.lib().shodh_w4_weight_create_device(q.device.index, q.data_ptr(), scale.data_ptr(), zp, n, k, group, sd, _stream(q.device), C.byref(h)))
             return cls(h, q.device)
         L.check(L.lib().shodh_w4_weight_create(int(device), q.data_ptr(), scale.data_ptr(), zp, n, k, group, sd, C.byref(h)))
         return cls(h, torch.device("cuda", int(device)))
@@ -178,6 +187,9 @@ class W4Weight:
         the result is of x's type (bf16 for int8 rows) unless out_dtype or `out` says otherwise."""
         if self._h is None:
             _refuse("the weight is closed", L.ERR_STATE)
+        if stream is not None:
+            with _current(stream, self.device):
+                return self.dense(x, x_scale, bias, out_dtype, out)
         rows, k, xs = _matrix(x, "x")
         if k != self.k:
             _refuse("x has %d columns, the weight %d inputs" % (k, self.k), L.ERR_DIM)
@@ -210,7 +222,7 @@ class W4Weight:
         if rows == 0:
             return out
         L.check(L.lib().shodh_w4_dense_device(self._h, x.data_ptr(), xd, xs, sp, rows, bp, out.data_ptr(), _dtype(out, "out"), os_,
-                                              _stream(self.device, stream)))
+                                              _stream(self.device)))
         return out
 
     def close(self):
@@ -260,6 +272,9 @@ def window_attention(q, k, v, cu, left=-1, right=-1, sinks=0, kv_start=None, kv_
     bound is none; causal: right=0. bf16 or fp16, head_dim a multiple of 8 up to 128, any strides of tokens and heads.
     -> out like q (and with return_lse the log of the sum of exponentials, f32 [tokens, heads]); tokens behind cu[-1] are left as they were."""
     device = q.device
+    if stream is not None:
+        with _current(stream, device):
+            return window_attention(q, k, v, cu, left, right, sinks, kv_start, kv_len, scale, return_lse, out)
     if device.type != "cuda":
         _refuse("q is on %s: there is no CPU fallback" % device, L.ERR_DEVICE)
     dt = _dtype(q, "q")
@@ -295,9 +310,7 @@ def window_attention(q, k, v, cu, left=-1, right=-1, sinks=0, kv_start=None, kv_
         cfg = L.AttentionCfg(n, kn, qs, qh, ks, kh, vs, vh, os_, oh, dt, heads, kv_heads, dim, seqs, sinks, left, right, scale or 0.0, 0)
         need = _attention_workspace(device.index, n, kn, dt, heads, kv_heads, dim, seqs, sinks, left, right)
         work = q.new_empty(need, dtype=torch.uint8) if need else None
-        st = _stream(device, stream)
-        if work is not None and stream is not None:
-            work.record_stream(torch.cuda.ExternalStream(stream, device=device))
         L.check(L.lib().shodh_window_attention_device(device.index, C.byref(cfg), q.data_ptr(), k.data_ptr(), v.data_ptr(), cup, sp, lp, out.data_ptr(),
-                                                      lse.data_ptr() if return_lse else None, work.data_ptr() if work is not None else None, need, st))
+                                                      lse.data_ptr() if return_lse else None, work.data_ptr() if work is not None else None, need,
+                                                      _stream(device)))
     return (out, lse) if return_lse else out

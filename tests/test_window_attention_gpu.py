@@ -230,6 +230,52 @@ def test_bad_descriptors_stay_in_bounds(layers):
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("seqs", [65, 256, 300, 4200])
+def test_many_sequences(layers, seqs):
+    """ragged texts, and single tokens over caches: more sequences than one load of cu, than one round of its search, than one table of parts"""
+    g = torch.Generator().manual_seed(seqs)
+    most = 6 if seqs > 1000 else 80
+    nq = [int(n) for n in torch.randint(0, most, (seqs,), generator=g)]
+    nq[seqs // 2], nq[-1] = 140, 0
+    q, k, v = normal(30, sum(nq), 2, 32).bfloat16(), normal(31, sum(nq), 1, 32).bfloat16(), normal(32, sum(nq), 1, 32).bfloat16()
+    out, lse = layers.window_attention(q, k, v, cu_of(nq), left=20, right=3, sinks=2, return_lse=True)
+    check(out, lse, exact(q, k, v, nq, nq, 20, 3, 2))
+    nk = [int(n) for n in torch.randint(0, most, (seqs,), generator=g)]
+    nk[1], nk[seqs // 3], nk[-2] = 2500, 0, 900
+    nq = [int(n) for n in torch.randint(0, 3, (seqs,), generator=g)]
+    starts = [sum(nk[:i]) for i in range(seqs)]
+    q, k, v = normal(33, sum(nq), 2, 32).half(), normal(34, sum(nk), 1, 32).half(), normal(35, sum(nk), 1, 32).half()
+    for left in (-1, 700):
+        out, lse = layers.window_attention(q, k, v, cu_of(nq), left=left, right=0, sinks=3, kv_start=torch.tensor(starts, device="cuda"),
+                                           kv_len=torch.tensor(nk, dtype=torch.int32, device="cuda"), return_lse=True)
+        check(out, lse, exact(q, k, v, nq, nk, left, 0, 3, starts))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("dim", [32, 56, 64, 128])
+@pytest.mark.parametrize("nq,nk", [([150, 1, 40], [150, 1, 40]), ([1, 3], [700, 260])])
+def test_odd_places(layers, dtype, dim, nq, nk):
+    """q, k and v at places and distances that are no multiples of 16 bytes, in both forms"""
+    starts = [sum(nk[:i]) + i for i in range(len(nk))]
+    t = TYPES[dtype]
+    q = normal(36, sum(nq), 4, dim + 3).to(t)[:, :, 1:1 + dim]
+    k, v = normal(37, sum(nk) + 3, 2, dim + 5).to(t)[:, :, 3:3 + dim], normal(38, sum(nk) + 3, 2, 2 * dim + 1).to(t)[:, :, dim:2 * dim]
+    for left, right, sinks in [(-1, 0, 0), (60, 0, 3), (33, 10, 0)]:
+        out, lse = layers.window_attention(q, k, v, cu_of(nq), left=left, right=right, sinks=sinks, kv_start=torch.tensor(starts, device="cuda"),
+                                           kv_len=torch.tensor(nk, dtype=torch.int32, device="cuda"), return_lse=True)
+        check(out, lse, exact(q, k, v, nq, nk, left, right, sinks, starts))
+
+
+def test_a_cache_in_many_parts(layers):
+    nk = [60000, 1, 33333]
+    starts = [0, 60000, 60001]
+    q, k, v = normal(39, 4, 8, 64).bfloat16(), normal(40, sum(nk), 1, 64).bfloat16(), normal(41, sum(nk), 1, 64).bfloat16()
+    for left in (-1, 50000):
+        out, lse = layers.window_attention(q, k, v, cu_of([1, 1, 2]), left=left, right=0, sinks=5, kv_start=torch.tensor(starts, device="cuda"),
+                                           kv_len=torch.tensor(nk, dtype=torch.int32, device="cuda"), return_lse=True)
+        check(out, lse, exact(q, k, v, [1, 1, 2], nk, left, 0, 5, starts))
+
+
 def test_streams_and_two_graphs(layers):
     """two captured graphs and eager calls in between, with lengths that change from replay to replay"""
     q = normal(26, 2, 8, 64).bfloat16()
