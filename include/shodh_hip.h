@@ -437,7 +437,7 @@ int shodh_rms_norm_device(int device, const shodh_rms_norm_cfg *cfg, const void 
  * A weight is laid out once; the handle is read-only afterwards (any number of calls at once). q: [N][ceil(K / 2)] bytes, two inputs a byte, the even one
  * in the low bits; scale f32 [N][ceil(K / group)], kept in `scale_dtype` (fp16 or bf16: values that are numbers of that type already stay what they
  * are); zero [N][ceil(K / group)] bytes 0 .. 15, NULL = 8 everywhere. group 32, 64 or 128; N and K any.
- * _create takes host data, _create_device device data (both wait for the device: not for captured streams); _quantize rounds f32 weights itself:
+ * _create takes host data, _create_device device data (both wait for the device and are refused while `stream` is captured); _quantize rounds f32 weights itself:
  * per group scale = max |w| / 7, or (max - min) / 15 with zero points. */
 typedef struct shodh_w4_weight shodh_w4_weight;
 int shodh_w4_weight_create(int device, const uint8_t *q, const float *scale, const uint8_t *zero, uint32_t N, uint32_t K, uint32_t group,
@@ -451,7 +451,7 @@ int shodh_w4_weight_dequantize(const shodh_w4_weight *w, float *out /* host [N][
 int shodh_w4_weight_shape(const shodh_w4_weight *w, uint32_t *N, uint32_t *K, uint32_t *group, uint64_t *bytes);
 /* x [rows][K]: fp32 (exact: three bf16 parts), bf16, fp16, or int8 with one f32 scale a row (what shodh_rms_norm_device writes with q_group 0; sums exact in
  * int32 per group); bias f32 [N] or NULL; y [rows][N] fp32, bf16 or fp16. Any number of rows (made for up to 64: beyond, the weights are read again
- * for each 64). A row that holds a NaN or an infinity gives NaN in all its outputs; f32 and bf16 rows are taken up to a sum |x| * 31 in f32's range. */
+ * for each 64). y may not overlap x. A row that holds a NaN or an infinity gives NaN in all its outputs; f32 and bf16 rows are taken up to a sum |x| * 31 in f32's range. */
 int shodh_w4_dense_device(const shodh_w4_weight *w, const void *d_x, uint32_t x_dtype, uint64_t x_stride, const float *d_x_scale, uint32_t rows,
                           const float *d_bias, void *d_y, uint32_t y_dtype, uint64_t y_stride, void *stream);
 
@@ -464,7 +464,7 @@ int shodh_w4_dense_device(const shodh_w4_weight *w, const void *d_x, uint32_t x_
  * -inf. What masked keys hold (NaN, infinities) does not matter. Rows of out and lse behind the last sequence are left as they were; a sequence whose
  * kv range does not lie in [0, kv_tokens) has no keys; what is written for one whose cu is out of order or range is undefined, within out and lse.
  * q [q_tokens][heads][head_dim], k and v [kv_tokens][kv_heads][head_dim], out like q: any token and head strides. Query head h reads key head
- * h * kv_heads / heads. Statistics and sums are f32; probabilities are multiplied in the inputs' 16-bit type.
+ * h * kv_heads / heads. Lengths up to 2^31 - 256 keys (longer: none is seen). out may be q, and overlaps neither k nor v. Statistics and sums are f32; probabilities are multiplied in the inputs' 16-bit type.
  * The workspace (shodh_window_attention_workspace bytes, may be 0; a multiple of 16) belongs to one call until that call's work is done. */
 typedef struct {
     uint64_t q_tokens, kv_tokens;                /* rows of q and of k and v, all sequences */

@@ -621,6 +621,9 @@ int shodh_w4_weight_create_device(int device, const uint8_t *d_q, const float *d
     if (!d_q || !d_scale) { set_error("null argument"); return SHODH_ERR_INVALID; }
     DeviceScope scope;
     SHODH_TRY(scope.enter(device));
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    SHODH_HIP_TRY(hipStreamIsCapturing((hipStream_t)stream, &capture));
+    if (capture != hipStreamCaptureStatusNone) { set_error("w4: weights are not laid out while their stream is captured"); return SHODH_ERR_STATE; }
     try {
         Buffers b;
         uint32_t *bad = b.take<uint32_t>(1);

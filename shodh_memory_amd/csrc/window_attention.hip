@@ -127,6 +127,7 @@ __device__ __forceinline__ int find_seq(const AttnArgs &a, int64_t slot, int bm,
 __device__ __forceinline__ int64_t uniform64(int64_t x) {       // a number that all lanes hold alike, in scalar registers
     return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)x));
 }
+constexpr int MOST_KEYS = 0x7FFFFF00;          // (a place behind the last tile is a number too)
 struct Seq {
     int64_t q0, k0;
     int nq, nk;
@@ -137,7 +138,7 @@ __device__ __forceinline__ Seq seq_at(const AttnArgs &a, int b, int64_t t0, int6
     s.q0 = t0; s.nq = (int)(t1 - t0);
     if (a.kv_start) {
         s.k0 = a.kv_start[b]; s.nk = a.kv_len[b];
-        if (s.k0 < 0 || s.nk < 0 || s.k0 > a.kv_tokens || s.nk > a.kv_tokens - s.k0) { s.k0 = 0; s.nk = 0; }      // no such keys: none is seen
+        if (s.k0 < 0 || s.nk < 0 || s.k0 > a.kv_tokens || s.nk > a.kv_tokens - s.k0 || s.nk > MOST_KEYS) { s.k0 = 0; s.nk = 0; }      // no such keys: none is seen
     } else { s.k0 = t0; s.nk = s.nq; }
     return s;
 }
@@ -805,8 +806,8 @@ static int check_attention(const shodh_attention_cfg *c) {
     if (c->dtype != SHODH_DTYPE_BF16 && c->dtype != SHODH_DTYPE_FP16) { set_error("attention: dtype %u is neither bf16 nor fp16", c->dtype); return SHODH_ERR_UNSUPPORTED; }
     if (c->heads == 0 || c->kv_heads == 0 || c->heads % c->kv_heads != 0) { set_error("attention: %u heads over %u key heads", c->heads, c->kv_heads); return SHODH_ERR_INVALID; }
     if (c->head_dim == 0 || c->head_dim % 8 != 0 || c->head_dim > 128) { set_error("attention: head_dim %u is no multiple of 8 up to 128", c->head_dim); return SHODH_ERR_UNSUPPORTED; }
-    if (!(c->scale == c->scale) || c->scale > 3.0e38f || c->scale < -3.0e38f) { set_error("attention: scale is no number"); return SHODH_ERR_INVALID; }
-    if (c->q_tokens > 0x7FFFFFFFull / (c->heads / c->kv_heads) || c->kv_tokens > (1ull << 40) || c->heads > 65535u || c->seqs > 0x3FFFFFFFu || c->sinks > 0x7FFFFFFFu) { set_error("attention: a size is out of range"); return SHODH_ERR_UNSUPPORTED; }
+    if (!(c->scale == c->scale) || c->scale > 2.0e38f || c->scale < -2.0e38f /* (times log2 e, in f32) */) { set_error("attention: scale is no number, or too large"); return SHODH_ERR_INVALID; }
+    if (c->q_tokens > (uint64_t)MOST_KEYS / (c->heads / c->kv_heads) || c->kv_tokens > (1ull << 40) || c->heads > 65535u || c->seqs > 0x3FFFFFFFu || c->sinks > 0x7FFFFFFFu) { set_error("attention: a size is out of range"); return SHODH_ERR_UNSUPPORTED; }
     if (c->q_tokens * (c->heads / c->kv_heads) / 32 + c->seqs > 0x7FFFFFFFull / c->kv_heads) { set_error("attention: too many rows for one launch"); return SHODH_ERR_UNSUPPORTED; }
     return SHODH_OK;
 }

@@ -9,6 +9,8 @@ import numpy as np
 import pytest
 import torch
 
+from .conftest import needs_capture
+
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -23
 TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
@@ -187,6 +189,7 @@ def test_f32_rows_keep_their_24_bits(layers):
     assert (got - torch.diag(got.diagonal())).abs().max() <= 48 * U * v.abs().max()
 
 
+@needs_capture
 def test_streams_threads_and_graph(layers):
     import threading
     q, packed, scale, z = make(300, 1024, 128, True, 4)
@@ -217,6 +220,24 @@ def test_streams_threads_and_graph(layers):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(held, want[k]), k
+
+
+@needs_capture
+def test_a_captured_stream_lays_out_no_weights(layers):
+    from shodh_memory_amd import ShodhError
+    q, packed, scale, z = make(64, 128, 64, True, 6)
+    w = layers.W4Weight.from_quantized(packed, scale, z, group=64)
+    x = torch.randn(2, 128, device="cuda").half()
+    want = w.dense(x)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = w.dense(x)
+        with pytest.raises(ShodhError):
+            layers.W4Weight.from_quantized(packed, scale, z, group=64)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(held, want)
 
 
 def test_refusals(layers):

@@ -7,6 +7,7 @@ import torch
 from . import test_dense_w4_gpu as W4
 from . import test_rms_norm_gpu as NORM
 from . import test_window_attention_gpu as ATTN
+from .conftest import needs_capture
 
 pytestmark = pytest.mark.gpu
 HEADS, KV, DIM, HIDDEN, UP = 6, 2, 64, 392, 1000
@@ -76,8 +77,9 @@ def parts(qkv):
     return qkv[:, :HEADS], qkv[:, HEADS:HEADS + KV], qkv[:, HEADS + KV:]
 
 
+@pytest.mark.parametrize("captured", [False, pytest.param(True, marks=needs_capture)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-def test_a_block_on_texts_then_on_single_tokens(layers, dtype):
+def test_a_block_on_texts_then_on_single_tokens(layers, dtype, captured):
     block = Block(layers, dtype)
     nq, left, sinks = [70, 1, 150, 0, 33], 40, 3
     tokens, room = sum(nq), 8
@@ -86,7 +88,7 @@ def test_a_block_on_texts_then_on_single_tokens(layers, dtype):
     s = block(x, lambda qkv: layers.window_attention(*parts(qkv), cu, left=left, right=0, sinks=sinks, return_lse=True))
     block.check(s, lambda qkv: ATTN.exact(*parts(qkv), nq, nq, left, 0, sinks))
 
-    # the texts' keys and values become a cache with room behind each; every sequence goes on by one token a step, the step captured once
+    # the texts' keys and values become a cache with room behind each; every sequence goes on by one token a step (the step captured once, or not)
     starts = [sum(nq[:i]) + room * i for i in range(len(nq))]
     total = tokens + room * len(nq)
     ck, cv = (torch.full((total, KV, DIM), float("nan"), device="cuda", dtype=dtype) for _ in range(2))
@@ -105,15 +107,19 @@ def test_a_block_on_texts_then_on_single_tokens(layers, dtype):
         ck.index_copy_(0, place, k)
         cv.index_copy_(0, place, v)
         return layers.window_attention(q, ck, cv, one, left=left, right=0, sinks=sinks, kv_start=start, kv_len=length + 1, return_lse=True)
-    block(xt, attend)                     # (written over by the first step)
-    torch.cuda.synchronize()
-    graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
-        held = block(xt, attend)
+    if captured:
+        block(xt, attend)                     # (written over by the first step)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = block(xt, attend)
     lens = list(nq)
     for step in range(4):
         xt.copy_(ATTN.normal(80 + step, len(nq), HIDDEN).to(dtype))
-        graph.replay()
+        if captured:
+            graph.replay()
+        else:
+            held = block(xt, attend)
         torch.cuda.synchronize()
         lens = [n + 1 for n in lens]
         block.check(held, lambda qkv: ATTN.exact(parts(qkv)[0], ck, cv, [1] * len(nq), lens, left, 0, sinks, starts))

@@ -107,6 +107,11 @@ def test_attention_refuses(L, kw, code):
     assert attn(L, **kw) == code and L.last_error()
 
 
+@pytest.mark.parametrize("kw", [dict(scale=2.5e38), dict(scale=-2.5e38), dict(q_tokens=(1 << 31) - 100, heads=1, kv_heads=1)])
+def test_attention_refuses_what_f32_and_places_cannot_hold(L, kw):
+    assert attn(L, **kw) in (-1, -8) and L.last_error()
+
+
 def test_attention_of_nothing_needs_no_device(L):
     assert attn(L, seqs=0, cu=None) == 0 and attn(L, q_tokens=0, kv_tokens=0, q=None, k=None, v=None, out=None) == 0
     n = C.c_uint64(7)

@@ -8,6 +8,8 @@ import numpy as np
 import pytest
 import torch
 
+from .conftest import needs_capture
+
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
 TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
@@ -160,6 +162,7 @@ def test_more_data_than_the_caches_hold(layers, dtype):
     check_rounded(r.y, y, TYPES[dtype], 70 * U)
 
 
+@needs_capture
 def test_streams_and_graph(layers):
     x, w = torch.randn(50, 1024, device="cuda").bfloat16(), torch.rand(1024, device="cuda").bfloat16()
     res = torch.randn(50, 1024, device="cuda").bfloat16()

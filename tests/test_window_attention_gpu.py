@@ -11,6 +11,8 @@ import math
 import pytest
 import torch
 
+from .conftest import needs_capture
+
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -23
 TYPES = {"bf16": torch.bfloat16, "f16": torch.float16}
@@ -266,6 +268,32 @@ def test_odd_places(layers, dtype, dim, nq, nk):
         check(out, lse, exact(q, k, v, nq, nk, left, right, sinks, starts))
 
 
+@pytest.mark.parametrize("nq,nk", [([300, 5], [300, 5]), ([1, 1], [3000, 12])])
+def test_over_the_queries(layers, nq, nk):
+    """out = q itself: each row of q is read by those that write its output alone, before they write"""
+    q = normal(42, sum(nq), 4, 64).bfloat16()
+    k, v = normal(43, sum(nk), 2, 64).bfloat16(), normal(44, sum(nk), 2, 64).bfloat16()
+    args = dict(left=900, right=0, kv_start=torch.tensor([0, nk[0]], device="cuda"), kv_len=torch.tensor(nk, dtype=torch.int32, device="cuda"))
+    want = layers.window_attention(q, k, v, cu_of(nq), **args)
+    got = q.clone()
+    assert layers.window_attention(got, k, v, cu_of(nq), out=got, **args) is got
+    assert torch.equal(got, want)
+
+
+def test_no_keys_at_all_and_the_largest_bounds(layers):
+    none = torch.empty(0, 2, 64, device="cuda", dtype=torch.bfloat16)
+    start, length = torch.zeros(1, dtype=torch.int64, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    for n in (1, 500):
+        out, lse = layers.window_attention(normal(45, n, 4, 64).bfloat16(), none, none, cu_of([n]), kv_start=start, kv_len=length, return_lse=True)
+        assert (out == 0).all() and (lse == -math.inf).all()
+    big = 2 ** 31 - 1
+    q, k, v = normal(46, 200, 4, 64).bfloat16(), normal(47, 200, 2, 64).bfloat16(), normal(48, 200, 2, 64).bfloat16()
+    for left, right, sinks in [(big, big, 0), (big, 0, big), (0, big, big), (-2 ** 31, -2 ** 31, 0)]:
+        for a, b in ((200, 200), (3, 200)):
+            out, lse = layers.window_attention(q[:a], k, v, cu_of([a]), left=left, right=right, sinks=sinks, kv_start=start, kv_len=length + b, return_lse=True)
+            check(out, lse, exact(q[:a], k, v, [a], [b], left, right, sinks, [0]))
+
+
 def test_a_cache_in_many_parts(layers):
     nk = [60000, 1, 33333]
     starts = [0, 60000, 60001]
@@ -276,6 +304,7 @@ def test_a_cache_in_many_parts(layers):
         check(out, lse, exact(q, k, v, [1, 1, 2], nk, left, 0, 5, starts))
 
 
+@needs_capture
 def test_streams_and_two_graphs(layers):
     """two captured graphs and eager calls in between, with lengths that change from replay to replay"""
     q = normal(26, 2, 8, 64).bfloat16()
