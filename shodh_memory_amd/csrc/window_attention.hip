@@ -210,15 +210,16 @@ struct Rows {
         }
     }
 
-    // Scores of NB blocks of 32 keys in LDS at Ks.
-    template <int NB>
-    __device__ __forceinline__ void scores(const unsigned char *Ks, f32x16 (&s)[NB]) const {
+    // Scores of NB blocks of 32 keys in LDS at Ks; `meanwhile` is called while their fragments are on their way.
+    template <int NB, class Meanwhile>
+    __device__ __forceinline__ void scores(const unsigned char *Ks, f32x16 (&s)[NB], Meanwhile meanwhile) const {
         V8 k[NB][DP / 16];
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i)
 #pragma unroll
             for (int b = 0; b < NB; ++b) k[b][i] = *reinterpret_cast<const V8 *>(Ks + at_k[i] + b * (32 * DP * 2));
         if constexpr (NB > 1) __builtin_amdgcn_sched_barrier(0);          // (all of them on their way before the first is waited for)
+        meanwhile();
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -509,7 +510,26 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs a) {
     if (n > 0) fetch(0);
     Rows<T, DP> rows;
     rows.init(a, s, kvh, row0 + wave * 32);
+    // Tiles [plain0, plain1) are whole and every row of the workgroup sees all of each: no masks, no looking through, no arithmetic but the rows'
+    // (8192 tokens, 2048 keys each, 32 over 8 heads of 128: 270 -> 266 us; of 32: 125 -> 120 us)
+    const int seen = min(all.hi_min, g.end) - g.begin;
+    const int plain0 = n_first + max(0, (all.lo_max - g.begin + KT - 1) / KT), plain1 = DMA && whole && seen > 0 ? n_first + seen / KT : 0;
     for (int i = 0; i < n; ++i) {
+        if (i >= plain0)
+            for (; i + 1 < plain1; ++i) {
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                const unsigned char *Ks = smem + (i & 1) * 2 * TILE;
+                f32x16 sc[KT / 32];
+                typename Rows<T, DP>::V8 p[KT / 32][2];
+                rows.scores(Ks, sc, [&] {
+                    const uint32_t to = lds0 + (~i & 1) * 2 * TILE;
+                    glds16_n(uniform_ptr((const unsigned char *)kn), off_k, to, 4096);
+                    glds16_n(uniform_ptr((const unsigned char *)vn), off_v, to + TILE, 4096);
+                    kn += k_step; vn += v_step;
+                });
+                rows.softmax(a, sc, p, 0, 0, false);
+                rows.values(Ks + TILE, p);
+            }
         // this tile has arrived, for every wave; nobody reads the other buffer any more
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         if (i + 1 < n) fetch(i + 1);
@@ -527,7 +547,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs a) {
             const bool masked = !(j + KT <= min(own.hi_min, limit) && (j >= own.lo_max || j + KT <= (int)a.sinks));
             f32x16 sc[KT / 32];
             typename Rows<T, DP>::V8 p[KT / 32][2];
-            rows.scores(Ks, sc);
+            rows.scores(Ks, sc, [] {});
             rows.softmax(a, sc, p, j, limit, masked);
             rows.values(Ks + TILE, p);
         }
