@@ -59,12 +59,13 @@ template <> struct Vec8<_Float16> { using V = f16x8; using V2 = f16x2; static co
 __device__ __forceinline__ f32x16 mma32(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16 mma32(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
-// Does a wave find a value that is no number in `bytes` of V in LDS?
-template <class T>
-__device__ __forceinline__ bool find_values(const unsigned char *Vs, int bytes, int lane) {
+// Does a wave find a value that is no number in BYTES of V in LDS?
+template <class T, int BYTES>
+__device__ __forceinline__ bool find_values(const unsigned char *Vs, int lane) {
     uint32_t m = 0;
-    for (int e = lane * 16; e < bytes; e += 1024) {
-        const u32x4 w = *reinterpret_cast<const u32x4 *>(Vs + e);
+#pragma unroll 8
+    for (int e = 0; e < BYTES; e += 1024) {
+        const u32x4 w = *reinterpret_cast<const u32x4 *>(Vs + e + lane * 16);
 #pragma unroll
         for (int i = 0; i < 4; ++i) m |= (w[i] & Vec8<T>::EXP) + Vec8<T>::ONE;          // an exponent of all ones carries into the sign's place
     }
@@ -237,16 +238,16 @@ struct Rows {
         for (int i = 0; i < DP / 16; ++i)
             s = mma32(*reinterpret_cast<const V8 *>(Ks + at_k[i]), *reinterpret_cast<const V8 *>(Qs + i * 1024 + lane * 16), s);
     }
-    // Scores to probabilities. Keys from `limit` on belong to no one here; masked: some row does not see some key of these.
+    // Scores to probabilities. Block b begins at key[b]; keys from limit[b] on belong to no one here; masked: some row does not see some key of these.
     template <int NB>
-    __device__ __forceinline__ void softmax(const AttnArgs &a, f32x16 (&s)[NB], V8 (&p)[NB][2], int key, int limit, bool masked) {
+    __device__ __forceinline__ void softmax(const AttnArgs &a, f32x16 (&s)[NB], V8 (&p)[NB][2], const int (&key)[NB], const int (&limit)[NB], bool masked) {
         if (masked) {
-            const int half = lane >> 5, end = min(hi, limit);
+            const int half = lane >> 5;
             auto first = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; };
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 // a bit for each of the block's keys that the row sees; in the order of the registers after a shift by the half's 4
-                const int j = key + b * 32;
+                const int j = key[b], end = min(hi, limit[b]);
                 const uint32_t seen = (first(end - j) & (~first(lo - j) | first((int)a.sinks - j))) >> (4 * half);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
@@ -470,10 +471,12 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs a) {
     if (row0 < 0 || row0 >= (int64_t)s.nq * a.group) return;
     const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const Range g = range_of(a, s, row0, row0 + BM);
-    const int n_first = (g.first + KT - 1) / KT, n = n_first + (g.end - g.begin + KT - 1) / KT;
+    // Up to 32 sinks share a tile with the window's first 32 keys: tile 0, of two blocks that begin at 0 and at g.begin. The tiles behind begin at w0.
+    const bool mixed = g.first > 0 && g.first <= 32;
+    const int n_first = (g.first + KT - 1) / KT, w0 = g.begin + (mixed ? 32 : 0), n = n_first + max(0, g.end - w0 + KT - 1) / KT;
     const Bounds own = bounds_of(a, s, row0 + wave * 32, row0 + wave * 32 + 32), all = bounds_of(a, s, row0, row0 + BM);
     const T *kb = (const T *)a.k + (uint64_t)s.k0 * a.k_stride + (uint64_t)kvh * a.k_head, *vb = (const T *)a.v + (uint64_t)s.k0 * a.v_stride + (uint64_t)kvh * a.v_head;
-    auto start_of = [&](int i) { return i < n_first ? i * KT : g.begin + (i - n_first) * KT; };
+    auto start_of = [&](int i) { return i < n_first ? i * KT : w0 + (i - n_first) * KT; };
     auto limit_of = [&](int i) { return i < n_first ? g.first : g.end; };
     // whole tiles: the lane's offsets from a base that moves on with the tiles
     constexpr int N = KT * DP / 8 / 256, STEP = 256 / (DP / 8);
@@ -485,12 +488,19 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs a) {
         off_v[i] = ((uint32_t)row * (uint32_t)a.v_stride + v_place<DP>(row, x) * 8) * 2;
     }
     const uint32_t lds0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds_address(smem) + wave * 1024));
-    const T *kn = kb + (n_first ? 0 : (uint64_t)g.begin * a.k_stride), *vn = vb + (n_first ? 0 : (uint64_t)g.begin * a.v_stride);       // the next tile's
+    const T *kn = kb + (n_first ? 0 : (uint64_t)w0 * a.k_stride), *vn = vb + (n_first ? 0 : (uint64_t)w0 * a.v_stride);       // the next tile's
     const uint64_t k_step = (uint64_t)KT * a.k_stride, v_step = (uint64_t)KT * a.v_stride;
     const bool whole = a.dim == DP;
     auto fetch = [&](int i) {
         const int last = min(KT, limit_of(i) - start_of(i)) - 1;
-        if (DMA && whole && last == KT - 1) {
+        if (mixed && i == 0) {              // half of the threads a block
+            const int b = wave >> 1, first = b ? g.begin : 0, last_b = (b ? min(32, g.end - g.begin) : g.first) - 1;
+            unsigned char *Ks = smem + b * (TILE / 2);
+            if (last_b >= 0) {
+                stage<T, DP, 32, 128, DMA>(Ks, kb + (uint64_t)first * a.k_stride, a.k_stride, last_b, a.dim, t & 127, KPlace<DP>());
+                stage<T, DP, 32, 128, DMA>(Ks + TILE, vb + (uint64_t)first * a.v_stride, a.v_stride, last_b, a.dim, t & 127, VPlace<DP>());
+            }
+        } else if (DMA && whole && last == KT - 1) {
             const uint32_t to = lds0 + (i & 1) * 2 * TILE;
             glds16_n(uniform_ptr((const unsigned char *)kn), off_k, to, 4096);
             glds16_n(uniform_ptr((const unsigned char *)vn), off_v, to + TILE, 4096);
@@ -499,7 +509,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs a) {
             stage<T, DP, KT, 256, DMA>(Ks, kn, a.k_stride, last, a.dim, t, KPlace<DP>());
             stage<T, DP, KT, 256, DMA>(Ks + TILE, vn, a.v_stride, last, a.dim, t, VPlace<DP>());
         }
-        if (i + 1 == n_first) { kn = kb + (uint64_t)g.begin * a.k_stride; vn = vb + (uint64_t)g.begin * a.v_stride; }
+        if (i + 1 == n_first) { kn = kb + (uint64_t)w0 * a.k_stride; vn = vb + (uint64_t)w0 * a.v_stride; }
         else { kn += k_step; vn += v_step; }
     };
     if (DMA && a.dim < DP) {
@@ -512,8 +522,8 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs a) {
     rows.init(a, s, kvh, row0 + wave * 32);
     // Tiles [plain0, plain1) are whole and every row of the workgroup sees all of each: no masks, no looking through, no arithmetic but the rows'
     // (8192 tokens, 2048 keys each, 32 over 8 heads of 128: 270 -> 266 us; of 32: 125 -> 120 us)
-    const int seen = min(all.hi_min, g.end) - g.begin;
-    const int plain0 = n_first + max(0, (all.lo_max - g.begin + KT - 1) / KT), plain1 = DMA && whole && seen > 0 ? n_first + seen / KT : 0;
+    const int seen = min(all.hi_min, g.end) - w0;
+    const int plain0 = n_first + max(0, (all.lo_max - w0 + KT - 1) / KT), plain1 = DMA && whole && seen > 0 ? n_first + seen / KT : 0;
     for (int i = 0; i < n; ++i) {
         if (i >= plain0)
             for (; i + 1 < plain1; ++i) {
@@ -527,7 +537,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs a) {
                     glds16_n(uniform_ptr((const unsigned char *)vn), off_v, to + TILE, 4096);
                     kn += k_step; vn += v_step;
                 });
-                rows.softmax(a, sc, p, 0, 0, false);
+                rows.softmax(a, sc, p, {0, 0}, {0, 0}, false);
                 rows.values(Ks + TILE, p);
             }
         // this tile has arrived, for every wave; nobody reads the other buffer any more
@@ -535,8 +545,9 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs a) {
         if (i + 1 < n) fetch(i + 1);
         unsigned char *Ks = smem + (i & 1) * 2 * TILE;
         const int j = start_of(i), limit = limit_of(i);
-        if (!(j + KT <= min(all.hi_min, limit) && (j >= all.lo_max || j + KT <= (int)a.sinks))) {        // some row of the workgroup sees it in part
-            if (__builtin_expect(find_values<T>(Ks + TILE, TILE, t & 63), 0)) {       // (every wave looks through all of it: all find the same)
+        const bool two = mixed && i == 0;
+        if (two || !(j + KT <= min(all.hi_min, limit) && (j >= all.lo_max || j + KT <= (int)a.sinks))) {        // some row of the workgroup sees it in part
+            if (__builtin_expect(find_values<T, TILE>(Ks + TILE, t & 63), 0)) {       // (every wave looks through all of it: all find the same)
                 __syncthreads();
                 clear_values<T, 256>(Ks + TILE, TILE, t);
                 __syncthreads();
@@ -544,11 +555,11 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs a) {
             }
         }
         if (j < own.hi_max && (j + KT > own.lo_min || j < (int)a.sinks)) {
-            const bool masked = !(j + KT <= min(own.hi_min, limit) && (j >= own.lo_max || j + KT <= (int)a.sinks));
+            const bool masked = two || !(j + KT <= min(own.hi_min, limit) && (j >= own.lo_max || j + KT <= (int)a.sinks));
             f32x16 sc[KT / 32];
             typename Rows<T, DP>::V8 p[KT / 32][2];
             rows.scores(Ks, sc, [] {});
-            rows.softmax(a, sc, p, j, limit, masked);
+            rows.softmax(a, sc, p, {j, two ? g.begin : j + 32}, {limit, two ? g.end : limit}, masked);
             rows.values(Ks + TILE, p);
         }
     }
@@ -678,9 +689,9 @@ __global__ __launch_bounds__(256, 2) void attn_split_kernel(const AttnArgs a) {
         rows.scores_lds(Ks, Qs, sc[0]);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         if (more) fetch_k(i + 4);
-        rows.softmax(a, sc, p, j, limit, masked);
+        rows.softmax(a, sc, p, {j}, {limit}, masked);
         arrived(!more);                       // V
-        if (masked && __builtin_expect(find_values<T>(Vs, TILE, rows.lane), 0)) {
+        if (masked && __builtin_expect(find_values<T, TILE>(Vs, rows.lane), 0)) {
             clear_values<T, 64>(Vs, TILE, rows.lane);
             spoiled = true;
         }
