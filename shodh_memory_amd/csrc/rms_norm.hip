@@ -80,15 +80,20 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(const R
     constexpr int WAVES = TPR / 64, ROWS = TPR < 256 ? 256 / TPR : 1;
     __shared__ float part[2][WAVES];
     __shared__ uint32_t part_max[2][WAVES];
+    constexpr bool HELD = C * TPR < 4096;       // the weights wait in registers for the row's sum; of the longest rows there is no room for them
+                                                // (8192 x 32768 bf16 380 -> 354 us)
     const int t = threadIdx.x % TPR, wave = t >> 6;
-    float w[C][8];
+    float w[HELD ? C : 1][8];
     uint32_t left[C];           // values of the row from this thread's place on: 8 or more where a step is whole
+    auto weight = [&](int c, float (&v)[8]) {
+        if (a.weight_f32) load8<false>(v, (const float *)a.weight + (c * TPR + t) * 8, left[c]);
+        else load8<false>(v, (const T *)a.weight + (c * TPR + t) * 8, left[c]);
+    };
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         const uint32_t at = (uint32_t)(c * TPR + t) * 8;
         left[c] = at < a.dim ? a.dim - at : 0;
-        if (a.weight_f32) load8<false>(w[c], (const float *)a.weight + at, left[c]);
-        else load8<false>(w[c], (const T *)a.weight + at, left[c]);
+        if constexpr (HELD) weight(c, w[c]);
     }
     auto row_sum = [&](float v, int slot) -> float {
         v = wave_sum(v);
@@ -138,9 +143,11 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(const R
         }
         const float rstd = 1.0f / __builtin_sqrtf(ss / (float)a.dim + eps);
 #pragma unroll
-        for (int c = 0; c < C; ++c)
+        for (int c = 0; c < C; ++c) {
+            if constexpr (!HELD) weight(c, w[0]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) h[c][i] = h[c][i] * rstd * w[c][i];
+            for (int i = 0; i < 8; ++i) h[c][i] = h[c][i] * rstd * w[HELD ? c : 0][i];
+        }
         if (a.y)
 #pragma unroll
             for (int c = 0; c < C; ++c) store8<STREAM>((T *)a.y + row * a.y_stride + (c * TPR + t) * 8, h[c], left[c]);
@@ -215,7 +222,7 @@ static int launch_rms(const RmsArgs &a, hipStream_t st) {
     // one workgroup for every one or four rows: its neighbours on the CU hide its waits (a loop over rows with the weights kept: 213 instead of 198 us
     // for 32768 x 4096 bf16 with residual, sum and e4m3)
     auto go = [&](auto kern, int threads, int rows_per_wg) {
-        const uint64_t wgs = ceil_div(a.rows, rows_per_wg), most = 1u << 24;
+        const uint64_t wgs = ceil_div(a.rows, rows_per_wg), most = (1u << 31) / threads;        // (a launch has fewer than 2^32 threads; further rows in turns)
         hipLaunchKernelGGL(kern, dim3((uint32_t)(wgs < most ? wgs : most)), dim3(threads), 0, st, a);
     };
     if (a.dim <= 512) go(rms_norm_kernel<T, 64, 1, STREAM>, 256, 4);

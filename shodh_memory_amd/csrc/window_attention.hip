@@ -849,10 +849,13 @@ static int check_attention(const shodh_attention_cfg *c) {
 
 template <class T, int DP, bool DMA>
 static int launch_attention(const AttnArgs &a, const AttnPlan &p, hipStream_t st) {
+    // a launch has fewer than 2^32 threads
+    const uint64_t tiles = (uint64_t)p.slots * a.kv_heads, joins = ceil_div((uint64_t)a.q_tokens * a.heads, 4);
+    if ((p.split ? p.splits > 1 ? joins : 0 : tiles) >= (1u << 24)) { set_error("attention: too many rows for one launch"); return SHODH_ERR_UNSUPPORTED; }
     if (!p.split) {
         constexpr size_t lds = 4 * 64 * DP * 2;
         SHODH_TRY(ensure_dynamic_lds((const void *)attn_tile_kernel<T, DP, DMA>, lds));
-        hipLaunchKernelGGL((attn_tile_kernel<T, DP, DMA>), dim3(p.slots * a.kv_heads), dim3(256), lds, st, a);
+        hipLaunchKernelGGL((attn_tile_kernel<T, DP, DMA>), dim3((uint32_t)tiles), dim3(256), lds, st, a);
         SHODH_HIP_TRY(hipGetLastError());
         return SHODH_OK;
     }
@@ -861,7 +864,7 @@ static int launch_attention(const AttnArgs &a, const AttnPlan &p, hipStream_t st
     hipLaunchKernelGGL((attn_split_kernel<T, DP, DMA>), dim3(p.grid), dim3(256), lds, st, a);
     SHODH_HIP_TRY(hipGetLastError());
     if (p.splits > 1) {
-        hipLaunchKernelGGL((attn_join_kernel<T, DP>), dim3((uint32_t)ceil_div((uint64_t)a.q_tokens * a.heads, 4)), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((attn_join_kernel<T, DP>), dim3((uint32_t)joins), dim3(256), 0, st, a);
         SHODH_HIP_TRY(hipGetLastError());
     }
     return SHODH_OK;

@@ -162,6 +162,15 @@ def test_more_data_than_the_caches_hold(layers, dtype):
     check_rounded(r.y, y, TYPES[dtype], 70 * U)
 
 
+def test_more_rows_than_a_launch_has_workgroups(layers):
+    """70 million rows of one value: y = x / sqrt(x^2 + eps) w, the tolerance of any y"""
+    x = torch.randn(70_000_001, 1, generator=torch.Generator(device="cuda").manual_seed(2), device="cuda").bfloat16()
+    w = torch.full((1,), 1.5, device="cuda")
+    y = layers.rms_norm(x, w, eps=1e-3).y
+    for part in (slice(0, 1000), slice(33_554_000, 33_555_000), slice(67_108_000, 67_110_000), slice(69_999_000, None)):
+        check_rounded(y[part], defined(x[part], w, None, 1e-3)[1], torch.bfloat16, 70 * U)
+
+
 @needs_capture
 def test_streams_and_graph(layers):
     x, w = torch.randn(50, 1024, device="cuda").bfloat16(), torch.rand(1024, device="cuda").bfloat16()
