@@ -46,6 +46,15 @@ def _current(stream, device):
     return torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device))
 
 
+def _like(t, dtype=None):
+    """a contiguous tensor of t's shape (empty_like takes 1.2 us, new_empty 1.8)"""
+    return torch.empty_like(t, dtype=dtype) if t.is_contiguous() else t.new_empty(t.shape, dtype=dtype)
+
+
+def _new(rows, cols, dtype, device):
+    return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)
+
+
 def _matrix(t, name):
     """(rows, columns, row stride) of [..., columns] with neighbouring elements next to each other: a view of rows at one distance."""
     if t.dim() == 2:
@@ -92,7 +101,7 @@ def rms_norm(x, weight, eps=1e-6, residual=None, want_y=True, quant=None, group=
         _on(residual, device, "residual")
         rs = _matrix(residual, "residual")[2]
         if sum_out is None:
-            total = x.new_empty(x.shape)
+            total = _like(x)
         else:
             total = sum_out
             if total.shape != x.shape or total.dtype != x.dtype:
@@ -101,15 +110,15 @@ def rms_norm(x, weight, eps=1e-6, residual=None, want_y=True, quant=None, group=
             ss = _matrix(total, "sum_out")[2]
     elif sum_out is not None:
         _refuse("sum_out without a residual")
-    y = x.new_empty(x.shape) if want_y else None
+    y = _like(x) if want_y else None
     q = scale = None
     qd = L.DTYPE_INT8
     if quant is not None:
         if quant not in _QUANT:
             _refuse("quant %r is neither 'int8' nor 'e4m3'" % (quant,))
         qd, qt = _QUANT[quant]
-        q = x.new_empty(x.shape, dtype=qt)
-        scale = x.new_empty((rows, -(-dim // group) if group else 1), dtype=torch.float32)
+        q = _like(x, qt)
+        scale = _new(rows, -(-dim // group) if group else 1, torch.float32, device)
     if rows == 0:
         return RmsNorm(y, q, scale, total)
     cfg = L.RmsNormCfg(rows, xs, rs, ss, 0, 0, dim, dt, wd, qd, group, eps)
@@ -210,11 +219,12 @@ class W4Weight:
                 _refuse("bias has to be contiguous f32 [%d]" % self.n, L.ERR_DIM)
             _on(bias, self.device, "bias")
             bp = bias.data_ptr()
-        shape = x.shape[:-1] + (self.n,)
         if out is None:
-            out = x.new_empty(shape, dtype=out_dtype or (torch.bfloat16 if xd == L.DTYPE_INT8 else x.dtype))
+            dtype = out_dtype or (torch.bfloat16 if xd == L.DTYPE_INT8 else x.dtype)
+            out = _new(rows, self.n, dtype, self.device) if x.dim() == 2 else x.new_empty(x.shape[:-1] + (self.n,), dtype=dtype)
             os_ = self.n
         else:
+            shape = x.shape[:-1] + (self.n,)
             if out.shape != shape or (out_dtype is not None and out.dtype != out_dtype):
                 _refuse("out has to be %s" % (tuple(shape),), L.ERR_DIM)
             _on(out, self.device, "out")
@@ -295,7 +305,7 @@ def window_attention(q, k, v, cu, left=-1, right=-1, sinks=0, kv_start=None, kv_
     if kv_start is not None:
         sp, lp = _descriptor(kv_start, "kv_start", device, torch.int64, seqs), _descriptor(kv_len, "kv_len", device, torch.int32, seqs)
     if out is None:
-        out = q.new_empty((n, heads, dim))
+        out = _like(q)
         os_, oh = heads * dim, dim
     else:
         if out.shape != q.shape:
@@ -305,7 +315,7 @@ def window_attention(q, k, v, cu, left=-1, right=-1, sinks=0, kv_start=None, kv_
         _refuse("left, right and sinks are 32-bit numbers, sinks 0 or more")
     if scale is not None and not scale != 0:
         _refuse("scale 0 (or no number)")
-    lse = q.new_empty((n, heads), dtype=torch.float32) if return_lse else None
+    lse = _new(n, heads, torch.float32, device) if return_lse else None
     if n and seqs:
         cfg = L.AttentionCfg(n, kn, qs, qh, ks, kh, vs, vh, os_, oh, dt, heads, kv_heads, dim, seqs, sinks, left, right, scale or 0.0, 0)
         need = _attention_workspace(device.index, n, kn, dt, heads, kv_heads, dim, seqs, sinks, left, right)
