@@ -8,8 +8,10 @@
 // down the lane's own registers, O^T = V^T P^T with P straight from those registers. The order in which the first product hands keys to a lane
 // (register r of half h holds key (r & 3) + 8 (r >> 2) + 4 h of 32) is taken as the order of the second product's inner index; V^T in that order is what
 // the transposing LDS read returns for four neighbouring keys. One pass over the keys, with a running maximum and sum in f32. The reference maximum is
-// only raised when a tile's maximum is more than 8 (in powers of two) above it: until then exp2 stays below 256, so nothing is lost and the accumulator
-// is not scaled again. P is rounded to the inputs' 16-bit type, because that is what the matrix instruction multiplies; the sum is of unrounded values.
+// only raised when a tile's maximum is more than 8 (in powers of two) above its place: until then the accumulator is not scaled again. P is rounded to the
+// inputs' 16-bit type, because that is what the matrix instruction multiplies; the sum is of unrounded values. fp16 has no number below 2^-24, so there
+// the reference lies 7 below the maximum: the largest P is 2^7 .. 2^15 and one step of the smallest is 2^-31 of it or less, which keeps what a sink with
+// nearly all the weight leaves to 4096 others (17.5 above them: within 0.02 %; with the reference at the maximum all of it was lost). bf16 needs no such room.
 //
 // A row of work is one (query token, head of a group): the heads that share a key head read the same tile. Two forms:
 //  * tiles (texts, prompts): 4 waves x 32 rows, K and V tiles of 64 keys straight to LDS, the next tile on its way meanwhile. Bound: the matrix unit, with
@@ -57,9 +59,10 @@ __device__ __forceinline__ float half_sum(float x) {
     return __uint_as_float(s[0]) + __uint_as_float(s[1]);
 }
 
+// (BELOW: how far the reference maximum lies below the largest score, in powers of two)
 template <class T> struct Vec8;
-template <> struct Vec8<__bf16> { using V = bf16x8; using V2 = bf16x2; static constexpr uint32_t EXP = 0x7F807F80u, ONE = 0x00800080u; };
-template <> struct Vec8<_Float16> { using V = f16x8; using V2 = f16x2; static constexpr uint32_t EXP = 0x7C007C00u, ONE = 0x04000400u; };
+template <> struct Vec8<__bf16> { using V = bf16x8; using V2 = bf16x2; static constexpr uint32_t EXP = 0x7F807F80u, ONE = 0x00800080u; static constexpr float BELOW = 0.0f; };
+template <> struct Vec8<_Float16> { using V = f16x8; using V2 = f16x2; static constexpr uint32_t EXP = 0x7C007C00u, ONE = 0x04000400u; static constexpr float BELOW = 7.0f; };
 __device__ __forceinline__ f32x16 mma32(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16 mma32(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
@@ -266,9 +269,9 @@ struct Rows {
 #pragma unroll
             for (int r = 0; r < 16; ++r) tops[r & 3] = fmaxf(tops[r & 3], s[b][r]);
         const float top = half_max(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]))) * a.scale2;
-        const bool raise = top > m + 8.0f;      // (m = -inf: any finite score); a row's own affair: its neighbours change nothing in it
+        const bool raise = top > m + (8.0f + Vec8<T>::BELOW);      // (m = -inf: any finite score); a row's own affair: its neighbours change nothing in it
         if (__any(raise)) {
-            const float next = raise ? top : m, c = raise ? __builtin_amdgcn_exp2f(m - next) : 1.0f;
+            const float next = raise ? top - Vec8<T>::BELOW : m, c = raise ? __builtin_amdgcn_exp2f(m - next) : 1.0f;
             m = next;
             l *= c;
 #pragma unroll

@@ -357,3 +357,29 @@ def test_refusals(layers):
             call()
     assert A(q[:0], k[:0], v[:0], cu_of([0])).shape == (0, 4, 64)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("lq,heads", [(1, 2), (3, 2), (700, 2), (1024, 32)])
+@pytest.mark.parametrize("above", [10.0, 14.0, 16.0, 17.5, 20.0])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_what_a_dominant_sink_leaves_over(layers, dtype, above, lq, heads):
+    """a first key with nearly all the weight and a value of zero: the output is what the many others make of the small rest. A probability in fp16 is
+    off by half its type's step relative, or by half of the smallest step: 2^-25 of 2^7 at least, the place of the largest (bf16 has that range):
+        |out - exact| <= (h + 2 e + 160 u) sum p |v| + h |exact| + [fp16] 2^-32 sum |v| + 2^-25
+    with scores of one exact product each: e = 66 u |s|, |s| <= above."""
+    t, n, d = TYPES[dtype], 4096, 64
+    q = torch.zeros(lq, heads, d, device="cuda", dtype=t)
+    q[:, :, 0] = 1
+    k = torch.zeros(n, heads, d, device="cuda", dtype=t)
+    k[1:, :, 0] = (0.02 * normal(60, n - 1, 1)).to(t)
+    k[0, :, 0] = above
+    v = normal(61, n, 1, d).to(t).expand(n, heads, d).contiguous()
+    v[:, :, :8] = 1                                            # rest after rest on the same side: nothing averages out
+    v[0] = 0
+    out = layers.window_attention(q, k, v, cu_of([lq]), left=n, right=n, sinks=1, scale=1.0, kv_start=torch.zeros(1, dtype=torch.int64, device="cuda"),
+                                  kv_len=torch.tensor([n], dtype=torch.int32, device="cuda"))
+    p, v0 = torch.softmax(k[:, 0, 0].double(), 0), v[:, 0].double()
+    want, size = p @ v0, p @ v0.abs()
+    h = torch.finfo(t).eps / 2
+    tol = (h + 2 * 66 * U * above + 160 * U) * size + h * want.abs() + ((2.0 ** -32 * v0.abs().sum(0) + 2.0 ** -25) if t == torch.float16 else 0)
+    assert ((out.double() - want).abs() <= tol * (1 + 1e-6)).all(), float(((out.double() - want).abs() / tol).max())
