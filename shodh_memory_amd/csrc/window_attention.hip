@@ -11,7 +11,7 @@
 // only raised when a tile's maximum is more than 8 (in powers of two) above its place: until then the accumulator is not scaled again. P is rounded to the
 // inputs' 16-bit type, because that is what the matrix instruction multiplies; the sum is of unrounded values. fp16 has no number below 2^-24, so there
 // the reference lies 7 below the maximum: the largest P is 2^7 .. 2^15 and one step of the smallest is 2^-31 of it or less, which keeps what a sink with
-// nearly all the weight leaves to 4096 others (17.5 above them: within 0.02 %; with the reference at the maximum all of it was lost). bf16 needs no such room.
+// nearly all the weight leaves to 4096 others (17.5 above them: within 0.02 %; with the reference at the maximum an eighth to all of it was lost). bf16 needs no such room.
 //
 // A row of work is one (query token, head of a group): the heads that share a key head read the same tile. Two forms:
 //  * tiles (texts, prompts): 4 waves x 32 rows, K and V tiles of 64 keys straight to LDS, the next tile on its way meanwhile. Bound: the matrix unit, with
@@ -37,15 +37,20 @@ struct AttnArgs {
     const int32_t *cu;
     const int64_t *kv_start;
     const int32_t *kv_len;
-    float *part;               // split form: [splits][rows of out][DP] sums, [splits][rows][2] maxima and sums, [rows] numbers of parts (0: the row is done)
+    float *part;               // split form, the workspace: 16 bytes (number of rows to be joined, per key head), [kv_heads][list_room] of these rows,
+                               // [kv_heads][room][DP] parts' sums, [kv_heads][room][2] maxima and sums
     uint64_t q_stride, q_head, k_stride, k_head, v_stride, v_head, o_stride, o_head;
     int64_t q_tokens, kv_tokens;
     uint32_t heads, kv_heads, group, dim, seqs, slots, splits, chunk /* blocks of 32 keys of a part */, sinks;
+    uint32_t room, list_room, coarser;       // (AttnPlan)
     int32_t left, right;       // negative: no bound
     float scale2;              // |scale| * log2(e)
     uint32_t sign;             // 0, or the sign bits of two 16-bit numbers
     int shift;                 // log2(group), or -1
     __device__ __forceinline__ uint32_t over_group(uint32_t x) const { return shift >= 0 ? x >> shift : x / group; }
+    __device__ __forceinline__ u32x4 *list() const { return reinterpret_cast<u32x4 *>(part) + 1; }          // of a row: its place in lse (64 bits), its first part, their number
+    __device__ __forceinline__ float *sums() const { return reinterpret_cast<float *>(list() + (uint64_t)kv_heads * list_room); }
+    __device__ __forceinline__ float *stats(int dp) const { return sums() + (uint64_t)kv_heads * room * dp; }
 };
 
 constexpr float NEG_INF = -__builtin_inff();
@@ -588,51 +593,90 @@ __global__ __launch_bounds__(256, 2) void attn_split_kernel(const AttnArgs a) {
     // workgroup takes every gridDim.x-th of them, so that short sequences cost what they are.
     struct Table {
         int64_t q0[64], k0[64];
-        int nq[64], nk[64], parts[64], begin[64], end[64];       // items of sequences base .. : [begin, end)
+        int nq[64], nk[64], parts[64];
+        uint32_t begin[64], end[64];             // items of sequences base .. : [begin, end)
+        uint32_t first[64], listed[64];          // places of a key head's parts and listed rows
+        uint32_t parts_before, rows_before, fewer, pad;        // places and listed rows of the sequences before base + 64
     };
+    static_assert(sizeof(Table) == 64 * 44 + 16, "");
     Table &table = *reinterpret_cast<Table *>(smem + 8 * TILE + 1024);
+    // A sequence is wanted in so many parts; `fewer` of these are one, where the places would not do for all: then its rows that are cut have two parts at
+    // least, and 2 / fewer of what was wanted at most.
+    constexpr uint32_t MOST = 1u << 24;            // (more than any room: counts stop there, and 64 of them and MOST are below 2^32)
+    auto wanted = [&](const Seq &s) {
+        int64_t seen = s.nk;
+        if (a.left >= 0 && a.right >= 0) seen = min(seen, (int64_t)a.left + a.right + 1 + BM + 64 + (int64_t)a.sinks);
+        return (uint32_t)min((int64_t)a.splits, max((int64_t)1, ((seen + 31) / 32 + a.chunk - 1) / a.chunk));
+    };
+    auto places = [&](const Seq &s, uint32_t parts) { return parts > 1 ? (uint32_t)min((int64_t)s.nq * a.group * parts, (int64_t)MOST) : 0u; };
+    if (a.coarser) {                               // (every workgroup finds the same number)
+        uint64_t sum = 0;
+        for (int64_t b = threadIdx.x; b < (int64_t)a.seqs; b += 256) {
+            const Seq s = seq_at(a, (int)b, a.cu[b], a.cu[b + 1]);
+            sum += places(s, wanted(s));
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) sum += (uint64_t)(uint32_t)__shfl_xor((int)(sum >> 32), o) << 32 | (uint32_t)__shfl_xor((int)sum, o);
+        uint64_t *sums = reinterpret_cast<uint64_t *>(smem);
+        if (lane == 0) sums[wave] = sum;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            const uint64_t f = (2 * (sums[0] + sums[1] + sums[2] + sums[3]) + a.room - 1) / a.room;
+            table.fewer = f < 1 ? 1u : f > 64 ? 64u : (uint32_t)f;           // (64: no sequence has more)
+        }
+        __syncthreads();
+    } else if (wave == 0) table.fewer = 1;
+    auto running = [&](uint32_t x) {               // sum over the lanes up to this one
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) { const uint32_t v = (uint32_t)__shfl_up((int)x, o); if (lane >= o) x += v; }
+        return x;
+    };
     auto count = [&](int base) {          // by wave 0; the items of 64 sequences
         const int b = base + lane;
-        int64_t q0 = 0, k0 = 0;
-        int nq = 0, nk = 0, parts = 1;
-        if (b < (int)a.seqs) {
-            const Seq s = seq_at(a, b, a.cu[b], a.cu[b + 1]);
-            q0 = s.q0; k0 = s.k0; nq = s.nq; nk = s.nk;
-            int64_t seen = nk;
-            if (a.left >= 0 && a.right >= 0) seen = min(seen, (int64_t)a.left + a.right + 1 + BM + 64 + (int64_t)a.sinks);
-            parts = (int)min((int64_t)a.splits, max((int64_t)1, ((seen + 31) / 32 + a.chunk - 1) / a.chunk));
+        Seq s = {0, 0, 0, 0};
+        if (b < (int)a.seqs) s = seq_at(a, b, a.cu[b], a.cu[b + 1]);
+        const int64_t rows = (int64_t)s.nq * a.group;
+        uint32_t parts = 1;
+        if (a.splits > 1) {
+            parts = (wanted(s) + table.fewer - 1) / table.fewer;
+            const uint32_t p = places(s, parts), p_end = (base ? table.parts_before : 0u) + running(p);
+            if (p_end > a.room) parts = 1;         // (only where cu is out of order)
+            const uint32_t r = parts > 1 ? (uint32_t)rows : 0u, r_end = (base ? table.rows_before : 0u) + running(r);
+            table.first[lane] = p_end - p; table.listed[lane] = r_end - r;
+            if (lane == 63) { table.parts_before = min(p_end, MOST); table.rows_before = r_end; }
         }
-        const int items = (int)(((int64_t)nq * a.group + BM - 1) / BM) * parts;
-        int end = items;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) { const int v = __shfl_up(end, o); if (lane >= o) end += v; }
-        table.q0[lane] = q0; table.k0[lane] = k0; table.nq[lane] = nq; table.nk[lane] = nk; table.parts[lane] = parts;
+        const uint32_t items = (uint32_t)((rows + BM - 1) / BM) * parts, end = running(items);          // (rows / 32 < 2^26 - 64 or so: 64 of them fit)
+        table.q0[lane] = s.q0; table.k0[lane] = s.k0; table.nq[lane] = s.nq; table.nk[lane] = s.nk; table.parts[lane] = (int)parts;
         table.begin[lane] = end - items; table.end[lane] = end;
     };
     int base = 0;
     uint32_t before = 0;                 // items of the sequences before base
     if (wave == 0) count(0);
     __syncthreads();
-    for (uint32_t id = blockIdx.x;; id += gridDim.x) {
+    for (uint32_t id = blockIdx.x, next;; id = next) {
+    next = id + gridDim.x;
     // (heads in turn, shifted from item to item: an XCD, which takes every eighth workgroup, sees all of them)
     const uint32_t item = id / a.kv_heads, kvh = (id + (item >> 1)) % a.kv_heads;
-    while (item - before >= (uint32_t)table.end[63]) {
-        before += (uint32_t)table.end[63];
+    while (item - before >= table.end[63]) {
+        before += table.end[63];
         base += 64;
-        if (base >= (int)a.seqs) return;
+        if (base >= (int)a.seqs) {
+            if (a.splits > 1 && blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<uint32_t *>(a.part) = table.rows_before;
+            return;
+        }
         __syncthreads();
         if (wave == 0) count(base);
         __syncthreads();
     }
-    const int at_lane = __ffsll((unsigned long long)__ballot((uint32_t)table.end[lane] > item - before)) - 1;
-    const int within = __builtin_amdgcn_readfirstlane((int)(item - before) - table.begin[at_lane]), parts = __builtin_amdgcn_readfirstlane(table.parts[at_lane]), split = within % parts;
+    const int at_lane = __ffsll((unsigned long long)__ballot(table.end[lane] > item - before)) - 1;
+    const int within = __builtin_amdgcn_readfirstlane((int)(item - before - table.begin[at_lane])), parts = __builtin_amdgcn_readfirstlane(table.parts[at_lane]), split = within % parts;
     Seq s;
     s.q0 = uniform64(table.q0[at_lane]); s.k0 = uniform64(table.k0[at_lane]);
     s.nq = __builtin_amdgcn_readfirstlane(table.nq[at_lane]); s.nk = __builtin_amdgcn_readfirstlane(table.nk[at_lane]);
     const int64_t row0 = (int64_t)(within / parts) * BM;
     Rows<T, DP> rows;
     rows.init(a, s, kvh, row0);
-    unsigned char *Qs = smem + 8 * TILE + 1024 + 64 * 36;          // the queries' fragments, the same for all four waves (registers for them would spill)
+    unsigned char *Qs = smem + 8 * TILE + 1024 + sizeof(Table);          // the queries' fragments, the same for all four waves (registers for them would spill)
     if (wave == 0)
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i) *reinterpret_cast<typename Rows<T, DP>::V8 *>(Qs + i * 1024 + rows.lane * 16) = rows.q[i];
@@ -727,13 +771,15 @@ __global__ __launch_bounds__(256, 2) void attn_split_kernel(const AttnArgs a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) sums[((wave * (DP / 32) + t) * 16 + r) * 64 + rows.lane] = rows.o[t][r] * mine;
     __syncthreads();
-    const uint64_t all = (uint64_t)a.q_tokens * a.heads, at = (uint64_t)(s.q0 + rows.token) * a.heads + rows.head;
-    float *stats = a.part + (uint64_t)a.splits * all * DP;
+    const uint32_t r = (uint32_t)row0 + (rows.lane & 31), place = kvh * a.room + table.first[at_lane] + r * (uint32_t)parts + split;
     rows.m = top;
     if (wave == 0 && rows.live && rows.lane < 32) {
-        if (a.splits > 1 && split == 0) reinterpret_cast<uint32_t *>(stats + (uint64_t)a.splits * all * 2)[at] = parts == 1 ? 0 : parts;
-        if (parts > 1) { stats[(split * all + at) * 2] = top; stats[(split * all + at) * 2 + 1] = total; }
-        else rows.store_lse(a, s, total);
+        if (parts > 1) {
+            float *stats = a.stats(DP) + (uint64_t)place * 2;
+            stats[0] = top; stats[1] = total;
+            const uint64_t at = (uint64_t)(s.q0 + rows.token) * a.heads + rows.head;
+            if (split == 0) a.list()[(uint64_t)kvh * a.list_room + table.listed[at_lane] + r] = u32x4{(uint32_t)at, (uint32_t)(at >> 32), place, (uint32_t)parts};
+        } else rows.store_lse(a, s, total);
     }
     if (wave < DP / 32 && rows.live) {
         f32x16 o;
@@ -746,7 +792,7 @@ __global__ __launch_bounds__(256, 2) void attn_split_kernel(const AttnArgs a) {
         }
         if (parts == 1) rows.store(a, s, o, wave, total);
         else {
-            float *dst = a.part + (split * all + at) * DP + wave * 32 + (rows.lane >> 5) * 4;
+            float *dst = a.sums() + (uint64_t)place * DP + wave * 32 + (rows.lane >> 5) * 4;
 #pragma unroll
             for (int gq = 0; gq < 4; ++gq) {
                 f32x4 e;
@@ -756,22 +802,26 @@ __global__ __launch_bounds__(256, 2) void attn_split_kernel(const AttnArgs a) {
             }
         }
     }
+    if (next < id) {                     // (only where cu is out of order: the items of valid sequences are fewer than 2^32)
+        if (a.splits > 1 && blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<uint32_t *>(a.part) = 0;
+        return;
+    }
     __syncthreads();                     // the sums' place is the next item's tiles'
     }
 }
 
-// the parts of a row, in their order: one wave a row
+// the parts of the listed rows, in their order: one wave a row
 template <class T, int DP>
 __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
-    const uint64_t all = (uint64_t)a.q_tokens * a.heads, at = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
-    int64_t last = a.cu[a.seqs];
-    if (at >= all || (int64_t)(at / a.heads) < (int64_t)a.cu[0] || (int64_t)(at / a.heads) >= last) return;       // rows behind the last sequence stay as they were
-    const float *stats = a.part + (uint64_t)a.splits * all * DP;
-    const uint32_t parts = reinterpret_cast<const uint32_t *>(stats + (uint64_t)a.splits * all * 2)[at];
-    if (parts == 0 || parts > a.splits) return;
+    const uint32_t used = *reinterpret_cast<const uint32_t *>(a.part);
+    const float *sums = a.sums(), *stats = a.stats(DP);
+    for (uint32_t e = blockIdx.x * 4 + (threadIdx.x >> 6); e < used * a.kv_heads; e += gridDim.x * 4) {
+    const u32x4 row = a.list()[(uint64_t)(e / used) * a.list_room + e % used];
+    const uint64_t at = (uint64_t)row[1] << 32 | row[0];
+    const uint32_t first = row[2], parts = row[3];
     float m = NEG_INF, l = 0.0f;
-    if ((uint32_t)lane < parts) { m = stats[(lane * all + at) * 2]; l = stats[(lane * all + at) * 2 + 1]; }
+    if ((uint32_t)lane < parts) { m = stats[(uint64_t)(first + lane) * 2]; l = stats[(uint64_t)(first + lane) * 2 + 1]; }
     float top = m;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
@@ -787,7 +837,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
 #pragma unroll
         for (int u = 0; u < 8; ++u)
 #pragma unroll
-            for (int x = 0; x < PER; ++x) r[u][x] = a.part[(min(i + u, parts - 1) * all + at) * DP + (d < DP ? d : 0) + x];
+            for (int x = 0; x < PER; ++x) r[u][x] = sums[(uint64_t)(first + min(i + u, parts - 1)) * DP + (d < DP ? d : 0) + x];
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
             const float c = __shfl(w, (int)min(i + u, 63u));
@@ -800,6 +850,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
     for (int x = 0; x < PER; ++x)
         if ((uint32_t)(d + x) < a.dim) dst[d + x] = (T)(total == 0.0f ? 0.0f : v[x] / total);
     if (a.lse && lane == 0) a.lse[at] = total == 0.0f ? NEG_INF : (top + __builtin_amdgcn_logf(total)) * 0.69314718055994530942f;
+    }
 }
 
 static int padded_dim(uint32_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
@@ -807,9 +858,14 @@ static int padded_dim(uint32_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 struct AttnPlan {
     bool split;
     uint32_t slots, splits, chunk, grid;
+    uint32_t room, list_room;  // places of a key head's parts, of its rows that are joined
+    bool coarser;              // there may be more parts than places: then they are made larger
     uint64_t workspace;
 };
-// Which form, and into how many parts the keys are cut.
+// Which form, and into how many parts the keys are cut. How long each sequence is stands in device memory: the longest may have all keys, or every one of
+// them (shared keys). The workspace holds no more than 8 rounds of resident workgroups' parts, 32 rows each; where places for every row at the largest number of
+// parts would take more, the kernel counts what the sequences want, and makes parts larger until they fit. (With a place for each 10000 texts of 30 tokens,
+// 32 heads x 128, took 298 GiB, now 66 MiB; 900 tokens over 32768 keys, 32 / 8 heads x 128, 915 MiB and 2.53 ms, now 66 and 1.82.)
 static AttnPlan plan_attention(const shodh_attention_cfg *c, int cus) {
     AttnPlan p;
     const uint64_t group = c->heads / c->kv_heads, rows = c->q_tokens * group;
@@ -817,6 +873,8 @@ static AttnPlan plan_attention(const shodh_attention_cfg *c, int cus) {
     p.split = rows <= 32ull * c->seqs || tiles < (uint64_t)cus;
     p.slots = (uint32_t)(rows / (p.split ? 32 : 128) + c->seqs);
     p.splits = p.chunk = p.grid = 1;
+    p.room = p.list_room = 0;
+    p.coarser = false;
     p.workspace = 0;
     if (p.split) {
         uint64_t seen = c->kv_tokens;
@@ -834,7 +892,13 @@ static AttnPlan plan_attention(const shodh_attention_cfg *c, int cus) {
         p.chunk = (uint32_t)chunk;
         const uint64_t items = groups * p.splits, resident = (uint64_t)cus * (dp == 128 ? 2 : 4);
         p.grid = (uint32_t)(items < resident ? items : resident);
-        if (p.splits > 1) p.workspace = (p.splits * (uint64_t)(dp + 2) + 1) * c->q_tokens * c->heads * 4;
+        if (p.splits > 1) {
+            const uint64_t most = 8 * resident * 32 / c->kv_heads + 2, each = rows * p.splits;
+            p.coarser = each > most;
+            p.room = (uint32_t)(p.coarser ? most : each);
+            p.list_room = p.room / 2;          // (a row that is joined has two parts or more)
+            p.workspace = 16 + c->kv_heads * (16ull * p.list_room + (uint64_t)p.room * (dp + 2) * 4);
+        }
     }
     return p;
 }
@@ -846,15 +910,14 @@ static int check_attention(const shodh_attention_cfg *c) {
     if (c->head_dim == 0 || c->head_dim % 8 != 0 || c->head_dim > 128) { set_error("attention: head_dim %u is no multiple of 8 up to 128", c->head_dim); return SHODH_ERR_UNSUPPORTED; }
     if (!(c->scale == c->scale) || c->scale > 2.0e38f || c->scale < -2.0e38f /* (times log2 e, in f32) */) { set_error("attention: scale is no number, or too large"); return SHODH_ERR_INVALID; }
     if (c->q_tokens > (uint64_t)MOST_KEYS / (c->heads / c->kv_heads) || c->kv_tokens > (1ull << 40) || c->heads > 65535u || c->seqs > 0x3FFFFFFFu || c->sinks > 0x7FFFFFFFu) { set_error("attention: a size is out of range"); return SHODH_ERR_UNSUPPORTED; }
-    if (c->q_tokens * (c->heads / c->kv_heads) / 32 + c->seqs > 0x7FFFFFFFull / c->kv_heads) { set_error("attention: too many rows for one launch"); return SHODH_ERR_UNSUPPORTED; }
+    const uint64_t rows = c->q_tokens * (c->heads / c->kv_heads);
+    if (rows / 32 + c->seqs > 0x7FFFFFFFull / c->kv_heads || (rows > 32ull * c->seqs && (rows / 128 + c->seqs) * c->kv_heads >= (1u << 24) /* of 256 threads: a launch has fewer than 2^32 */)) { set_error("attention: too many rows for one launch"); return SHODH_ERR_UNSUPPORTED; }
     return SHODH_OK;
 }
 
 template <class T, int DP, bool DMA>
 static int launch_attention(const AttnArgs &a, const AttnPlan &p, hipStream_t st) {
-    // a launch has fewer than 2^32 threads
-    const uint64_t tiles = (uint64_t)p.slots * a.kv_heads, joins = ceil_div((uint64_t)a.q_tokens * a.heads, 4);
-    if ((p.split ? p.splits > 1 ? joins : 0 : tiles) >= (1u << 24)) { set_error("attention: too many rows for one launch"); return SHODH_ERR_UNSUPPORTED; }
+    const uint64_t tiles = (uint64_t)p.slots * a.kv_heads;
     if (!p.split) {
         constexpr size_t lds = 4 * 64 * DP * 2;
         SHODH_TRY(ensure_dynamic_lds((const void *)attn_tile_kernel<T, DP, DMA>, lds));
@@ -862,12 +925,13 @@ static int launch_attention(const AttnArgs &a, const AttnPlan &p, hipStream_t st
         SHODH_HIP_TRY(hipGetLastError());
         return SHODH_OK;
     }
-    constexpr size_t lds = 8 * 32 * DP * 2 + 1024 + 64 * 36 + DP * 64;          // tiles or sums, statistics, the table of sequences, queries
+    constexpr size_t lds = 8 * 32 * DP * 2 + 1024 + 64 * 44 + 16 + DP * 64;          // tiles or sums, statistics, the table of sequences, queries
     SHODH_TRY(ensure_dynamic_lds((const void *)attn_split_kernel<T, DP, DMA>, lds));
     hipLaunchKernelGGL((attn_split_kernel<T, DP, DMA>), dim3(p.grid), dim3(256), lds, st, a);
     SHODH_HIP_TRY(hipGetLastError());
     if (p.splits > 1) {
-        hipLaunchKernelGGL((attn_join_kernel<T, DP>), dim3((uint32_t)joins), dim3(256), 0, st, a);
+        const uint64_t rows = (uint64_t)a.q_tokens * a.heads, listed = (uint64_t)p.list_room * a.kv_heads, joins = ceil_div(rows < listed ? rows : listed, 4);
+        hipLaunchKernelGGL((attn_join_kernel<T, DP>), dim3((uint32_t)(joins < 4096 ? joins : 4096)), dim3(256), 0, st, a);
         SHODH_HIP_TRY(hipGetLastError());
     }
     return SHODH_OK;
@@ -936,7 +1000,7 @@ int shodh_window_attention_device(int device, const shodh_attention_cfg *cfg, co
     a.q = d_q; a.k = d_k; a.v = d_v; a.out = d_out; a.lse = d_lse; a.cu = d_cu; a.kv_start = d_kv_start; a.kv_len = d_kv_len; a.part = (float *)d_workspace;
     a.q_tokens = (int64_t)cfg->q_tokens; a.kv_tokens = (int64_t)cfg->kv_tokens;
     a.heads = cfg->heads; a.kv_heads = cfg->kv_heads; a.group = cfg->heads / cfg->kv_heads; a.shift = (a.group & (a.group - 1)) == 0 ? __builtin_ctz(a.group) : -1; a.dim = cfg->head_dim; a.seqs = cfg->seqs;
-    a.slots = p.slots; a.splits = p.splits; a.chunk = p.chunk; a.sinks = cfg->sinks; a.left = cfg->left; a.right = cfg->right;
+    a.slots = p.slots; a.splits = p.splits; a.chunk = p.chunk; a.room = p.room; a.list_room = p.list_room; a.coarser = p.coarser; a.sinks = cfg->sinks; a.left = cfg->left; a.right = cfg->right;
     const float scale = cfg->scale == 0.0f ? 1.0f / __builtin_sqrtf((float)d) : cfg->scale;
     a.scale2 = __builtin_fabsf(scale) * 1.44269504088896340736f;
     a.sign = scale < 0.0f ? 0x80008000u : 0u;

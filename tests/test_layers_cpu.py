@@ -117,3 +117,42 @@ def test_attention_of_nothing_needs_no_device(L):
     n = C.c_uint64(7)
     assert L.lib().shodh_window_attention_workspace(0, None, C.byref(n)) == -1 and n.value == 0
     assert L.lib().shodh_window_attention_workspace(0, C.byref(L.AttentionCfg()), None) == -1
+
+
+def workspace(L, **kw):
+    cfg = L.AttentionCfg()
+    L.lib().shodh_attention_cfg_default(C.byref(cfg))
+    for name, value in kw.items():
+        setattr(cfg, name, value)
+    n = C.c_uint64()
+    return L.lib().shodh_window_attention_workspace(0, C.byref(cfg), C.byref(n)), n.value
+
+
+@pytest.mark.parametrize("texts,tokens,heads,kv_heads,dim,left,right", [
+    (1024, 20, 32, 32, 128, -1, -1), (10000, 30, 12, 12, 32, -1, -1), (10000, 30, 32, 32, 128, -1, -1), (10000, 30, 32, 32, 128, 4095, 0), (4096, 8, 32, 8, 128, -1, 0),
+    (100000, 12, 32, 8, 128, -1, -1), (20000, 31, 12, 12, 64, -1, -1)])
+def test_attention_workspace_of_many_short_texts(L, texts, tokens, heads, kv_heads, dim, left, right):
+    """parts for what fills the card (8 rounds of at most 4 workgroups a CU, 32 rows each), not for what the longest sequence could be in all rows"""
+    n = texts * tokens
+    rc, need = workspace(L, q_tokens=n, kv_tokens=n, seqs=texts, heads=heads, kv_heads=kv_heads, head_dim=dim, left=left, right=right)
+    resident = 256 * (2 if dim == 128 else 4)
+    assert rc == 0 and need <= 16 + (8 * resident * 32 + 2 * kv_heads) * ((dim + 2) * 4 + 8)
+
+
+@pytest.mark.parametrize("tokens,keys,heads,kv_heads,seqs", [(900, 32768, 32, 8, 1), (4000, 4000, 8, 1, 1), (256, 256 * 32768, 32, 8, 256), (5, 1 << 20, 64, 8, 1)])
+def test_attention_workspace_of_prompts_and_caches(L, tokens, keys, heads, kv_heads, seqs):
+    rc, need = workspace(L, q_tokens=tokens, kv_tokens=keys, seqs=seqs, heads=heads, kv_heads=kv_heads, head_dim=128, right=0)
+    assert rc == 0 and need <= 16 + (8 * 512 * 32 + 2 * kv_heads) * (130 * 4 + 8)
+    if tokens < 100:          # (few rows: no more than every row's parts take)
+        assert need <= 16 + tokens * heads * 64 * (130 * 4 + 8)
+
+
+@pytest.mark.parametrize("kw", [dict(q_tokens=1 << 21, kv_tokens=1 << 21, seqs=1 << 18, heads=32, kv_heads=8, head_dim=64), dict(q_tokens=(1 << 26), kv_tokens=(1 << 26), seqs=1, heads=8, kv_heads=8, head_dim=8),
+                                dict(q_tokens=1 << 25, kv_tokens=1 << 25, seqs=1 << 20, heads=64, kv_heads=64, head_dim=128)])
+def test_attention_workspace_is_given_for_calls_that_are_taken(L, kw):
+    """the question and the call have the same limits (no device here: a call that is taken ends at that)"""
+    if torch.cuda.is_available():
+        pytest.skip("pointers of no memory")
+    rc, need = workspace(L, **kw)
+    got = attn(L, work=P if need else None, nwork=need, k=1 << 45, v=1 << 46, out=1 << 47, **kw)
+    assert (rc, got) in ((0, L.ERR_DEVICE), (-8, -8))

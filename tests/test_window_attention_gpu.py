@@ -383,3 +383,64 @@ def test_what_a_dominant_sink_leaves_over(layers, dtype, above, lq, heads):
     h = torch.finfo(t).eps / 2
     tol = (h + 2 * 66 * U * above + 160 * U) * size + h * want.abs() + ((2.0 ** -32 * v0.abs().sum(0) + 2.0 ** -25) if t == torch.float16 else 0)
     assert ((out.double() - want).abs() <= tol * (1 + 1e-6)).all(), float(((out.double() - want).abs() / tol).max())
+
+
+def used_by(call):
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    out = call()
+    torch.cuda.synchronize()
+    return out, torch.cuda.max_memory_allocated() - before
+
+
+@pytest.mark.parametrize("dtype,heads,kv,dim,lq,nk,left", [("bf16", 8, 1, 128, 1500, 9000, -1), ("f16", 8, 1, 128, 1500, 9000, 6000), ("bf16", 24, 1, 64, 611, 30011, -1), ("bf16", 32, 8, 32, 300, 33000, -1)])
+def test_a_prompt_over_a_long_cache(layers, dtype, heads, kv, dim, lq, nk, left):
+    """hundreds of new tokens behind tens of thousands: more parts are wanted than there are places for"""
+    t = TYPES[dtype]
+    q, k, v = normal(70, lq, heads, dim).to(t), normal(71, nk + 5, kv, dim).to(t), normal(72, nk + 5, kv, dim).to(t)
+    start, length = torch.tensor([5], device="cuda"), torch.tensor([nk], dtype=torch.int32, device="cuda")
+    (out, lse), most = used_by(lambda: layers.window_attention(q, k, v, cu_of([lq]), left=left, right=0, sinks=3, kv_start=start, kv_len=length, return_lse=True))
+    assert most <= 160 << 20
+    some = slice(lq - 40, lq)            # (the last queries, as a shorter prompt over the same keys, and the first ones)
+    ref = exact(q[some], k[5:], v[5:], [40], [nk], left, 0, 3, [0])
+    check(out[some], lse[some], ref)
+    ref = exact(q[:40], k[5:], v[5:], [40], [nk - lq + 40], left, 0, 3, [0])
+    check(out[:40], lse[:40], ref)
+
+
+@pytest.mark.parametrize("heads,kv,dim,seqs,lq,nk", [(16, 2, 128, 70, 2, 20000), (32, 4, 128, 300, 4, 2100), (8, 8, 32, 1500, 1, 5000)])
+def test_sequences_that_share_their_keys(layers, heads, kv, dim, seqs, lq, nk):
+    """every sequence over the same cache: the keys are read far more often than there are of them"""
+    q, k, v = normal(73, seqs * lq, heads, dim).bfloat16(), normal(74, nk, kv, dim).bfloat16(), normal(75, nk, kv, dim).bfloat16()
+    start = torch.zeros(seqs, dtype=torch.int64, device="cuda")
+    length = torch.full((seqs,), nk, dtype=torch.int32, device="cuda")
+    for cut in (0, 2):                   # all alike; or of every length, some of them of none
+        if cut:
+            length[::3], length[1::7] = nk // 2, 0
+        (out, lse), most = used_by(lambda: layers.window_attention(q, k, v, cu_of([lq] * seqs), kv_start=start, kv_len=length, return_lse=True))
+        assert most <= 160 << 20
+        for n in (nk, nk // 2, 0):
+            at = (length == n).repeat_interleave(lq)
+            if at.any():
+                rows = int(at.sum())
+                check(out[at][:200], lse[at][:200], exact(q[at][:200], k, v, [min(rows, 200)], [n], -1, -1, 0, [0]))
+                check(out[at][-50:], lse[at][-50:], exact(q[at][-50:], k, v, [min(rows, 50)], [n], -1, -1, 0, [0]))
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(12, 12, 32), (4, 1, 128)])
+def test_thousands_of_short_texts_without_a_window(layers, heads, kv, dim):
+    """and one long text among them"""
+    g = torch.Generator().manual_seed(9)
+    nq = [int(n) for n in torch.randint(0, 51, (10000,), generator=g)]
+    for long in (None, 7001):
+        if long:
+            nq[long] = 3000
+        n = sum(nq)
+        q, k, v = normal(76, n, heads, dim).bfloat16(), normal(77, n, kv, dim).bfloat16(), normal(78, n, kv, dim).bfloat16()
+        (out, lse), most = used_by(lambda: layers.window_attention(q, k, v, cu_of(nq), return_lse=True))
+        assert most <= (160 << 20) + 2 * out.numel() * 2
+        for b in (0, 1, 63, 64, 65, 4999, 7000, 7001, 7002, 9998, 9999):
+            f, c = sum(nq[:b]), nq[b]
+            few = min(c, 60)
+            check(out[f:f + few], lse[f:f + few], exact(q[f:f + few], k[f:f + c], v[f:f + c], [few], [c], -1, -1, 0, [0]))
