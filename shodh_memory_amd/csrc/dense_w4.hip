@@ -388,7 +388,7 @@ __global__ __launch_bounds__(512, FEW && GROUP != 32 ? 6 : MT == 1 && (FEW || X 
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) v[i] = P::load(x_row(i), block * W4_TK, piece_place);
     };
-    auto store_x = [&](const u32x4 (&v)[PIECES]) {          // (LDS serves a wave's accesses in order: only the compiler has to be held)
+    auto store_x = [&](const u32x4 (&v)[PIECES]) {          // (LDS serves a wave's accesses in order: only the compiler has to be held, from its loads of memory too: 9.1 us, and 9.6 with a fence for LDS alone)
         asm volatile("" ::: "memory");
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) P::store(xs, i * STEP + piece_row, piece_place, v[i]);
@@ -465,6 +465,7 @@ __global__ __launch_bounds__(512, 2) void w4_dense_shared_kernel(const W4Args a)
     auto store = [&](const u32x4 (&v)[N], int half) {
 #pragma unroll
         for (int i = 0; i < N; ++i) P::store(xs + half * TILE, i * STEP + piece_row, piece_place, v[i]);
+        wave_lds_order();
 #pragma unroll
         for (int c = 0; c < MINE; c += COLS)
 #pragma unroll

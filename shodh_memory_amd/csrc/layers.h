@@ -25,6 +25,10 @@ __device__ __forceinline__ void load_any(T (&dst)[N], const T *src) { __builtin_
 template <class T, int N>
 __device__ __forceinline__ void store_any(T *dst, const T (&src)[N]) { __builtin_memcpy(__builtin_assume_aligned(dst, sizeof(T)), src, sizeof(T) * N); }
 
+// Between a wave's stores to LDS and loads of what its other lanes stored: LDS serves a wave's accesses in their order, so only the compiler has to be held,
+// which may move a lane's load over stores of its own that it knows to lie elsewhere.
+__device__ __forceinline__ void wave_lds_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local"); }
+
 inline size_t dtype_bytes(uint32_t t) { return t == SHODH_DTYPE_FP32 ? 4 : t == SHODH_DTYPE_INT8 || t == SHODH_DTYPE_E4M3 ? 1 : 2; }
 inline bool is_float_dtype(uint32_t t) { return t == SHODH_DTYPE_FP32 || t == SHODH_DTYPE_BF16 || t == SHODH_DTYPE_FP16; }
 inline bool aligned_to(const void *p, size_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }

@@ -744,6 +744,7 @@ __global__ __launch_bounds__(256, 2) void attn_split_kernel(const AttnArgs a) {
         arrived(!more);                       // V
         if (masked && __builtin_expect(find_values<T, TILE>(Vs, rows.lane), 0)) {
             clear_values<T, 64>(Vs, TILE, rows.lane);
+            wave_lds_order();
             spoiled = true;
         }
         rows.values(Vs, p);
