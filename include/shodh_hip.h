@@ -409,13 +409,15 @@ int shodh_int8_dense_quantized(int device, const float *x, const void *wq, uint3
  * The pieces of a layer that newer towers have and the MiniLM encoder above does not: a host that runs such a tower next to the index builds
  * its layers from these (and finishes the pooled vector with shodh_finalize_pooled). All of them take HIP device pointers, are asynchronous on
  * `stream` (NULL = default stream of `device`), allocate nothing, keep no state between calls and can be captured into a graph; two calls at
- * once are two calls. The calling thread's current device is left as it was. Strides count elements; 0 = packed. Rows and offsets are 64 bits. */
+ * once are two calls. The calling thread's current device is left as it was. Strides count elements; 0 = packed. Offsets are 64 bits.
+ * An output that overlaps an input or another output is refused, but for the places in one that each operator names; views of different columns, heads or rows
+ * of one buffer do not overlap. */
 enum { SHODH_DTYPE_FP16 = 3, SHODH_DTYPE_E4M3 = 4 };     /* for these operators; e4m3 = the OCP 8-bit float with largest value 448 */
 
 /* RMS norm with the residual's addition, and an output in 8 bits with scales:
  *   h = x + residual;  sum = h;  y = h / sqrt(mean(h^2) + eps) * weight;  per group of a row: scale = max |y| / 127 (448), q = round(y / scale)
- * h, the mean and y are f32 inside; every output is rounded once, to nearest even. x [rows][dim], residual and sum likewise (sum may be residual or x
- * itself, y may be x: element for element in place). d_residual, d_sum, d_y and d_q + d_scale may be NULL, one output at least is asked for.
+ * h, the mean and y are f32 inside; every output is rounded once, to nearest even. x [rows][dim], residual and sum likewise (sum and y may be residual or x
+ * itself: element for element in place). d_residual, d_sum, d_y and d_q + d_scale may be NULL, one output at least is asked for.
  * q is of `q_dtype` int8 or e4m3, [rows][dim] bytes; d_scale f32 [rows][ceil(dim / q_group)], one a row with q_group 0. A group whose largest
  * |y| is below 2^-100 is written as scale 0 and zeros; one that holds a NaN or an infinity as scale NaN and zeros: every value reads as NaN. */
 typedef struct {

@@ -726,6 +726,12 @@ int shodh_w4_dense_device(const shodh_w4_weight *w, const void *d_x, uint32_t x_
     if (!aligned_to(d_x, dtype_bytes(x_dtype)) || !aligned_to(d_y, dtype_bytes(y_dtype)) || !aligned_to(d_x_scale, 4) || !aligned_to(d_bias, 4)) {
         set_error("w4: a pointer is not a multiple of its element's size"); return SHODH_ERR_INVALID;
     }
+    const size_t xb = dtype_bytes(x_dtype), yb = dtype_bytes(y_dtype);
+    const Region y(d_y, w->N * yb, rows, ys * yb);
+    if (may_overlap(y, Region(d_x, w->K * xb, rows, xs * xb)) || may_overlap(y, Region(d_x_scale, rows * 4ull)) || may_overlap(y, Region(d_bias, w->N * 4ull)) ||
+        may_overlap(y, Region(w->data, (uint64_t)w->tiles * w->blocks * w->record))) {
+        set_error("w4: y overlaps another operand"); return SHODH_ERR_INVALID;
+    }
     DeviceScope scope;
     SHODH_TRY(scope.enter(w->device));
     W4Args a;

@@ -33,6 +33,41 @@ inline size_t dtype_bytes(uint32_t t) { return t == SHODH_DTYPE_FP32 ? 4 : t == 
 inline bool is_float_dtype(uint32_t t) { return t == SHODH_DTYPE_FP32 || t == SHODH_DTYPE_BF16 || t == SHODH_DTYPE_FP16; }
 inline bool aligned_to(const void *p, size_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
 
+// The bytes of an operand: runs of `width` bytes, n[0] x n[1] of them at distances step[0] and step[1] (bytes). Null, or none of them: no bytes.
+struct Region {
+    const void *p;
+    uint64_t width, n[2], step[2];
+    Region(const void *p, uint64_t width, uint64_t n0 = 1, uint64_t step0 = 0, uint64_t n1 = 1, uint64_t step1 = 0) : p(p), width(width), n{n0, n1}, step{step0, step1} {}
+    bool empty() const { return !p || !width || !n[0] || !n[1]; }
+    // where the runs lie modulo m (0: not modulo anything), as a length from p on
+    unsigned __int128 span(uint64_t m) const {
+        unsigned __int128 s = width;
+        for (int i = 0; i < 2; ++i)
+            if (n[i] > 1 && (m == 0 || step[i] % m != 0)) s += (unsigned __int128)(n[i] - 1) * step[i];
+        return s;
+    }
+};
+inline bool same_place(const Region &a, const Region &b) {
+    if (a.p != b.p || a.width != b.width) return false;
+    for (int i = 0; i < 2; ++i)
+        if (a.n[i] != b.n[i] || (a.n[i] > 1 && a.step[i] != b.step[i])) return false;
+    return true;
+}
+// False only where the two have no byte in common: they lie one behind the other, or in different places of the rows (heads, tokens) of one buffer.
+inline bool may_overlap(const Region &a, const Region &b) {
+    if (a.empty() || b.empty()) return false;
+    const uintptr_t x = (uintptr_t)a.p, y = (uintptr_t)b.p;
+    if (x + a.span(0) <= y || y + b.span(0) <= x) return false;
+    for (const Region *r : {&a, &b})
+        for (int i = 0; i < 2; ++i) {
+            const uint64_t m = r->n[i] > 1 ? r->step[i] : 0;
+            if (m == 0 || a.span(m) > m || b.span(m) > m) continue;
+            const uint64_t apart = y >= x ? (uint64_t)(y - x) % m : (m - (uint64_t)(x - y) % m) % m;
+            if (apart >= a.span(m) && apart + b.span(m) <= m) return false;
+        }
+    return true;
+}
+
 // The calling thread's current device is the caller's (torch keeps its own idea of it): it is switched for the call and put back.
 struct DeviceScope {
     int before = -1;

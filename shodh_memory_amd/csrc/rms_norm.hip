@@ -283,12 +283,24 @@ int shodh_rms_norm_device(int device, const shodh_rms_norm_cfg *cfg, const void 
         set_error("rms_norm: a pointer is not a multiple of its element's size"); return SHODH_ERR_INVALID;
     }
     if (!d_x) { set_error("null argument"); return SHODH_ERR_INVALID; }
+    const uint32_t groups = cfg->q_group ? (uint32_t)ceil_div(dim, cfg->q_group) : 1;
+    {   // sum and y are written element for element by the threads that read x and residual there: in place, but not beside it
+        const uint64_t n = cfg->rows;
+        const Region x(d_x, dim * b, n, xs * b), res(d_residual, dim * b, n, rs * b), weight(d_weight, dim * dtype_bytes(cfg->weight_dtype)),
+            out[4] = {Region(d_sum, dim * b, n, ss * b), Region(d_y, dim * b, n, ys * b), Region(d_q, dim, n, qs), Region(d_scale, groups * 4ull, n, groups * 4ull)};
+        for (int i = 0; i < 4; ++i) {
+            bool bad = may_overlap(out[i], weight);
+            for (const Region *in : {&x, &res}) bad |= !(i < 2 && same_place(out[i], *in)) && may_overlap(out[i], *in);
+            for (int j = 0; j < i; ++j) bad |= may_overlap(out[i], out[j]);
+            if (bad) { set_error("rms_norm: %s overlaps another operand (sum and y may be x or residual themselves)", i == 0 ? "sum" : i == 1 ? "y" : i == 2 ? "q" : "scale"); return SHODH_ERR_INVALID; }
+        }
+    }
     DeviceScope scope;
     SHODH_TRY(scope.enter(device));
     RmsArgs a;
     a.x = d_x; a.residual = d_residual; a.weight = d_weight; a.sum = d_sum; a.y = d_y; a.q = d_q; a.scale = d_scale;
     a.rows = cfg->rows; a.x_stride = xs; a.residual_stride = rs; a.sum_stride = ss; a.y_stride = ys; a.q_stride = qs;
-    a.dim = cfg->dim; a.group_lanes = cfg->q_group / 8; a.groups = cfg->q_group ? (uint32_t)ceil_div(dim, cfg->q_group) : 1;
+    a.dim = cfg->dim; a.group_lanes = cfg->q_group / 8; a.groups = groups;
     a.weight_f32 = cfg->weight_dtype == SHODH_DTYPE_FP32; a.q_dtype = d_q ? cfg->q_dtype : 0; a.eps = cfg->eps;
     hipStream_t st = (hipStream_t)stream;
     // 16-bit types, whole 16-byte pieces: past the caches from 256 MiB on, the size of the last level (what is written does not stay there anyway).

@@ -992,9 +992,20 @@ int shodh_window_attention_device(int device, const shodh_attention_cfg *cfg, co
         !aligned_to(d_kv_len, 4) || !aligned_to(d_workspace, 16)) {
         set_error("attention: a pointer is not a multiple of its element's size (the workspace: of 16)"); return SHODH_ERR_INVALID;
     }
+    const uint64_t n = cfg->q_tokens, kn = cfg->kv_tokens, KV = cfg->kv_heads;
+    const Region q(d_q, d * 2, n, a.q_stride * 2, H, a.q_head * 2), out(d_out, d * 2, n, a.o_stride * 2, H, a.o_head * 2), lse(d_lse, n * H * 4),
+        in[6] = {q, Region(d_k, d * 2, kn, a.k_stride * 2, KV, a.k_head * 2), Region(d_v, d * 2, kn, a.v_stride * 2, KV, a.v_head * 2), Region(d_cu, (cfg->seqs + 1ull) * 4),
+                 Region(d_kv_start, cfg->seqs * 8ull), Region(d_kv_len, cfg->seqs * 4ull)};
+    bool bad = may_overlap(out, lse);
+    for (const Region &r : in) bad |= (!(&r == in && same_place(out, q)) && may_overlap(out, r)) || may_overlap(lse, r);
+    if (bad) { set_error("attention: out or lse overlaps another operand (out may be q itself)"); return SHODH_ERR_INVALID; }
     DeviceScope scope;
     SHODH_TRY(scope.enter(device));
     const AttnPlan p = plan_attention(cfg, compute_units(device));
+    const Region work(d_workspace, p.workspace);
+    bad = may_overlap(work, out) || may_overlap(work, lse);
+    for (const Region &r : in) bad |= may_overlap(work, r);
+    if (bad) { set_error("attention: the workspace overlaps another operand"); return SHODH_ERR_INVALID; }
     if (p.workspace && (!d_workspace || workspace_bytes < p.workspace)) {
         set_error("attention: a workspace of %llu bytes is needed (%llu given)", (unsigned long long)p.workspace, (unsigned long long)(d_workspace ? workspace_bytes : 0)); return SHODH_ERR_INVALID;
     }

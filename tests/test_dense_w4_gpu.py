@@ -264,3 +264,21 @@ def test_refusals(layers):
     with pytest.raises(ShodhError):
         w.dense(x)
     torch.cuda.synchronize()
+
+
+def test_out_that_overlaps_is_refused(layers):
+    """the result over its own inputs would be read by other workgroups; beside them in one buffer it is as good as anywhere"""
+    from shodh_memory_amd import ShodhError
+    q, packed, scale, z = make(128, 128, 64, True, 12)
+    w = layers.W4Weight.from_quantized(packed, scale, z, group=64)
+    wide = torch.randn(9, 300, device="cuda").half()
+    x, want = wide[:, :128], w.dense(wide[:, :128].contiguous())
+    bias, x8 = torch.zeros(9 * 128, device="cuda"), torch.ones(9, 128, dtype=torch.int8, device="cuda")
+    for call in [lambda: w.dense(x, out=x), lambda: w.dense(x, out=wide[:, 100:228]), lambda: w.dense(x[1:], out=wide[:-1, :128]), lambda: w.dense(x, bias=bias[:128], out=bias.view(9, 128)),
+                 lambda: w.dense(x8, x_scale=bias[:9], out=bias.view(9, 128))]:
+        with pytest.raises(ShodhError):
+            call()
+    assert w.dense(x, out=wide[:, 128:256]).shape == (9, 128) and torch.equal(wide[:, 128:256], want)
+    square = torch.randn(5, 128, device="cuda").half()
+    assert torch.equal(w.dense(square, out=torch.empty_like(square)), w.dense(square))
+    torch.cuda.synchronize()

@@ -154,5 +154,42 @@ def test_attention_workspace_is_given_for_calls_that_are_taken(L, kw):
     if torch.cuda.is_available():
         pytest.skip("pointers of no memory")
     rc, need = workspace(L, **kw)
-    got = attn(L, work=P if need else None, nwork=need, k=1 << 45, v=1 << 46, out=1 << 47, **kw)
+    got = attn(L, work=1 << 48 if need else None, nwork=need, k=1 << 45, v=1 << 46, out=1 << 47, **kw)
     assert (rc, got) in ((0, L.ERR_DEVICE), (-8, -8))
+
+
+X = 1 << 30          # (64 values of 2 bytes x 4 rows are 512 bytes)
+
+
+@pytest.mark.parametrize("taken,kw", [
+    (False, dict(y=X + 2)), (False, dict(y=X - 2)), (False, dict(y=X + 510)), (True, dict(y=X + 512)), (True, dict(y=X - 512)), (True, dict(y=X)), (False, dict(y=X, y_stride=65)), (False, dict(y=X, x_stride=70)),
+    (True, dict(y=X, x_stride=70, y_stride=70)), (True, dict(y=X + 128, x_stride=128, y_stride=128)), (False, dict(y=X + 126, x_stride=128, y_stride=128)), (False, dict(y=X + 130, x_stride=128, y_stride=128)),
+    (True, dict(y=X - 128, x_stride=128, y_stride=128)), (False, dict(y=X - 130, x_stride=128, y_stride=128)), (False, dict(y=X + 128, x_stride=128, y_stride=127)),
+    (True, dict(residual=2 * X, total=2 * X)), (True, dict(residual=2 * X, total=X)), (False, dict(residual=2 * X, total=2 * X + 2)), (False, dict(residual=2 * X, total=2 * X + 128)),
+    (True, dict(residual=2 * X, total=2 * X, y=X)), (True, dict(residual=2 * X, total=X, y=2 * X)), (False, dict(residual=2 * X, total=X, y=X)), (False, dict(residual=2 * X, total=4 * X, y=4 * X + 256)),
+    (False, dict(y=None, q=X, scale=4 * X)), (False, dict(y=None, q=X + 511, scale=4 * X)), (True, dict(y=None, q=X + 512, scale=4 * X)), (False, dict(y=None, q=4 * X, scale=4 * X + 252)), (False, dict(y=None, q=4 * X, scale=X + 4)),
+    (False, dict(y=None, q=4 * X, scale=8 * X, weight=8 * X + 8)), (True, dict(y=None, q=4 * X, scale=4 * X + 256, q_group=32)), (False, dict(y=3 * X + 64, weight=3 * X)), (False, dict(rows=1, y=X + 2)), (True, dict(rows=1, y=X + 128))])
+def test_rms_norm_outputs_that_overlap(L, taken, kw):
+    if torch.cuda.is_available():
+        pytest.skip("pointers of no memory")
+    kw = dict(dict(x=X, weight=3 * X, y=5 * X), **kw)
+    assert rms(L, **kw) == (L.ERR_DEVICE if taken else -1) and ("overlap" in L.last_error()) == (not taken)
+
+
+# q|k|v of 8 tokens side by side: 4 + 2 + 2 heads of 64 values, 1024 bytes a token
+QKV = dict(q=X, k=X + 512, v=X + 768, q_stride=512, k_stride=512, v_stride=512)
+
+
+@pytest.mark.parametrize("taken,kw", [
+    (True, dict(out=2 * X)), (True, dict(QKV, out=X, out_stride=512)), (False, dict(QKV, out=X)), (False, dict(QKV, out=X + 512, out_stride=512)), (False, dict(QKV, out=X + 256, out_stride=512)), (False, dict(QKV, out=X + 2, out_stride=512)),
+    (True, dict(q=X, k=X + 512, v=X + 768, q_stride=1024, k_stride=1024, v_stride=1024, out=X + 1024, out_stride=1024)), (False, dict(q=X, k=X + 512, v=X + 768, q_stride=1024, k_stride=1024, v_stride=1024, out=X + 1022, out_stride=1024)),
+    (True, dict(q=X, k=X + 4096, v=X + 6144, out=X)), (False, dict(q=X, k=X + 4096, v=X + 6144, out=X + 128)), (False, dict(out=2 * X, lse=2 * X + 4092)), (True, dict(out=2 * X, lse=2 * X + 4096)), (False, dict(out=2 * X, lse=X)),
+    (False, dict(out=2 * X, lse=3 * X, cu=3 * X + 4)), (False, dict(out=2 * X, cu=2 * X + 4)), (False, dict(out=2 * X, start=2 * X + 8, length=P)),
+    # head by head: q, k, v and out of a head one after another, and each other head's place in between
+    (True, dict(kv_heads=4, q=X, k=X + 1024, v=X + 2048, out=X + 3072, q_stride=64, k_stride=64, v_stride=64, out_stride=64, q_head_stride=2048, k_head_stride=2048, v_head_stride=2048, out_head_stride=2048)),
+    (False, dict(kv_heads=4, q=X, k=X + 1024, v=X + 2048, out=X + 3070, q_stride=64, k_stride=64, v_stride=64, out_stride=64, q_head_stride=2048, k_head_stride=2048, v_head_stride=2048, out_head_stride=2048))])
+def test_attention_outputs_that_overlap(L, taken, kw):
+    if torch.cuda.is_available():
+        pytest.skip("pointers of no memory")
+    kw = dict(dict(q=X, k=X + 8192, v=X + 16384, cu=7 * X), **kw)
+    assert attn(L, **kw) == (L.ERR_DEVICE if taken else -1) and ("overlap" in L.last_error()) == (not taken)
