@@ -722,7 +722,6 @@ int shodh_w4_dense_device(const shodh_w4_weight *w, const void *d_x, uint32_t x_
     if ((x_dtype == SHODH_DTYPE_INT8) != (d_x_scale != nullptr)) { set_error("w4: int8 rows come with a scale each, others with none"); return SHODH_ERR_INVALID; }
     const uint64_t xs = x_stride ? x_stride : w->K, ys = y_stride ? y_stride : w->N;
     if (rows > 1 && ys < w->N) { set_error("w4: y's rows overlap (stride %llu below %u)", (unsigned long long)ys, w->N); return SHODH_ERR_DIM; }
-    if (rows > 32u * 65535u) { set_error("w4: %u rows: at most 2097120", rows); return SHODH_ERR_UNSUPPORTED; }
     if (!aligned_to(d_x, dtype_bytes(x_dtype)) || !aligned_to(d_y, dtype_bytes(y_dtype)) || !aligned_to(d_x_scale, 4) || !aligned_to(d_bias, 4)) {
         set_error("w4: a pointer is not a multiple of its element's size"); return SHODH_ERR_INVALID;
     }
@@ -735,17 +734,19 @@ int shodh_w4_dense_device(const shodh_w4_weight *w, const void *d_x, uint32_t x_
     DeviceScope scope;
     SHODH_TRY(scope.enter(w->device));
     W4Args a;
-    a.w = w->data; a.x = d_x; a.x_scale = d_x_scale; a.bias = d_bias; a.y = d_y; a.x_stride = xs; a.y_stride = ys;
-    a.M = rows; a.N = w->N; a.K = w->K; a.blocks = w->blocks; a.record = w->record; a.y_dtype = y_dtype;
+    a.w = w->data; a.bias = d_bias; a.x_stride = xs; a.y_stride = ys; a.N = w->N; a.K = w->K; a.blocks = w->blocks; a.record = w->record; a.y_dtype = y_dtype;
     a.f16_mask = w->scale_dtype == SHODH_DTYPE_FP16 ? 0xFFFFFFFFu : 0u;
     a.zero_at = w->zeros ? 1024 + (W4_TK / w->group) * 32 : 1024; a.zero_mask = w->zeros ? 0xFFFFFFFFu : 0u; a.zero_else = w->zeros ? 0u : 0x18181818u;
     hipStream_t st = (hipStream_t)stream;
-    switch (x_dtype) {
-        case SHODH_DTYPE_BF16: return pick_w4<W4_BF16>(a, w, st);
-        case SHODH_DTYPE_FP16: return pick_w4<W4_F16>(a, w, st);
-        case SHODH_DTYPE_FP32: return pick_w4<W4_F32>(a, w, st);
-        default: return pick_w4<W4_I8>(a, w, st);
+    // A launch has at most 65535 workgroups of 32 rows or more, and fewer than 2^31 threads (512 for each tile of outputs): further rows in turns.
+    const uint32_t most = 0x7FFFFFFFu / (w->tiles * 512u), turn = 32u * (most < 65535u ? most : 65535u);
+    for (uint64_t r = 0; r < rows; r += turn) {
+        a.x = (const uint8_t *)d_x + r * xs * xb; a.y = (uint8_t *)d_y + r * ys * yb; a.x_scale = d_x_scale ? d_x_scale + r : nullptr;
+        a.M = (uint32_t)(rows - r < turn ? rows - r : turn);
+        SHODH_TRY(x_dtype == SHODH_DTYPE_BF16 ? pick_w4<W4_BF16>(a, w, st) : x_dtype == SHODH_DTYPE_FP16 ? pick_w4<W4_F16>(a, w, st) : x_dtype == SHODH_DTYPE_FP32 ? pick_w4<W4_F32>(a, w, st) :
+                                                                                                                                                                   pick_w4<W4_I8>(a, w, st));
     }
+    return SHODH_OK;
 }
 
 }  // extern "C"

@@ -282,3 +282,19 @@ def test_out_that_overlaps_is_refused(layers):
     square = torch.randn(5, 128, device="cuda").half()
     assert torch.equal(w.dense(square, out=torch.empty_like(square)), w.dense(square))
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("n,rows", [(16, 32 * 65535 + 50), (1048560, 2100)])
+def test_more_rows_than_a_launch_takes(layers, n, rows):
+    """in turns: every row is what it is in a call of its own"""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    packed = torch.randint(0, 256, (n, 16), generator=g, dtype=torch.uint8, device="cuda")
+    w = layers.W4Weight.from_quantized(packed, torch.full((n, 1), 0.03, device="cuda"), group=32)
+    x = torch.randn(rows, 32, generator=g, device="cuda").bfloat16()
+    out = w.dense(x)
+    for r in (0, 2047, 2048, 2099, rows - 50, rows - 1):
+        assert torch.equal(out[r:r + 1], w.dense(x[r:r + 1])), r
+    x8, xs = torch.randint(-127, 128, (rows, 32), generator=g, device="cuda").to(torch.int8), torch.rand(rows, generator=g, device="cuda")
+    w.dense(x8, x_scale=xs, out=out)
+    for r in (0, 2048, rows - 1):
+        assert torch.equal(out[r:r + 1], w.dense(x8[r:r + 1], x_scale=xs[r:r + 1])), r
