@@ -20,6 +20,13 @@ def _refuse(msg, code=L.ERR_INVALID):
     raise L.ShodhError(code, msg)
 
 
+def _u32(code=L.ERR_UNSUPPORTED, **sizes):
+    """sizes that the C boundary takes in 32 bits (ctypes would cut them off without a word)"""
+    for name, n in sizes.items():
+        if not 0 <= n < 2 ** 32:
+            _refuse("%s %d is no 32-bit number" % (name, n), code)
+
+
 def _dtype(t, name):
     d = _DTYPES.get(t.dtype)
     if d is None:
@@ -89,6 +96,8 @@ def rms_norm(x, weight, eps=1e-6, residual=None, want_y=True, quant=None, group=
         _refuse("x is on %s: there is no CPU fallback" % device, L.ERR_DEVICE)
     dt = _dtype(x, "x")
     rows, dim, xs = _matrix(x, "x")
+    if dim >= 2 ** 32 or not 0 <= group < 2 ** 32:
+        _u32(dim=dim, group=group)
     if weight.dim() != 1 or weight.shape[0] != dim or (dim > 1 and weight.stride(0) != 1):
         _refuse("weight has to be contiguous [%d]" % dim, L.ERR_DIM)
     _on(weight, device, "weight")
@@ -151,6 +160,7 @@ class W4Weight:
         w = torch.as_tensor(w, dtype=torch.float32, device="cpu").contiguous()
         if w.dim() != 2:
             _refuse("the weight has to be [N, K]", L.ERR_DIM)
+        _u32(outputs=w.shape[0], inputs=w.shape[1], group=group)
         h = C.c_void_p()
         L.check(L.lib().shodh_w4_weight_quantize(int(device), w.data_ptr(), w.shape[0], w.shape[1], group, int(bool(zeros)), cls._scale_dtype(scale_dtype), C.byref(h)))
         return cls(h, torch.device("cuda", int(device)))
@@ -169,6 +179,7 @@ class W4Weight:
             _refuse("q has %d bytes a row, %d inputs need %d" % (q.shape[1], k, (k + 1) // 2), L.ERR_DIM)
         if group not in (32, 64, 128):
             _refuse("group %r is none of 32, 64, 128" % (group,), L.ERR_UNSUPPORTED)
+        _u32(outputs=n, inputs=k)
         shape = (n, -(-k // group))
         if tuple(scale.shape) != shape or (zeros is not None and (tuple(zeros.shape) != shape or zeros.dtype != torch.uint8)):
             _refuse("scale (and uint8 zeros) have to be %s" % (shape,), L.ERR_DIM)
@@ -202,6 +213,8 @@ class W4Weight:
         rows, k, xs = _matrix(x, "x")
         if k != self.k:
             _refuse("x has %d columns, the weight %d inputs" % (k, self.k), L.ERR_DIM)
+        if rows >= 2 ** 32:
+            _u32(rows=rows)
         _on(x, self.device, "x")
         sp = bp = None
         if x.dtype == torch.int8:
@@ -311,10 +324,12 @@ def window_attention(q, k, v, cu, left=-1, right=-1, sinks=0, kv_start=None, kv_
         if out.shape != q.shape:
             _refuse("out has to be of q's shape", L.ERR_DIM)
         os_, oh = _heads(out, "out", device, q.dtype)
-    if sinks < 0 or not -2 ** 31 <= left < 2 ** 31 or not -2 ** 31 <= right < 2 ** 31:
+    if not 0 <= sinks < 2 ** 31 or not -2 ** 31 <= left < 2 ** 31 or not -2 ** 31 <= right < 2 ** 31:
         _refuse("left, right and sinks are 32-bit numbers, sinks 0 or more")
-    if scale is not None and not scale != 0:
-        _refuse("scale 0 (or no number)")
+    if heads >= 2 ** 32 or kv_heads >= 2 ** 32 or dim >= 2 ** 32 or seqs >= 2 ** 32:
+        _u32(heads=heads, kv_heads=kv_heads, head_dim=dim, sequences=seqs)
+    if scale is not None and not C.c_float(scale).value != 0:
+        _refuse("scale 0 in f32 (or no number)")
     lse = _new(n, heads, torch.float32, device) if return_lse else None
     if n and seqs:
         cfg = L.AttentionCfg(n, kn, qs, qh, ks, kh, vs, vh, os_, oh, dt, heads, kv_heads, dim, seqs, sinks, left, right, scale or 0.0, 0)

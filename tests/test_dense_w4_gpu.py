@@ -298,3 +298,14 @@ def test_more_rows_than_a_launch_takes(layers, n, rows):
     w.dense(x8, x_scale=xs, out=out)
     for r in (0, 2048, rows - 1):
         assert torch.equal(out[r:r + 1], w.dense(x8[r:r + 1], x_scale=xs[r:r + 1])), r
+
+
+def test_sizes_that_32_bits_cannot_hold(layers):
+    from shodh_memory_amd import ShodhError
+    q, packed, scale, z = make(16, 32, 32, False, 1)
+    w = layers.W4Weight.from_quantized(packed, scale, group=32)
+    held = torch.zeros(2 ** 32 + 64, dtype=torch.bfloat16, device="cuda")
+    for call in [lambda: w.dense(held.as_strided((2 ** 32 + 1, 32), (1, 1))), lambda: w.dense(held.as_strided((2 ** 32, 32), (1, 1))), lambda: layers.W4Weight.quantize(torch.zeros(16, 32), group=2 ** 32 + 32),
+                 lambda: layers.W4Weight.quantize(torch.zeros(16, 32), group=-32)]:
+        with pytest.raises(ShodhError):
+            call()

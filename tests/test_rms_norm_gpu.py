@@ -205,3 +205,16 @@ def test_refusals(layers):
         with pytest.raises(ShodhError):
             call()
     torch.cuda.synchronize()
+
+
+def test_sizes_that_32_bits_cannot_hold(layers):
+    """(a group of 2^32 + 32 would be taken as 32, and scales written for it where one a row has room)"""
+    from shodh_memory_amd import ShodhError
+    x, w = torch.randn(4, 256, device="cuda"), torch.ones(256, device="cuda")
+    for group in (2 ** 32, 2 ** 32 + 32, -32, -2 ** 32 + 64):
+        with pytest.raises(ShodhError):
+            layers.rms_norm(x, w, quant="int8", group=group)
+    wide = torch.empty(2 ** 32 + 64, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ShodhError):
+        layers.rms_norm(wide[None], wide)
+    torch.cuda.synchronize()

@@ -444,3 +444,12 @@ def test_thousands_of_short_texts_without_a_window(layers, heads, kv, dim):
             f, c = sum(nq[:b]), nq[b]
             few = min(c, 60)
             check(out[f:f + few], lse[f:f + few], exact(q[f:f + few], k[f:f + c], v[f:f + c], [few], [c], -1, -1, 0, [0]))
+
+
+def test_numbers_that_32_bits_cannot_hold(layers):
+    from shodh_memory_amd import ShodhError
+    q, k, v, cu = normal(1, 6, 4, 64).bfloat16(), normal(2, 6, 2, 64).bfloat16(), normal(3, 6, 2, 64).bfloat16(), cu_of([6])
+    for kw in [dict(sinks=2 ** 32 + 4), dict(sinks=2 ** 32), dict(sinks=2 ** 31), dict(left=2 ** 31), dict(left=-2 ** 31 - 1), dict(right=2 ** 32), dict(scale=1e-46), dict(scale=-1e-60), dict(scale=1e39)]:
+        with pytest.raises(ShodhError):
+            layers.window_attention(q, k, v, cu, **kw)
+    torch.cuda.synchronize()
