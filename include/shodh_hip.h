@@ -438,7 +438,7 @@ int shodh_rms_norm_device(int device, const shodh_rms_norm_cfg *cfg, const void 
  *   y[m][n] = sum_k x[m][k] * (q[n][k] - z[n][k / group]) * s[n][k / group] * x_scale[m] + bias[n]
  * A weight is laid out once; the handle is read-only afterwards (any number of calls at once). q: [N][ceil(K / 2)] bytes, two inputs a byte, the even one
  * in the low bits; scale f32 [N][ceil(K / group)], kept in `scale_dtype` (fp16 or bf16: values that are numbers of that type already stay what they
- * are); zero [N][ceil(K / group)] bytes 0 .. 15, NULL = 8 everywhere. group 32, 64 or 128; N and K any.
+ * are, others are rounded; one that is too large, or not 0 and so small that it would be off by more than half a step of the type, is refused); zero [N][ceil(K / group)] bytes 0 .. 15, NULL = 8 everywhere. group 32, 64 or 128; N and K any.
  * _create takes host data, _create_device device data (both wait for the device and are refused while `stream` is captured); _quantize rounds f32 weights itself:
  * per group scale = max |w| / 7, or (max - min) / 15 with zero points. */
 typedef struct shodh_w4_weight shodh_w4_weight;

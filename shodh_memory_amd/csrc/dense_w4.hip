@@ -59,6 +59,7 @@ __global__ __launch_bounds__(256) void w4_pack_kernel(const uint8_t *__restrict_
         const float s = in ? scale[(size_t)m * groups + g] : 0.0f;
         const S r = (S)s;
         if (!(__builtin_fabsf((float)r) < __builtin_inff())) atomicOr(bad, 1u);
+        else if (__builtin_fabsf((float)r - s) > __builtin_fabsf(s) * (std::is_same_v<S, _Float16> ? 0x1p-11f : 0x1p-8f)) atomicOr(bad, 8u);       // more than its half step: too small for S
         reinterpret_cast<S *>(rec + 1024)[t] = r;
         if (zero) {
             const uint32_t z = in ? zero[(size_t)m * groups + g] : 8u;
@@ -595,6 +596,7 @@ static int lay_out(int device, const uint8_t *q, const float *scale, const uint8
         (void)dev_free(w->data); delete w;
         if (e != hipSuccess) { set_error("w4: laying out failed: %s", hipGetErrorString(e)); return SHODH_ERR_DEVICE; }
         if (bad & 2u) { set_error("w4: a zero point is over 15"); return SHODH_ERR_INVALID; }
+        if ((bad & 13u) == 8u) { set_error("w4: a scale is not 0 but below what its 16-bit type holds%s", scale_dtype == SHODH_DTYPE_FP16 ? " (bf16 reaches further)" : ""); return SHODH_ERR_INVALID; }
         set_error(bad & 4u ? "w4: a weight is a NaN or an infinity" : "w4: a scale is no finite number of its 16-bit type"); return SHODH_ERR_NONFINITE;
     }
     *out = w;

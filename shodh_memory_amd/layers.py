@@ -166,9 +166,10 @@ class W4Weight:
         return cls(h, torch.device("cuda", int(device)))
 
     @classmethod
-    def from_quantized(cls, q, scale, zeros=None, k=None, group=128, scale_dtype=torch.float16, device=0):
+    def from_quantized(cls, q, scale, zeros=None, k=None, group=128, scale_dtype=None, device=0):
         """q uint8 [N, ceil(K / 2)] (two inputs a byte, the even one in the low bits), scale [N, ceil(K / group)], zeros uint8 of scale's shape or None (8):
-        device tensors (their device is used) or host tensors / arrays (`device`)."""
+        device tensors (their device is used) or host tensors / arrays (`device`). Scales are kept as they are in fp16 and bf16, others in fp16 unless
+        scale_dtype says otherwise; those that the type cannot hold to half a step are refused."""
         q, scale = torch.as_tensor(q), torch.as_tensor(scale)
         zeros = None if zeros is None else torch.as_tensor(zeros)
         if q.dim() != 2 or q.dtype != torch.uint8:
@@ -183,7 +184,7 @@ class W4Weight:
         shape = (n, -(-k // group))
         if tuple(scale.shape) != shape or (zeros is not None and (tuple(zeros.shape) != shape or zeros.dtype != torch.uint8)):
             _refuse("scale (and uint8 zeros) have to be %s" % (shape,), L.ERR_DIM)
-        sd = cls._scale_dtype(scale_dtype)
+        sd = cls._scale_dtype(scale_dtype or (torch.bfloat16 if scale.dtype == torch.bfloat16 else torch.float16))
         for t, name in ((scale, "scale"), (zeros, "zeros")):
             if t is not None:
                 _on(t, q.device, name)

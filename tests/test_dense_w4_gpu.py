@@ -309,3 +309,37 @@ def test_sizes_that_32_bits_cannot_hold(layers):
                  lambda: layers.W4Weight.quantize(torch.zeros(16, 32), group=-32)]:
         with pytest.raises(ShodhError):
             call()
+
+
+def test_scales_keep_their_type(layers):
+    """bf16 scales are kept as they are, however small; scales that a type cannot hold to half its step are refused in it"""
+    from shodh_memory_amd import ShodhError
+    W = layers.W4Weight
+    q, packed, _, z = make(16, 96, 32, True, 5)
+    each = (q.double() - z.cpu().double()[:, torch.arange(96) // 32])
+    for value in (1.0, 1e-6, 1e-7, 2e-8, 1e-20, 3e38, 0.0):
+        for scale in (torch.full((16, 3), value, device="cuda").bfloat16(), torch.full((16, 3), value).bfloat16()):
+            zz, pp = (z, packed) if scale.is_cuda else (z.cpu(), packed.cpu())
+            w = W.from_quantized(pp, scale, zz, group=32) if value < 1e38 else None
+            if w is not None:
+                assert torch.equal(w.dequantize(), (each * scale.cpu().double()[:, torch.arange(96) // 32]).float())
+        half = torch.full((16, 3), value, device="cuda").half()
+        if torch.isfinite(half).all():           # what is a number of fp16 already stays what it is, the smallest ones too
+            w = W.from_quantized(packed, half, z, group=32)
+            assert torch.equal(w.dequantize(), (each * half.cpu().double()[:, torch.arange(96) // 32]).float())
+        for dtype, least in ((None, 2.0 ** -14), (torch.float16, 2.0 ** -14), (torch.bfloat16, 2.0 ** -126)):
+            f = torch.full((16, 3), 0.05, device="cuda")
+            f[7, 2] = value
+            largest = 65504 if dtype is not torch.bfloat16 else 3.38e38
+            if value and not least <= value <= largest:
+                with pytest.raises(ShodhError):
+                    W.from_quantized(packed, f, z, group=32, scale_dtype=dtype)
+            else:
+                d = W.from_quantized(packed, f, z, group=32, scale_dtype=dtype).dequantize().double()
+                want = each * f.cpu().double()[:, torch.arange(96) // 32]
+                over = want.abs() > 3.5e38           # 2 x 3e38 and more: no numbers of dequantize's f32 (its largest is 3.403e38), but infinities of their sign
+                assert torch.equal(d[over], torch.sign(want[over]) * float("inf"))
+                assert ((d - want).abs() <= torch.finfo(dtype or torch.float16).eps / 2 * want.abs() * (1 + 1e-6))[~over].all()
+    w = 1e-9 * torch.randn(8, 64)
+    assert ((W.quantize(w, group=32, scale_dtype=torch.bfloat16).dequantize() - w).abs().max() <= 1e-9 * 0.4)
+    torch.cuda.synchronize()
