@@ -439,8 +439,9 @@ int shodh_rms_norm_device(int device, const shodh_rms_norm_cfg *cfg, const void 
  * A weight is laid out once; the handle is read-only afterwards (any number of calls at once). q: [N][ceil(K / 2)] bytes, two inputs a byte, the even one
  * in the low bits; scale f32 [N][ceil(K / group)], kept in `scale_dtype` (fp16 or bf16: values that are numbers of that type already stay what they
  * are, others are rounded; one that is too large, or not 0 and so small that it would be off by more than half a step of the type, is refused); zero [N][ceil(K / group)] bytes 0 .. 15, NULL = 8 everywhere. group 32, 64 or 128; N and K any.
- * _create takes host data, _create_device device data (both wait for the device and are refused while `stream` is captured); _quantize rounds f32 weights itself:
- * per group scale = max |w| / 7, or (max - min) / 15 with zero points. */
+ * _create takes host data, _create_device device data in the order of `stream`; _quantize rounds f32 host weights itself: per group scale = max |w| / 7, or
+ * (max - min) / 15 with zero points, rounded to scale_dtype before the weights are (fp16 has no scale below 2^-24: bf16 for weights that small). They return when
+ * the weight is laid out. _create_device is refused while `stream` is captured; the others, _dequantize and _destroy work beside any capture. */
 typedef struct shodh_w4_weight shodh_w4_weight;
 int shodh_w4_weight_create(int device, const uint8_t *q, const float *scale, const uint8_t *zero, uint32_t N, uint32_t K, uint32_t group,
                            uint32_t scale_dtype, shodh_w4_weight **out);
@@ -448,7 +449,7 @@ int shodh_w4_weight_create_device(int device, const uint8_t *d_q, const float *d
                                   uint32_t scale_dtype, void *stream, shodh_w4_weight **out);
 int shodh_w4_weight_quantize(int device, const float *w /* host [N][K] */, uint32_t N, uint32_t K, uint32_t group, uint32_t zeros, uint32_t scale_dtype,
                              shodh_w4_weight **out);
-void shodh_w4_weight_destroy(shodh_w4_weight *w);          /* no call may be in flight on it */
+void shodh_w4_weight_destroy(shodh_w4_weight *w);          /* no call may be in flight on it, and no captured graph that holds one may run afterwards */
 int shodh_w4_weight_dequantize(const shodh_w4_weight *w, float *out /* host [N][K] */);
 int shodh_w4_weight_shape(const shodh_w4_weight *w, uint32_t *N, uint32_t *K, uint32_t *group, uint64_t *bytes);
 /* x [rows][K]: fp32 (exact: three bf16 parts), bf16, fp16, or int8 with one f32 scale a row (what shodh_rms_norm_device writes with q_group 0; sums exact in

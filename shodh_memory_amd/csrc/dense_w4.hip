@@ -629,6 +629,7 @@ int shodh_w4_weight_create_device(int device, const uint8_t *d_q, const float *d
     hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
     SHODH_HIP_TRY(hipStreamIsCapturing((hipStream_t)stream, &capture));
     if (capture != hipStreamCaptureStatusNone) { set_error("w4: weights are not laid out while their stream is captured"); return SHODH_ERR_STATE; }
+    const BesideCaptures beside;
     try {
         Buffers b;
         uint32_t *bad = b.take<uint32_t>(1);
@@ -643,16 +644,19 @@ int shodh_w4_weight_create(int device, const uint8_t *q, const float *scale, con
     if (!q || !scale) { set_error("null argument"); return SHODH_ERR_INVALID; }
     DeviceScope scope;
     SHODH_TRY(scope.enter(device));
+    const BesideCaptures beside;
     try {
         Buffers b;
+        OwnStream own;             // (ends before the buffers do)
+        SHODH_TRY(own.make());
         const size_t nq = (size_t)N * ((K + 1) / 2), ng = (size_t)N * ((K + group - 1) / group);
         uint8_t *dq = b.take<uint8_t>(nq), *dz = zero ? b.take<uint8_t>(ng) : nullptr;
         float *ds = b.take<float>(ng);
         if (!dq || !ds || (zero && !dz)) { set_error("out of HBM"); return SHODH_ERR_OOM; }
-        SHODH_HIP_TRY(hipMemcpy(dq, q, nq, hipMemcpyHostToDevice));
-        SHODH_HIP_TRY(hipMemcpy(ds, scale, ng * 4, hipMemcpyHostToDevice));
-        if (zero) SHODH_HIP_TRY(hipMemcpy(dz, zero, ng, hipMemcpyHostToDevice));
-        return shodh_w4_weight_create_device(device, dq, ds, dz, N, K, group, scale_dtype, nullptr, out);
+        SHODH_HIP_TRY(hipMemcpyAsync(dq, q, nq, hipMemcpyHostToDevice, own.st));
+        SHODH_HIP_TRY(hipMemcpyAsync(ds, scale, ng * 4, hipMemcpyHostToDevice, own.st));
+        if (zero) SHODH_HIP_TRY(hipMemcpyAsync(dz, zero, ng, hipMemcpyHostToDevice, own.st));
+        return shodh_w4_weight_create_device(device, dq, ds, dz, N, K, group, scale_dtype, own.st, out);
     } catch (const std::exception &ex) { set_error("w4: %s", ex.what()); return SHODH_ERR_OOM; }
 }
 
@@ -661,28 +665,32 @@ int shodh_w4_weight_quantize(int device, const float *w, uint32_t N, uint32_t K,
     if (!w) { set_error("null argument"); return SHODH_ERR_INVALID; }
     DeviceScope scope;
     SHODH_TRY(scope.enter(device));
+    const BesideCaptures beside;
     try {
         Buffers b;
+        OwnStream own;
+        SHODH_TRY(own.make());
         const size_t n = (size_t)N * K, ng = (size_t)N * ((K + group - 1) / group), pairs = (size_t)N * ((K + 1) / 2);
         float *dw = b.take<float>(n), *ds = b.take<float>(ng);
         uint8_t *d1 = b.take<uint8_t>(n), *dq = b.take<uint8_t>(pairs), *dz = zeros ? b.take<uint8_t>(ng) : nullptr;
         uint32_t *bad = b.take<uint32_t>(1);
         if (!dw || !ds || !d1 || !dq || (zeros && !dz) || !bad) { set_error("out of HBM"); return SHODH_ERR_OOM; }
-        SHODH_HIP_TRY(hipMemcpy(dw, w, n * 4, hipMemcpyHostToDevice));
-        SHODH_HIP_TRY(hipMemset(bad, 0, 4));
+        SHODH_HIP_TRY(hipMemcpyAsync(dw, w, n * 4, hipMemcpyHostToDevice, own.st));
+        SHODH_HIP_TRY(hipMemsetAsync(bad, 0, 4, own.st));
         const uint32_t ny = N < 32768 ? N : 32768;
         const dim3 grid((K + group - 1) / group, ny, (N + ny - 1) / ny);
-        if (scale_dtype == SHODH_DTYPE_FP16) hipLaunchKernelGGL((w4_quantize_kernel<_Float16>), grid, dim3(64), 0, nullptr, dw, N, K, group, zeros, d1, ds, dz, bad);
-        else hipLaunchKernelGGL((w4_quantize_kernel<__bf16>), grid, dim3(64), 0, nullptr, dw, N, K, group, zeros, d1, ds, dz, bad);
-        hipLaunchKernelGGL(w4_pairs_kernel, dim3((uint32_t)(ceil_div(pairs, 256) < 8192 ? ceil_div(pairs, 256) : 8192)), dim3(256), 0, nullptr, d1, N, K, dq);
+        if (scale_dtype == SHODH_DTYPE_FP16) hipLaunchKernelGGL((w4_quantize_kernel<_Float16>), grid, dim3(64), 0, own.st, dw, N, K, group, zeros, d1, ds, dz, bad);
+        else hipLaunchKernelGGL((w4_quantize_kernel<__bf16>), grid, dim3(64), 0, own.st, dw, N, K, group, zeros, d1, ds, dz, bad);
+        hipLaunchKernelGGL(w4_pairs_kernel, dim3((uint32_t)(ceil_div(pairs, 256) < 8192 ? ceil_div(pairs, 256) : 8192)), dim3(256), 0, own.st, d1, N, K, dq);
         SHODH_HIP_TRY(hipGetLastError());
-        return lay_out(device, dq, ds, dz, N, K, group, scale_dtype, bad, nullptr, out);
+        return lay_out(device, dq, ds, dz, N, K, group, scale_dtype, bad, own.st, out);
     } catch (const std::exception &ex) { set_error("w4: %s", ex.what()); return SHODH_ERR_OOM; }
 }
 
 void shodh_w4_weight_destroy(shodh_w4_weight *w) {
     if (!w) return;
     DeviceScope scope;
+    const BesideCaptures beside;
     if (scope.enter(w->device) == SHODH_OK) (void)dev_free(w->data);
     delete w;
 }
@@ -691,16 +699,20 @@ int shodh_w4_weight_dequantize(const shodh_w4_weight *w, float *out) {
     if (!w || !out) { set_error("null argument"); return SHODH_ERR_INVALID; }
     DeviceScope scope;
     SHODH_TRY(scope.enter(w->device));
+    const BesideCaptures beside;
     try {
         Buffers b;
+        OwnStream own;
+        SHODH_TRY(own.make());
         const size_t n = (size_t)w->N * w->K;
         float *d = b.take<float>(n);
         if (!d) { set_error("out of HBM"); return SHODH_ERR_OOM; }
         const dim3 grid(w->blocks, w->tiles);
-        if (w->scale_dtype == SHODH_DTYPE_FP16) hipLaunchKernelGGL((w4_unpack_kernel<_Float16>), grid, dim3(256), 0, nullptr, w->data, w->N, w->K, w->group, w->blocks, w->record, w->zeros, d);
-        else hipLaunchKernelGGL((w4_unpack_kernel<__bf16>), grid, dim3(256), 0, nullptr, w->data, w->N, w->K, w->group, w->blocks, w->record, w->zeros, d);
+        if (w->scale_dtype == SHODH_DTYPE_FP16) hipLaunchKernelGGL((w4_unpack_kernel<_Float16>), grid, dim3(256), 0, own.st, w->data, w->N, w->K, w->group, w->blocks, w->record, w->zeros, d);
+        else hipLaunchKernelGGL((w4_unpack_kernel<__bf16>), grid, dim3(256), 0, own.st, w->data, w->N, w->K, w->group, w->blocks, w->record, w->zeros, d);
         SHODH_HIP_TRY(hipGetLastError());
-        SHODH_HIP_TRY(hipMemcpy(out, d, n * 4, hipMemcpyDeviceToHost));
+        SHODH_HIP_TRY(hipMemcpyAsync(out, d, n * 4, hipMemcpyDeviceToHost, own.st));
+        SHODH_HIP_TRY(hipStreamSynchronize(own.st));
         return SHODH_OK;
     } catch (const std::exception &ex) { set_error("w4: %s", ex.what()); return SHODH_ERR_OOM; }
 }

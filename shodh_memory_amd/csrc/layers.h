@@ -82,6 +82,20 @@ struct DeviceScope {
     ~DeviceScope() { if (changed) (void)hipSetDevice(before); }
 };
 
+// Allocations and frees of calls that are not captured themselves: a capture of another thread neither refuses them nor is ended by them.
+struct BesideCaptures {
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    BesideCaptures() { (void)hipThreadExchangeStreamCaptureMode(&mode); }
+    ~BesideCaptures() { (void)hipThreadExchangeStreamCaptureMode(&mode); }
+    BesideCaptures(const BesideCaptures &) = delete;
+};
+// ... and a stream of its own for a call on host data (work on the default stream ends a capture)
+struct OwnStream {
+    hipStream_t st = nullptr;
+    int make() { SHODH_HIP_TRY(hipStreamCreateWithFlags(&st, hipStreamNonBlocking)); return SHODH_OK; }
+    ~OwnStream() { if (st) { (void)hipStreamSynchronize(st); (void)hipStreamDestroy(st); } }
+};
+
 int compute_units(int device);      // of an existing device; asked once per device
 
 }  // namespace shodh

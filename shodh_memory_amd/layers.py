@@ -139,7 +139,7 @@ def rms_norm(x, weight, eps=1e-6, residual=None, want_y=True, quant=None, group=
 
 class W4Weight:
     """A dense layer's weights in 4 bits with group scales, laid out on the device once (shodh_w4_weight). The handle is read-only: any number of
-    threads and streams may use it."""
+    threads and streams may use it. It has to outlive the captured graphs that do. Made from device tensors it cannot be while their stream is captured."""
 
     def __init__(self, handle, device):
         self._h, self.device = handle, device
@@ -250,7 +250,7 @@ class W4Weight:
         return out
 
     def close(self):
-        """Frees the device copy (the runtime waits for what was started on it; not while a graph is being captured)."""
+        """Frees the device copy (the runtime waits for what was started on it). Captured graphs that hold a product of this weight may not run afterwards."""
         if self._h is not None:
             h, self._h = self._h, None
             L.lib().shodh_w4_weight_destroy(h)

@@ -343,3 +343,45 @@ def test_scales_keep_their_type(layers):
     w = 1e-9 * torch.randn(8, 64)
     assert ((W.quantize(w, group=32, scale_dtype=torch.bfloat16).dequantize() - w).abs().max() <= 1e-9 * 0.4)
     torch.cuda.synchronize()
+
+
+@needs_capture
+@pytest.mark.parametrize("elsewhere", [True, False])
+def test_weights_come_and_go_beside_a_capture(layers, elsewhere):
+    """made from host data, read back and freed while a graph is captured, by another thread or the same one: the capture is what it would be without"""
+    import threading
+    q, packed, scale, z = make(64, 128, 64, True, 6, device="cpu")
+    w = layers.W4Weight.from_quantized(packed, scale, z, group=64)
+    f, held_weights = torch.randn(40, 96, generator=torch.Generator().manual_seed(3)), [layers.W4Weight.from_quantized(packed, scale, z, group=64) for _ in range(2)]
+    x = torch.randn(2, 128, device="cuda").half()
+    want, made, wrong = w.dense(x), [], []
+
+    def work():
+        try:
+            made.append(layers.W4Weight.from_quantized(packed, scale, z, group=64))
+            made.append(layers.W4Weight.quantize(f, group=32))
+            made.append(made[0].dequantize())
+            held_weights.pop()                       # (collected)
+            held_weights.pop().close()
+        except Exception as e:
+            wrong.append(e)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        first = w.dense(x)
+        if elsewhere:
+            th = threading.Thread(target=work)
+            th.start()
+            th.join()
+        else:
+            work()
+        second = w.dense(x)
+    assert not wrong and not held_weights
+    for k in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(first, want) and torch.equal(second, want)
+        assert torch.equal(made[0].dense(x), want) and torch.equal(made[2], w.dequantize())
+        x.mul_(0.5)
+        want = w.dense(x)
+    assert torch.equal(made[1].dequantize(), layers.W4Weight.quantize(f, group=32).dequantize())
