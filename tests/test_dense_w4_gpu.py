@@ -385,3 +385,39 @@ def test_weights_come_and_go_beside_a_capture(layers, elsewhere):
         x.mul_(0.5)
         want = w.dense(x)
     assert torch.equal(made[1].dequantize(), layers.W4Weight.quantize(f, group=32).dequantize())
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("rows", [1, 2, 3, 5, 16, 17, 64, 100])
+def test_f32_rows_come_through_bit_for_bit(layers, group, rows):
+    """one weight of 1 for each output, all others 0: a row's three parts times 1 add up to the value itself without a rounding, the rest to 0"""
+    for k, n in ((31, 20), (128, 100), (300, 333), (1161, 50)):
+        g = torch.Generator().manual_seed(k + rows)
+        place = torch.randint(0, k, (n,), generator=g)
+        place[0], place[-1] = 0, k - 1
+        z = torch.randint(0, 15, (n, -(-k // group)), generator=g, dtype=torch.uint8)
+        q = z.repeat_interleave(group, 1)[:, :k].contiguous()
+        q[torch.arange(n), place] += 1
+        p = torch.nn.functional.pad(q, (0, k % 2))
+        w = layers.W4Weight.from_quantized(p[:, 0::2] | (p[:, 1::2] << 4), torch.ones(n, z.shape[1]), z, k=k, group=group)
+        x = (torch.randn(rows, k, generator=g) * torch.exp(4 * torch.randn(rows, k, generator=g))).cuda()
+        assert torch.equal(w.dense(x), x[:, place.cuda()])
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_f32_rows_against_the_definition_without_the_16s(layers, group):
+    """f32 rows multiply q - z itself. A product of a part of x (8 bits) with q - z (5 bits) is exact; a group's three sums of G of them, the scale, the sum over
+    groups, the waves and the bias are one u = 2^-23 of what has been added up each: |y - exact| <= (3 G + K / G + 16) u sum |x| |q - z| s (+ |bias|) + u / 2 |exact|.
+    That is a tenth and less of what the form 16 + q would need; rows of one sign and weights whose sum is near 0 would show it."""
+    for i, (m, n, k) in enumerate(SHAPES):
+        for zeros in (False, True):
+            q, packed, scale, z = make(n, k, group, zeros, 13 * i + group)
+            w = layers.W4Weight.from_quantized(packed, scale, z, k=k, group=group)
+            x = rows_of("f32", m, k, i)[0]
+            if i % 2:
+                x = x.abs() + 1
+            y, _ = exact(x, None, q, scale, z, None, group)
+            _, t = exact(x, torch.ones(m), q, scale, z, None, group)
+            off = (w.dense(x).cpu().double() - y).abs()
+            tol = (3 * group + -(-k // group) + 16) * U * t + U / 2 * y.abs()
+            assert (off <= tol).all(), float((off / tol).max())
