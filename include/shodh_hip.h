@@ -454,7 +454,7 @@ int shodh_w4_weight_dequantize(const shodh_w4_weight *w, float *out /* host [N][
 int shodh_w4_weight_shape(const shodh_w4_weight *w, uint32_t *N, uint32_t *K, uint32_t *group, uint64_t *bytes);
 /* x [rows][K]: fp32 (exact: three bf16 parts), bf16, fp16, or int8 with one f32 scale a row (what shodh_rms_norm_device writes with q_group 0; sums exact in
  * int32 per group); bias f32 [N] or NULL; y [rows][N] fp32, bf16 or fp16. Up to 2^32 - 1 rows (made for up to 64: beyond, the weights are read again
- * for each 64). y may not overlap x. A row that holds a NaN or an infinity gives NaN in all its outputs; f32 and bf16 rows are taken up to a sum |x| * 31 in f32's range. */
+ * for each 64). y may not overlap x. A row that holds a NaN or an infinity gives NaN in all its outputs (16-bit rows and fp32 y: what the formula gives); f32 and bf16 rows are taken up to a sum |x| * 31 in f32's range. */
 int shodh_w4_dense_device(const shodh_w4_weight *w, const void *d_x, uint32_t x_dtype, uint64_t x_stride, const float *d_x_scale, uint32_t rows,
                           const float *d_bias, void *d_y, uint32_t y_dtype, uint64_t y_stride, void *stream);
 

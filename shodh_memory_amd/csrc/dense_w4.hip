@@ -10,9 +10,10 @@
 //  * a 4-bit number becomes a matrix operand with a shift and an and-or per PAIR: or-ed into the mantissa of 16.0 it reads as 16 + q, in bf16 as in
 //    fp16, exactly. sum x (16 + q) - (16 + z) sum x is the group's sum; sum x comes from the same matrix instruction with ones for weights, in the same
 //    order. int8 rows multiply q as a byte: sums exact in int32, (q - z) likewise;
-//  * f32 rows are split into three bf16 parts (8 + 8 + 8 bits, by truncation, exact): three products with q - z itself, sums in f32;
+//  * f32 rows are split into three bf16 parts (8 + 8 + 8 bits, by truncation, exact): three products with q - z itself, sums in f32. 16-bit rows with an f32
+//    result are multiplied with q - z too;
 //  * scales multiply the f32 sum of a group, so no weight is rounded to 16 bits on the way.
-// A row of x that holds a NaN or an infinity gives NaN in all its outputs (16 x - 16 x).
+// A row of x that holds a NaN or an infinity gives NaN in all its outputs (16 x - 16 x; f32 parts x - x); 16-bit rows with an f32 result what x (q - z) gives.
 #include "layers.h"
 
 #include <cstddef>
@@ -130,19 +131,25 @@ struct W4Args {
     uint32_t zero_at, zero_mask, zero_else;     // place of the zero points in a record, or (mask 0) of anything, and what stands in for them
 };
 
-enum { W4_BF16 = 0, W4_F16 = 1, W4_F32 = 2, W4_I8 = 3 };      // type of x
+enum { W4_BF16 = 0, W4_F16 = 1, W4_F32 = 2, W4_I8 = 3, W4_BF16_TO_F32 = 4, W4_F16_TO_F32 = 5 };      // type of x (and, of 16 bits, of y)
+constexpr bool w4_half(int x) { return x == W4_F16 || x == W4_F16_TO_F32; }
+// Weights as q - z themselves: f32 rows, and 16-bit rows whose result keeps 32 bits. (16 + q) would leave it the rounding of terms that are 16 times and more as
+// large where large values of x meet small weights; a 16-bit result rounds that away. 14336 x 4096, f32 result, 16 + q / q - z (us): one fp16 row 8.0 / 8.1, 64
+// fp16 rows 19.9 / 18.2; one bf16 row 8.1 / 10.2, 64 bf16 rows 19.9 / 21.2 (no packed subtraction in bf16).
+constexpr bool w4_exact(int x) { return x == W4_F32 || x == W4_BF16_TO_F32 || x == W4_F16_TO_F32; }
 
 // One lane's 8 neighbouring inputs of one row as matrix operands: one for 16-bit types and int8, three for f32.
 template <int X> struct XFrag;
 template <> struct XFrag<W4_BF16> { static constexpr int P = 1; using E = __bf16; u32x4 v[1]; };
 template <> struct XFrag<W4_F16> { static constexpr int P = 1; using E = _Float16; u32x4 v[1]; };
 template <> struct XFrag<W4_F32> { static constexpr int P = 3; using E = float; u32x4 v[3]; };
+template <> struct XFrag<W4_BF16_TO_F32> : XFrag<W4_BF16> {};
+template <> struct XFrag<W4_F16_TO_F32> : XFrag<W4_F16> {};
 template <> struct XFrag<W4_I8> { static constexpr int P = 1; using E = int8_t; u32x2 v[1]; };
 
 template <int X>
 __device__ __forceinline__ void x_convert(XFrag<X> &f, const typename XFrag<X>::E (&e)[8]) {
-    if constexpr (X == W4_BF16 || X == W4_F16) __builtin_memcpy(&f.v[0], e, 16);
-    else if constexpr (X == W4_F32) {
+    if constexpr (X == W4_F32) {
         uint32_t u[3][8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -156,7 +163,8 @@ __device__ __forceinline__ void x_convert(XFrag<X> &f, const typename XFrag<X>::
         for (int p = 0; p < 3; ++p)
 #pragma unroll
             for (int i = 0; i < 4; ++i) f.v[p][i] = __builtin_amdgcn_perm(u[p][2 * i + 1], u[p][2 * i], 0x07060302u);     // the high halves of two words
-    } else {
+    } else if constexpr (X != W4_I8) __builtin_memcpy(&f.v[0], e, 16);
+    else {
         // in the order in which a word of 4-bit numbers leaves its bytes: 0 4 1 5 | 2 6 3 7
         uint32_t lo, hi;
         __builtin_memcpy(&lo, e, 4);
@@ -221,14 +229,25 @@ __device__ __forceinline__ WFrag<X> w_expand(uint32_t w) {
     }
     return f;
 }
-// f32 rows: the weights' own numbers q - z (exact in bf16), so that nothing cancels; zero = 16 + z of the lane's output
-__device__ __forceinline__ WFrag<W4_F32> w_expand_exact(uint32_t w, float zero) {
-    const WFrag<W4_F32> f = w_expand<W4_F32>(w);
-    WFrag<W4_F32> r;
+// the weights' own numbers q - z (exact in bf16 and fp16), so that nothing cancels; zero = 16 + z of the lane's output
+template <int X>
+__device__ __forceinline__ WFrag<X> w_expand_exact(uint32_t w, float zero) {
+    WFrag<X> r;
+    if constexpr (w4_half(X)) {
+        const WFrag<W4_F16> f = w_expand<W4_F16>(w);
+        const f16x2 z = {(_Float16)zero, (_Float16)zero};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float lo = __uint_as_float(f.v[i] << 16) - zero, hi = __uint_as_float(f.v[i] & 0xFFFF0000u) - zero;
-        r.v[i] = __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t pair = f.v[i];          // (a bit cast of a vector's element itself takes the first one)
+            r.v[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, pair) - z);
+        }
+    } else {
+        const WFrag<W4_BF16> f = w_expand<W4_BF16>(w);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float lo = __uint_as_float(f.v[i] << 16) - zero, hi = __uint_as_float(f.v[i] & 0xFFFF0000u) - zero;
+            r.v[i] = __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+        }
     }
     return r;
 }
@@ -244,7 +263,7 @@ template <> struct Acc<W4_I8> { using V = i32x4; };
 template <int X>
 __device__ __forceinline__ typename Acc<X>::V mma(const WFrag<X> &a, const XFrag<X> &b, typename Acc<X>::V c) {
     if constexpr (X == W4_I8) return __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, a.v), __builtin_bit_cast(long, b.v[0]), c, 0, 0, 0);
-    else if constexpr (X == W4_F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a.v), __builtin_bit_cast(f16x8, b.v[0]), c, 0, 0, 0);
+    else if constexpr (w4_half(X)) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a.v), __builtin_bit_cast(f16x8, b.v[0]), c, 0, 0, 0);
     else {
 #pragma unroll
         for (int p = XFrag<X>::P - 1; p >= 0; --p) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a.v), __builtin_bit_cast(bf16x8, b.v[p]), c, 0, 0, 0);
@@ -256,7 +275,7 @@ __device__ __forceinline__ typename Acc<X>::V mma(const WFrag<X> &a, const XFrag
 template <int X, int GROUP, int MT, int NT>
 struct Block {
     static constexpr int PER = W4_TK / GROUP, STEPS = GROUP / 32;       // groups of a record; steps of 32 inputs of a group
-    static constexpr bool EXACT = X == W4_F32;
+    static constexpr bool EXACT = w4_exact(X);
     u32x4 w[NT];
     u32x2 s[NT][PER];
     uint32_t z[NT][PER];
@@ -285,7 +304,7 @@ struct Block {
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
                 sum[i] = V{0, 0, 0, 0};
-                if constexpr (!OWN) sum[i][0] = total(g, i);
+                if constexpr (!OWN && !EXACT) sum[i][0] = total(g, i);
 #pragma unroll
                 for (int j = 0; j < NT; ++j) d[j][i] = V{0, 0, 0, 0};
             }
@@ -297,7 +316,7 @@ struct Block {
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
                     WFrag<X> wf;
-                    if constexpr (EXACT) wf = w_expand_exact(w[j][t], (float)(z[j][g] & 255u));
+                    if constexpr (EXACT) wf = w_expand_exact<X>(w[j][t], (float)(z[j][g] & 255u));
                     else wf = w_expand<X>(w[j][t]);
 #pragma unroll
                     for (int i = 0; i < MT; ++i) d[j][i] = mma<X>(wf, x[i], d[j][i]);
@@ -305,6 +324,7 @@ struct Block {
                 if constexpr (!EXACT && OWN)
 #pragma unroll
                     for (int i = 0; i < MT; ++i) sum[i] = mma<X>(w_ones<X>(), x[i], sum[i]);
+                if constexpr (X == W4_F16_TO_F32 && GROUP == 64 && MT == 4) __builtin_amdgcn_sched_barrier(0);          // (registers for one step's operands: with two's some spill)
             }
             if constexpr (PER > 1) __builtin_amdgcn_sched_barrier(0);          // (groups one after another: side by side they would only cost registers)
 #pragma unroll
@@ -366,7 +386,7 @@ __device__ __forceinline__ void finish(const W4Args &a, const f32x4 (&acc)[NT][M
 // outputs 4 (lane >> 4) .. + 3. U blocks are asked for before the first is multiplied; with U = 1 the next one is on its way meanwhile.
 // FEW: there are no more rows than one piece a lane covers (2, 4 or 8 by type): the others' columns hold whatever LDS held, and are not written.
 template <int X, int GROUP, int MT, int NT, int U, bool FEW>
-__global__ __launch_bounds__(512, FEW && GROUP != 32 ? 6 : MT == 1 && (FEW || X != W4_F32 || GROUP == 128) ? 4 : 2) void w4_dense_kernel(const W4Args a) {
+__global__ __launch_bounds__(512, FEW && GROUP != 32 && (X == W4_F32 || !w4_exact(X)) ? 6 : MT == 1 && (FEW || X != W4_F32 || GROUP == 128) ? 4 : 2) void w4_dense_kernel(const W4Args a) {
     using P = Piece<X>;
     using E = typename P::E;
     constexpr int STEP = 64 / P::PLACES, PIECES = FEW ? 1 : MT * 16 / STEP, TILE = MT * 16 * P::ROW;         // rows between a lane's pieces of a block, their number
@@ -466,6 +486,7 @@ __global__ __launch_bounds__(512, 2) void w4_dense_shared_kernel(const W4Args a)
     auto store = [&](const u32x4 (&v)[N], int half) {
 #pragma unroll
         for (int i = 0; i < N; ++i) P::store(xs + half * TILE, i * STEP + piece_row, piece_place, v[i]);
+        if constexpr (w4_exact(X)) return;
         wave_lds_order();
 #pragma unroll
         for (int c = 0; c < MINE; c += COLS)
@@ -757,8 +778,13 @@ int shodh_w4_dense_device(const shodh_w4_weight *w, const void *d_x, uint32_t x_
     for (uint64_t r = 0; r < rows; r += turn) {
         a.x = (const uint8_t *)d_x + r * xs * xb; a.y = (uint8_t *)d_y + r * ys * yb; a.x_scale = d_x_scale ? d_x_scale + r : nullptr;
         a.M = (uint32_t)(rows - r < turn ? rows - r : turn);
-        SHODH_TRY(x_dtype == SHODH_DTYPE_BF16 ? pick_w4<W4_BF16>(a, w, st) : x_dtype == SHODH_DTYPE_FP16 ? pick_w4<W4_F16>(a, w, st) : x_dtype == SHODH_DTYPE_FP32 ? pick_w4<W4_F32>(a, w, st) :
-                                                                                                                                                                   pick_w4<W4_I8>(a, w, st));
+        const bool wide = y_dtype == SHODH_DTYPE_FP32;
+        switch (x_dtype) {
+            case SHODH_DTYPE_BF16: SHODH_TRY(wide ? pick_w4<W4_BF16_TO_F32>(a, w, st) : pick_w4<W4_BF16>(a, w, st)); break;
+            case SHODH_DTYPE_FP16: SHODH_TRY(wide ? pick_w4<W4_F16_TO_F32>(a, w, st) : pick_w4<W4_F16>(a, w, st)); break;
+            case SHODH_DTYPE_FP32: SHODH_TRY(pick_w4<W4_F32>(a, w, st)); break;
+            default: SHODH_TRY(pick_w4<W4_I8>(a, w, st));
+        }
     }
     return SHODH_OK;
 }

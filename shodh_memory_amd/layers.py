@@ -205,7 +205,8 @@ class W4Weight:
 
     def dense(self, x, x_scale=None, bias=None, out_dtype=None, out=None, stream=None):
         """x [..., K] -> [..., N]: x @ W^T (* x_scale per row) + bias. x fp32, bf16, fp16, or int8 with x_scale f32 [rows] (or [rows, 1]);
-        the result is of x's type (bf16 for int8 rows) unless out_dtype or `out` says otherwise."""
+        the result is of x's type (bf16 for int8 rows) unless out_dtype or `out` says otherwise. A row that holds a NaN or an infinity gives NaN in all its
+        outputs (16-bit rows with an f32 result: what the formula gives)."""
         if self._h is None:
             _refuse("the weight is closed", L.ERR_STATE)
         if stream is not None:

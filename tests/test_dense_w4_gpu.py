@@ -421,3 +421,25 @@ def test_f32_rows_against_the_definition_without_the_16s(layers, group):
             off = (w.dense(x).cpu().double() - y).abs()
             tol = (3 * group + -(-k // group) + 16) * U * t + U / 2 * y.abs()
             assert (off <= tol).all(), float((off / tol).max())
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16", "f32", "int8"])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("m,n,k", [(1, 50, 1000), (4, 33, 384), (16, 100, 700), (33, 40, 513), (64, 9000, 384), (20, 17000, 257), (49, 30000, 300)])
+def test_large_values_that_meet_no_weight(layers, kind, group, m, n, k):
+    """every other input is huge, its weights are 0 (q = z); the others are whole numbers that f32 adds up exactly: an f32 result is that sum, without a trace of
+    the rounding of the large ones. (|sum| <= 1000 / 2 x 120 x 15 < 2^24, scale 1)"""
+    g = torch.Generator().manual_seed(m + group)
+    z = torch.randint(0, 16, (n, -(-k // group)), generator=g, dtype=torch.uint8)
+    q = torch.randint(0, 16, (n, k), generator=g, dtype=torch.uint8)
+    q[:, ::2] = z.repeat_interleave(group, 1)[:, :k:2]
+    p = torch.nn.functional.pad(q, (0, k % 2))
+    w = layers.W4Weight.from_quantized((p[:, 0::2] | (p[:, 1::2] << 4)).cuda(), torch.ones(n, z.shape[1], device="cuda"), z.cuda(), k=k, group=group)
+    x = torch.randint(-120, 121, (m, k), generator=g).float()
+    want = x[:, 1::2].double() @ (q.double() - z.repeat_interleave(group, 1)[:, :k].double())[:, 1::2].t()
+    x[:, ::2] = {"bf16": 2.0 ** 40, "f16": 2.0 ** 15, "f32": 2.0 ** 40, "int8": 127}[kind]
+    if kind == "int8":
+        got = w.dense(x.to(torch.int8).cuda(), x_scale=torch.ones(m, device="cuda"), out_dtype=torch.float32)
+    else:
+        got = w.dense(x.to(TYPES[kind]).cuda(), out_dtype=torch.float32)
+    assert torch.equal(got.cpu().double(), want)
