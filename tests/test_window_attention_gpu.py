@@ -7,6 +7,7 @@ step h = eps(type) / 2 relative (fp16: or 2^-25, half its smallest step, of the 
     |out - exact| <= (h + 2 e + 80 u (1 + n / 4096)) sum p |v| + [fp16] n 2^-25 max |v| + h |exact|
 lse is off by at most e + 80 u + u |lse|."""
 import math
+import os
 
 import pytest
 import torch
@@ -386,6 +387,9 @@ def test_what_a_dominant_sink_leaves_over(layers, dtype, above, lq, heads):
 
 
 def used_by(call):
+    """(result, most bytes of device memory taken meanwhile; 0 under the guard's allocator, which does not count them)"""
+    if os.environ.get("SHODH_GUARD", "0") not in ("", "0"):
+        return call(), 0
     torch.cuda.synchronize()
     before = torch.cuda.memory_allocated()
     torch.cuda.reset_peak_memory_stats()
@@ -453,3 +457,42 @@ def test_numbers_that_32_bits_cannot_hold(layers):
         with pytest.raises(ShodhError):
             layers.window_attention(q, k, v, cu, **kw)
     torch.cuda.synchronize()
+
+
+def test_sequences_out_of_order_and_their_parts(layers):
+    """a cu that is not rising: rows that one sequence alone claims are right, nothing outside them is touched"""
+    q, k, v = normal(80, 6, 8, 128).bfloat16(), normal(81, 9000, 1, 128).bfloat16(), normal(82, 9000, 1, 128).bfloat16()
+    start = torch.zeros(4, dtype=torch.int64, device="cuda")
+    length = torch.full((4,), 9000, dtype=torch.int32, device="cuda")
+    good = layers.window_attention(q, k, v, cu_of([4, 0, 0, 0]), kv_start=start, kv_len=length)
+    for order in ([0, 4, 1, 2, 2], [0, 4, 0, -3, 9], [0, 4, 2, 3, 1]):
+        out = torch.full_like(q, 5.0)
+        layers.window_attention(q, k, v, torch.tensor(order, dtype=torch.int32, device="cuda"), kv_start=start, kv_len=length, out=out)
+        assert torch.equal(out[0], good[0]) and torch.equal(out[3], good[3]) and (out[4:] == 5).all(), order
+    torch.cuda.synchronize()
+
+
+@needs_capture
+def test_a_graph_whose_lengths_need_larger_parts(layers):
+    """how many parts there are is found anew in every run: lengths that grow and shrink between replays, of a capture made at any of them"""
+    seqs, heads, kv, dim, nk = 400, 32, 4, 128, 2500
+    q, k, v = normal(83, seqs, heads, dim).bfloat16(), normal(84, nk, kv, dim).bfloat16(), normal(85, nk, kv, dim).bfloat16()
+    start, cu = torch.zeros(seqs, dtype=torch.int64, device="cuda"), cu_of([1] * seqs)
+    length = torch.full((seqs,), 40, dtype=torch.int32, device="cuda")
+
+    def call():
+        return layers.window_attention(q, k, v, cu, kv_start=start, kv_len=length, return_lse=True)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = call()
+    for i, n in enumerate((2500, 40, 1300, 0, 2500)):
+        length.fill_(n)
+        length[i::7] = 2500 - n
+        want = call()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(held[0], want[0]) and torch.equal(held[1], want[1]), n
+        at = length == n
+        check(want[0][at][:64], want[1][at][:64], exact(q[at][:64], k, v, [64], [n], -1, -1, 0, [0]))
