@@ -606,7 +606,7 @@ __global__ __launch_bounds__(256, 2) void attn_split_kernel(const AttnArgs a) {
     auto wanted = [&](const Seq &s) {
         int64_t seen = s.nk;
         if (a.left >= 0 && a.right >= 0) seen = min(seen, (int64_t)a.left + a.right + 1 + BM + 64 + (int64_t)a.sinks);
-        return (uint32_t)min((int64_t)a.splits, max((int64_t)1, ((seen + 31) / 32 + a.chunk - 1) / a.chunk));
+        return min(a.splits, max(1u, ((uint32_t)((seen + 31) >> 5) + a.chunk - 1) / a.chunk));
     };
     auto places = [&](const Seq &s, uint32_t parts) { return parts > 1 ? (uint32_t)min((int64_t)s.nq * a.group * parts, (int64_t)MOST) : 0u; };
     if (a.coarser) {                               // (every workgroup finds the same number)
@@ -626,26 +626,41 @@ __global__ __launch_bounds__(256, 2) void attn_split_kernel(const AttnArgs a) {
         }
         __syncthreads();
     } else if (wave == 0) table.fewer = 1;
-    auto running = [&](uint32_t x) {               // sum over the lanes up to this one
+    auto running = [&](auto &x) {                  // sums over the lanes up to this one, side by side
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) { const uint32_t v = (uint32_t)__shfl_up((int)x, o); if (lane >= o) x += v; }
-        return x;
+        for (int o = 1; o < 64; o <<= 1)
+#pragma unroll
+            for (uint32_t &v : x) { const uint32_t u = (uint32_t)__shfl_up((int)v, o); v += lane >= o ? u : 0u; }
     };
     auto count = [&](int base) {          // by wave 0; the items of 64 sequences
         const int b = base + lane;
         Seq s = {0, 0, 0, 0};
         if (b < (int)a.seqs) s = seq_at(a, b, a.cu[b], a.cu[b + 1]);
         const int64_t rows = (int64_t)s.nq * a.group;
-        uint32_t parts = 1;
+        const uint32_t tiles = (uint32_t)((rows + BM - 1) / BM);          // (below 2^26: 64 times that fits)
+        uint32_t parts = 1, items = tiles, end;
         if (a.splits > 1) {
-            parts = (wanted(s) + table.fewer - 1) / table.fewer;
-            const uint32_t p = places(s, parts), p_end = (base ? table.parts_before : 0u) + running(p);
-            if (p_end > a.room) parts = 1;         // (only where cu is out of order)
-            const uint32_t r = parts > 1 ? (uint32_t)rows : 0u, r_end = (base ? table.rows_before : 0u) + running(r);
+            parts = table.fewer == 1 ? wanted(s) : (wanted(s) + table.fewer - 1) / table.fewer;
+            const uint32_t p = places(s, parts);
+            uint32_t r = parts > 1 ? (uint32_t)rows : 0u;
+            items = tiles * parts;
+            uint32_t sums[3] = {p, r, items};
+            running(sums);
+            const uint32_t p_end = (base ? table.parts_before : 0u) + sums[0];
+            if (__any(p_end > a.room)) {           // (only where cu is out of order: what has no places is not cut)
+                if (p_end > a.room) { parts = 1; r = 0; items = tiles; }
+                sums[1] = r; sums[2] = items;
+                running(sums);
+            }
+            const uint32_t r_end = (base ? table.rows_before : 0u) + sums[1];
+            end = sums[2];
             table.first[lane] = p_end - p; table.listed[lane] = r_end - r;
             if (lane == 63) { table.parts_before = min(p_end, MOST); table.rows_before = r_end; }
+        } else {
+            uint32_t sums[1] = {items};
+            running(sums);
+            end = sums[0];
         }
-        const uint32_t items = (uint32_t)((rows + BM - 1) / BM) * parts, end = running(items);          // (rows / 32 < 2^26 - 64 or so: 64 of them fit)
         table.q0[lane] = s.q0; table.k0[lane] = s.k0; table.nq[lane] = s.nq; table.nk[lane] = s.nk; table.parts[lane] = (int)parts;
         table.begin[lane] = end - items; table.end[lane] = end;
     };
