@@ -1,7 +1,8 @@
 """Layer operators of a text tower on torch device tensors, over the C ABI (include/shodh_hip.h, "layer operators"): RMS norm with residual and 8-bit
 output, dense layers on 4-bit weights, attention with a sliding window and always-visible first tokens. They run on the tensors' device, on its
 current stream unless `stream` names another (a raw hipStream_t, made the current one for the call: new tensors are that stream's), and can be captured
-into a graph. They are for inference: results carry no gradients. Nothing here computes on the host."""
+into a graph. They are for inference: results carry no gradients, and inputs that require one are refused while torch records (torch.no_grad() takes them).
+Nothing here computes on the host."""
 import collections
 import ctypes as C
 import functools
@@ -25,6 +26,11 @@ def _u32(code=L.ERR_UNSUPPORTED, **sizes):
     for name, n in sizes.items():
         if not 0 <= n < 2 ** 32:
             _refuse("%s %d is no 32-bit number" % (name, n), code)
+
+
+def _gradient():
+    if torch.is_grad_enabled():
+        _refuse("an input requires a gradient, which a layer operator does not give: call it under torch.no_grad()", L.ERR_UNSUPPORTED)
 
 
 def _dtype(t, name):
@@ -94,6 +100,8 @@ def rms_norm(x, weight, eps=1e-6, residual=None, want_y=True, quant=None, group=
             return rms_norm(x, weight, eps, residual, want_y, quant, group, sum_out)
     if device.type != "cuda":
         _refuse("x is on %s: there is no CPU fallback" % device, L.ERR_DEVICE)
+    if x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad) or (sum_out is not None and sum_out.requires_grad):
+        _gradient()
     dt = _dtype(x, "x")
     rows, dim, xs = _matrix(x, "x")
     if dim >= 2 ** 32 or not 0 <= group < 2 ** 32:
@@ -212,6 +220,8 @@ class W4Weight:
         if stream is not None:
             with _current(stream, self.device):
                 return self.dense(x, x_scale, bias, out_dtype, out)
+        if x.requires_grad or (bias is not None and bias.requires_grad) or (x_scale is not None and x_scale.requires_grad) or (out is not None and out.requires_grad):
+            _gradient()
         rows, k, xs = _matrix(x, "x")
         if k != self.k:
             _refuse("x has %d columns, the weight %d inputs" % (k, self.k), L.ERR_DIM)
@@ -302,6 +312,8 @@ def window_attention(q, k, v, cu, left=-1, right=-1, sinks=0, kv_start=None, kv_
             return window_attention(q, k, v, cu, left, right, sinks, kv_start, kv_len, scale, return_lse, out)
     if device.type != "cuda":
         _refuse("q is on %s: there is no CPU fallback" % device, L.ERR_DEVICE)
+    if q.requires_grad or k.requires_grad or v.requires_grad or (out is not None and out.requires_grad):
+        _gradient()
     dt = _dtype(q, "q")
     qs, qh = _heads(q, "q", device, q.dtype)
     ks, kh = _heads(k, "k", device, q.dtype)

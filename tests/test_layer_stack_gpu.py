@@ -129,3 +129,27 @@ def test_a_block_on_texts_then_on_single_tokens(layers, dtype, captured):
         assert torch.equal(eager["n3"].y, held["n3"].y) and torch.equal(eager["n3"].sum, held["n3"].sum)
         length += 1
         torch.cuda.synchronize()
+
+
+def test_inputs_that_require_a_gradient(layers):
+    """no gradient is lost without a word: such inputs are refused while torch records, and taken where it does not"""
+    from shodh_memory_amd import ShodhError
+    w4 = layers.W4Weight.quantize(torch.randn(32, 64), group=32)
+    x, g, bias = torch.randn(4, 64, device="cuda"), torch.ones(64, device="cuda"), torch.zeros(32, device="cuda")
+    q, k, v, cu = ATTN.normal(1, 4, 2, 32).half(), ATTN.normal(2, 4, 1, 32).half(), ATTN.normal(3, 4, 1, 32).half(), ATTN.cu_of([4])
+
+    def leaf(t):
+        return t.clone().requires_grad_()
+    calls = [lambda: layers.rms_norm(leaf(x), g).y, lambda: layers.rms_norm(x, torch.nn.Parameter(g)).y, lambda: layers.rms_norm(x, g, residual=leaf(x)).y, lambda: w4.dense(leaf(x)), lambda: w4.dense(x, bias=leaf(bias)),
+             lambda: w4.dense((2 * leaf(x)).half()), lambda: layers.window_attention(leaf(q), k, v, cu), lambda: layers.window_attention(q, leaf(k), v, cu), lambda: layers.window_attention(q, k, leaf(v), cu)]
+    plain = [layers.rms_norm(x, g).y, layers.rms_norm(x, g).y, layers.rms_norm(x, g, residual=x).y, w4.dense(x), w4.dense(x, bias=bias), w4.dense((2 * x).half())] + [layers.window_attention(q, k, v, cu)] * 3
+    for call, want in zip(calls, plain):
+        with pytest.raises(ShodhError):
+            call()
+        with torch.no_grad():
+            assert torch.equal(call(), want)
+        with torch.inference_mode():
+            assert torch.equal(call(), want)
+    for call in [lambda: layers.rms_norm(x, g, residual=x, sum_out=leaf(x)), lambda: w4.dense(x, out=leaf(x[:, :32])), lambda: layers.window_attention(q, k, v, cu, out=leaf(q))]:
+        with pytest.raises(ShodhError):
+            call()
