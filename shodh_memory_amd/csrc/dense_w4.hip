@@ -2,8 +2,9 @@
 //
 //   y[m][n] = (sum_k x[m][k] * (q[n][k] - z[n][g]) * s[n][g]) * x_scale[m] + bias[n],   g = k / group, q and z in 0 .. 15
 //
-// Bound: the weights' bytes (half a byte a weight) for up to 16 rows; a launch for small layers; the making of operands for 64 rows (28672 x 4096, bf16:
-// 27 us, 65 MB at 2.4 TB/s; matrix unit 30 % busy, vector unit 52 %). One fp16 row x 14336 x 4096: 8.8 us with the call, 31 MB at 3.5 TB/s.
+// Bound: the weights' bytes (half a byte a weight) for up to 16 rows; a launch for small layers; waits for 64 rows (28672 x 4096, bf16: 28 us, 65 MB at 2.3 TB/s:
+// CUs are busy for 65 % of it -- 224 workgroups for 256 CUs, a barrier a block -- and in that the vector unit for 52 %, the matrix unit for 30 %). One fp16 row
+// x 14336 x 4096: 8.8 us with the call where the last-level cache holds the 31 MB of weights, 10.3 (3.0 TB/s) where they come from HBM.
 // Everything follows from that:
 //  * weights are laid out once, in records of 16 outputs x 128 inputs (1 KiB of 4-bit numbers, 16 B a lane, then the record's scales and zero
 //    points): a wave's load of a record is one contiguous KiB and lands where the matrix instruction wants it;

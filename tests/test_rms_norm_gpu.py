@@ -218,3 +218,34 @@ def test_sizes_that_32_bits_cannot_hold(layers):
     with pytest.raises(ShodhError):
         layers.rms_norm(wide[None], wide)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,dim", [(300, 64), (5, 1000), (40, 4096), (3, 20000)])
+def test_in_place_through_the_c_boundary(layers, dtype, rows, dim):
+    """sum and y over x or the residual themselves, element for element; any other overlap is refused and leaves what was there"""
+    import ctypes as C
+
+    from shodh_memory_amd import _lib as L
+    t = TYPES[dtype]
+    x0, r0 = (torch.randn(rows, dim, generator=torch.Generator(device="cuda").manual_seed(i), device="cuda").to(t) for i in (1, 2))
+    w = torch.rand(dim, device="cuda").to(t)
+    want = layers.rms_norm(x0, w, residual=r0)
+    kind = {"f32": L.DTYPE_FP32, "bf16": L.DTYPE_BF16}[dtype]
+    cfg = L.RmsNormCfg(rows, 0, 0, 0, 0, 0, dim, kind, kind, L.DTYPE_INT8, 0, 1e-6)
+
+    def call(x, r, total, y):
+        return L.lib().shodh_rms_norm_device(0, C.byref(cfg), x.data_ptr(), r.data_ptr(), w.data_ptr(), total, y, None, None, torch.cuda.current_stream().cuda_stream)
+    for total_at, y_at in (("r", "x"), ("x", "r"), ("r", None), (None, "x"), (None, "r"), ("x", "new")):
+        x, r, new = x0.clone(), r0.clone(), torch.empty_like(x0)
+        at = {"x": x, "r": r, "new": new}
+        assert call(x, r, at[total_at].data_ptr() if total_at else None, at[y_at].data_ptr() if y_at else None) == 0
+        if total_at:
+            assert torch.equal(at[total_at], want.sum)
+        if y_at:
+            assert torch.equal(at[y_at], want.y)
+    x, r = x0.clone(), r0.clone()
+    one = x.element_size()
+    assert call(x, r, x.data_ptr(), x.data_ptr()) == L.ERR_INVALID and call(x, r, r.data_ptr() + one, None) == L.ERR_INVALID and call(x, r, None, x.data_ptr() + dim * one) == L.ERR_INVALID
+    torch.cuda.synchronize()
+    assert torch.equal(x, x0) and torch.equal(r, r0)
