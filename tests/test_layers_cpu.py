@@ -186,8 +186,8 @@ QKV = dict(q=X, k=X + 512, v=X + 768, q_stride=512, k_stride=512, v_stride=512)
     (True, dict(q=X, k=X + 4096, v=X + 6144, out=X)), (False, dict(q=X, k=X + 4096, v=X + 6144, out=X + 128)), (False, dict(out=2 * X, lse=2 * X + 4092)), (True, dict(out=2 * X, lse=2 * X + 4096)), (False, dict(out=2 * X, lse=X)),
     (False, dict(out=2 * X, lse=3 * X, cu=3 * X + 4)), (False, dict(out=2 * X, cu=2 * X + 4)), (False, dict(out=2 * X, start=2 * X + 8, length=P)),
     # head by head: q, k, v and out of a head one after another, and each other head's place in between
-    (True, dict(kv_heads=4, q=X, k=X + 1024, v=X + 2048, out=X + 3072, q_stride=64, k_stride=64, v_stride=64, out_stride=64, q_head_stride=2048, k_head_stride=2048, v_head_stride=2048, out_head_stride=2048)),
-    (False, dict(kv_heads=4, q=X, k=X + 1024, v=X + 2048, out=X + 3070, q_stride=64, k_stride=64, v_stride=64, out_stride=64, q_head_stride=2048, k_head_stride=2048, v_head_stride=2048, out_head_stride=2048))])
+    (True, dict(kv_heads=4, q=X, k=X + 1024, v=X + 2048, out=X + 2048 + 1024, q_stride=64, k_stride=64, v_stride=64, out_stride=64, q_head_stride=2048, k_head_stride=2048, v_head_stride=2048, out_head_stride=2048)),
+    (False, dict(kv_heads=4, q=X, k=X + 1024, v=X + 2048, out=X + 2048 + 1022, q_stride=64, k_stride=64, v_stride=64, out_stride=64, q_head_stride=2048, k_head_stride=2048, v_head_stride=2048, out_head_stride=2048))])
 def test_attention_outputs_that_overlap(L, taken, kw):
     if torch.cuda.is_available():
         pytest.skip("pointers of no memory")
